@@ -64,6 +64,9 @@ SIGNATURES = {
     "bpt_tile_plan_device_export": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp]),
     "bpt_tile_plan_device_destroy": (None, [_vp]),
     "bpt_add_layer_norm": (_int, [_vp, _vp, _vp, _vp, _dbl, _vp, _i64, _int, _int, _vp]),
+    "bpt_layer_norm_forward": (_int, [_vp, _vp, _vp, _vp, _dbl, _vp, _vp, _vp, _i64, _int, _int, _vp]),
+    "bpt_layer_norm_backward_workspace_bytes": (_sz, [_i64, _int]),
+    "bpt_layer_norm_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _vp, _sz, _vp]),
     "bpt_dense_blocks_fill": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp]),
     "bpt_export_in_csr": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp]),
     "bpt_export_out_csr": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp]),

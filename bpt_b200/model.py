@@ -19,44 +19,19 @@ import math
 import torch
 import torch.nn as nn
 
-from . import _lib
 from .attention import bpt_attention
-
-
-class _AddLayerNorm(torch.autograd.Function):
-    """y = LayerNorm(x + r) through bpt_add_layer_norm (one pass over memory).  The backward
-    recomputes the sum and goes through torch's layer-norm derivative."""
-
-    @staticmethod
-    def forward(ctx, x, r, weight, bias, eps):
-        y = torch.empty_like(x)
-        with torch.cuda.device(x.device):
-            _lib.check(_lib.lib().bpt_add_layer_norm(x.data_ptr(), r.data_ptr(), weight.data_ptr(), bias.data_ptr(),
-                                                     float(eps), y.data_ptr(), x.numel() // x.size(-1), x.size(-1),
-                                                     _lib.dtype_code(x.dtype), _lib.stream()))
-        ctx.save_for_backward(x, r, weight, bias)
-        ctx.eps = eps
-        return y
-
-    @staticmethod
-    def backward(ctx, gy):
-        x, r, weight, bias = ctx.saved_tensors
-        with torch.enable_grad():
-            s = (x + r).detach().requires_grad_(True)
-            w, b = weight.detach().requires_grad_(True), bias.detach().requires_grad_(True)
-            out = nn.functional.layer_norm(s, (s.size(-1),), w, b, ctx.eps)
-            gs, gw, gb = torch.autograd.grad(out, (s, w, b), gy)
-        return gs, gs, gw, gb, None
+from .norm import layer_norm
 
 
 def add_layer_norm(x, r, norm):
-    """norm(x + r) for an nn.LayerNorm over the last dimension; fused on CUDA when the kernel's
-    shape rules hold (same dtype everywhere, last dimension a multiple of 8 up to 4096)."""
+    """norm(x + r) for an nn.LayerNorm over the last dimension; fused on CUDA, forward and backward (norm.py), when
+    the rules of the kernel of a warp per row hold (same dtype everywhere, last dimension a multiple of 8 up to 4096),
+    torch's operators otherwise.  `norm.layer_norm` itself takes every width up to 8192."""
     dim = x.size(-1)
     if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16, torch.float16) and dim % 8 == 0 and dim <= 4096
             and norm.weight is not None and norm.bias is not None and norm.weight.dtype == x.dtype
             and r.dtype == x.dtype and r.shape == x.shape and tuple(norm.normalized_shape) == (dim,)):
-        return _AddLayerNorm.apply(x.contiguous(), r.contiguous(), norm.weight, norm.bias, norm.eps)
+        return layer_norm(x, norm.weight, norm.bias, norm.eps, residual=r)
     return norm(x + r)
 
 

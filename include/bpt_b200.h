@@ -487,6 +487,21 @@ int bpt_attn_forward_static(const void *plan, const int32_t *counts_host, int64_
 int bpt_add_layer_norm(const void *x, const void *r, const void *gamma, const void *beta, double eps, void *y,
                        int64_t n_rows, int dim, int dtype, bpt_stream_t stream);
 
+/* The same for any dim from 1 to 8192 and any alignment, for training: mean and rstd (fp32, one per row; both or
+ * neither may be NULL) are what bpt_layer_norm_backward reads.  Where bpt_add_layer_norm takes the arguments too,
+ * y is the same bit for bit.  No counterpart in the reference, which spells it with torch operators.
+ *
+ * bpt_layer_norm_backward: gy: gradient of y; x, r (may be NULL), gamma (may be NULL: ones), mean, rstd as in the
+ * forward.  da: gradient of x + r, that is of x and of r; dgamma, dbeta (dim): sums over the rows.  Each of the three
+ * may be NULL to skip it.  All of `dtype`, sums in fp32 in a fixed order (bitwise reproducible).  The workspace is
+ * needed for dgamma and dbeta only, nothing in it has to be zero. */
+int bpt_layer_norm_forward(const void *x, const void *r, const void *gamma, const void *beta, double eps, void *y,
+                           float *mean, float *rstd, int64_t n_rows, int dim, int dtype, bpt_stream_t stream);
+size_t bpt_layer_norm_backward_workspace_bytes(int64_t n_rows, int dim);
+int bpt_layer_norm_backward(const void *gy, const void *x, const void *r, const void *gamma, const float *mean,
+                            const float *rstd, void *da, void *dgamma, void *dbeta, int64_t n_rows, int dim,
+                            int dtype, void *workspace, size_t workspace_bytes, bpt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
