@@ -67,6 +67,12 @@ SIGNATURES = {
     "bpt_layer_norm_forward": (_int, [_vp, _vp, _vp, _vp, _dbl, _vp, _vp, _vp, _i64, _int, _int, _vp]),
     "bpt_layer_norm_backward_workspace_bytes": (_sz, [_i64, _int]),
     "bpt_layer_norm_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _vp, _sz, _vp]),
+    "bpt_linear_ce_forward_workspace_bytes": (_sz, [_vp, _i64, _vp, _i64, _i64, _int, _int, _int]),
+    "bpt_linear_ce_forward": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _dbl, _int, _vp, _vp, _vp, _i64, _int, _int, _int,
+                                     _vp, _sz, _vp]),
+    "bpt_linear_ce_backward_workspace_bytes": (_sz, [_vp, _i64, _vp, _i64, _i64, _int, _int, _int, _int, _int, _int]),
+    "bpt_linear_ce_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _dbl, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                                      _int, _int, _int, _vp, _sz, _vp]),
     "bpt_dense_blocks_fill": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp]),
     "bpt_export_in_csr": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp]),
     "bpt_export_out_csr": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp]),

@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 
 from .attention import bpt_attention
+from .loss import linear_cross_entropy
 from .norm import layer_norm
 
 
@@ -151,6 +152,12 @@ class Generator(nn.Module):  # modules/model.py:8-17
     def forward(self, x):
         return torch.log_softmax(self.proj(x), dim=-1)
 
+    def loss(self, x, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+        """Cross entropy of forward(x) against target in one call that never holds the (rows, classes)
+        log-probabilities (loss.py)."""
+        return linear_cross_entropy(x, self.proj.weight, target, bias=self.proj.bias, ignore_index=ignore_index,
+                                    label_smoothing=label_smoothing, reduction=reduction)
+
 
 class Embedding(nn.Module):
     """modules/embedding.py:13-21: the token table sits in `.lut`, so its state-dict key is `<name>.lut.weight`
@@ -178,15 +185,24 @@ class BPTLanguageModel(nn.Module):
         self.norm = nn.LayerNorm(dim_model)
         self.emb_dropout = nn.Dropout(dropout)
 
-    def forward(self, tokens, leaf_ids, plan):
+    def features(self, tokens, leaf_ids, plan):
         """tokens: (n_leaves,) int64 in leaf order; leaf_ids: their node ids; plan.n_nodes nodes.
-        Returns log-probabilities (n_leaves, vocab)."""
+        Returns the leaves' features after the last block (n_leaves, dim_model)."""
         x = self.norm(self.emb_dropout(self.embed(tokens)))                     # model.py:249-262
         h = x.new_zeros((plan.n_nodes, x.size(-1)))                             # span nodes start at zero
         h[leaf_ids] = x
         for layer in self.layers:                                              # model.py:268-269
             h = layer(h, plan)
-        return self.generator(h[leaf_ids])                                      # model.py:275
+        return h[leaf_ids]
+
+    def forward(self, tokens, leaf_ids, plan):
+        """As `features`; returns log-probabilities (n_leaves, vocab)."""
+        return self.generator(self.features(tokens, leaf_ids, plan))            # model.py:275
+
+    def loss(self, tokens, leaf_ids, plan, target, **options):
+        """Cross entropy of forward(...) against target (n_leaves,), without the log-probabilities in memory
+        (lm.py:120-140 computes nll_loss of them).  options: ignore_index, label_smoothing, reduction."""
+        return self.generator.loss(self.features(tokens, leaf_ids, plan), target, **options)
 
 
 class BPTClassifier(nn.Module):
@@ -208,10 +224,10 @@ class BPTClassifier(nn.Module):
         self.norm = nn.LayerNorm(dim_model)
         self.emb_dropout = nn.Dropout(dropout)
 
-    def forward(self, tokens, leaf_ids, plan, root_ids, lengths=None):
+    def features(self, tokens, leaf_ids, plan, root_ids, lengths=None):
         """tokens: (n_leaves,) in leaf order; root_ids: (B,) node id of every sequence's root;
         lengths: (B,) leaves per sequence (needed for readout="mean"; leaves of a sequence are
-        contiguous in `tokens`).  Returns log-probabilities (B, n_classes)."""
+        contiguous in `tokens`).  Returns one vector per sequence (B, dim_model)."""
         x = self.norm(self.emb_dropout(self.embed(tokens)))
         h = x.new_zeros((plan.n_nodes, x.size(-1)))
         h[leaf_ids] = x
@@ -224,7 +240,15 @@ class BPTClassifier(nn.Module):
             pooled = torch.zeros((lengths.numel(), h.size(-1)), dtype=h.dtype, device=h.device)
             pooled.index_add_(0, seq, h[leaf_ids])
             pooled = pooled / lengths.to(h.dtype).unsqueeze(1)
-        return self.generator(pooled)
+        return pooled
+
+    def forward(self, tokens, leaf_ids, plan, root_ids, lengths=None):
+        """As `features`; returns log-probabilities (B, n_classes)."""
+        return self.generator(self.features(tokens, leaf_ids, plan, root_ids, lengths))
+
+    def loss(self, tokens, leaf_ids, plan, root_ids, target, lengths=None, **options):
+        """Cross entropy of forward(...) against target (B,).  options: ignore_index, label_smoothing, reduction."""
+        return self.generator.loss(self.features(tokens, leaf_ids, plan, root_ids, lengths), target, **options)
 
 
 class BPTEncoderDecoder(nn.Module):
@@ -250,15 +274,28 @@ class BPTEncoderDecoder(nn.Module):
         h[leaf_ids] = x
         return h
 
-    def forward(self, enc_tokens, enc_leaf_ids, enc_plan, dec_tokens, dec_leaf_ids, dec_plan, inter_plan,
-                readout_ids):
+    def features(self, enc_tokens, enc_leaf_ids, enc_plan, dec_tokens, dec_leaf_ids, dec_plan, inter_plan,
+                 readout_ids):
         """Tokens in leaf order, their node ids, the three plans (inter_plan: sources = encoder
-        nodes, destinations = decoder nodes) and the decoder nodes to read out.  Returns
-        log-probabilities (len(readout_ids), vocab)."""
+        nodes, destinations = decoder nodes) and the decoder nodes to read out.  Returns their
+        features after the last block (len(readout_ids), dim_model)."""
         h_enc = self._embed(self.embed[0], enc_tokens, enc_leaf_ids, enc_plan.n_nodes)
         for layer in self.enc_layers:                                              # model.py:85-86
             h_enc = layer(h_enc, enc_plan)
         h_dec = self._embed(self.embed[-1], dec_tokens, dec_leaf_ids, dec_plan.n_nodes)
         for layer in self.dec_layers:                                              # model.py:101-102
             h_dec = layer(h_dec, dec_plan, h_enc, inter_plan)
-        return self.generator(h_dec[readout_ids])                                  # model.py:104
+        return h_dec[readout_ids]
+
+    def forward(self, enc_tokens, enc_leaf_ids, enc_plan, dec_tokens, dec_leaf_ids, dec_plan, inter_plan,
+                readout_ids):
+        """As `features`; returns log-probabilities (len(readout_ids), vocab)."""
+        return self.generator(self.features(enc_tokens, enc_leaf_ids, enc_plan, dec_tokens, dec_leaf_ids, dec_plan,
+                                            inter_plan, readout_ids))               # model.py:104
+
+    def loss(self, enc_tokens, enc_leaf_ids, enc_plan, dec_tokens, dec_leaf_ids, dec_plan, inter_plan, readout_ids,
+             target, **options):
+        """Cross entropy of forward(...) against target (len(readout_ids),), without the log-probabilities in memory
+        (mt.py trains with label smoothing, loss/__init__.py:4-28).  options: ignore_index, label_smoothing, reduction."""
+        return self.generator.loss(self.features(enc_tokens, enc_leaf_ids, enc_plan, dec_tokens, dec_leaf_ids, dec_plan,
+                                                 inter_plan, readout_ids), target, **options)

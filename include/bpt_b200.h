@@ -502,6 +502,42 @@ int bpt_layer_norm_backward(const void *gy, const void *x, const void *r, const 
                             const float *rstd, void *da, void *dgamma, void *dbeta, int64_t n_rows, int dim,
                             int dtype, void *workspace, size_t workspace_bytes, bpt_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Softmax cross entropy of the logits z = x W^T + bias, without the logits: the generator of modules/model.py:8-17
+ * (projection + log-softmax) and the loss the task scripts put on it (nll_loss, lm.py:120-140; label smoothing,
+ * loss/__init__.py:4-28) as one call, and its gradients.
+ *
+ * x: (n, dim), w: (vocab, dim), row strides ldx, ldw in elements; bias (vocab) or NULL; all of `dtype` (BPT_F32,
+ * BPT_BF16, BPT_F16).  target: (n) int64.  A token whose target is ignore_index has loss 0 and no gradient, whatever
+ * its features hold; any other target outside [0, vocab) makes its loss (and the gradients it reaches) NaN.
+ * smoothing: the target's weight is 1 - smoothing, and smoothing / vocab goes to every class.
+ * reduction: BPT_LOSS_NONE (loss: n floats), BPT_LOSS_MEAN (over the tokens that count; NaN if there are none) or
+ * BPT_LOSS_SUM (one float).  lse: log sum exp z per token (n floats) and count: the number of tokens that count (one
+ * float, MEAN and SUM) are what the backward reads; either may be NULL.
+ *
+ * Backward: grad: gradient of the loss, n floats or one.  dx: (n, dim), dw: (vocab, dim), db: (vocab), contiguous, of
+ * `dtype`; each may be NULL to skip it.  The logits are computed again, in pieces of tokens x vocabulary whose gradient
+ * fits the L2.  Bitwise reproducible.
+ *
+ * The workspace sizes depend on the operands' addresses too (operands that are not 16-byte aligned are copied).  Calls
+ * that may overlap need workspaces of their own; nothing in one has to be zero.  A kernel whose bounded wait ran out
+ * leaves NaN in the loss, or in the first element of each gradient.
+ * ---------------------------------------------------------------------------------- */
+enum { BPT_LOSS_NONE = 0, BPT_LOSS_MEAN = 1, BPT_LOSS_SUM = 2 };
+size_t bpt_linear_ce_forward_workspace_bytes(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t n, int vocab,
+                                             int dim, int dtype);
+int bpt_linear_ce_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
+                          const int64_t *target, int64_t ignore_index, double smoothing, int reduction, float *loss,
+                          float *lse, float *count, int64_t n, int vocab, int dim, int dtype, void *workspace,
+                          size_t workspace_bytes, bpt_stream_t stream);
+size_t bpt_linear_ce_backward_workspace_bytes(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t n, int vocab,
+                                              int dim, int dtype, int want_dx, int want_dw, int want_db);
+int bpt_linear_ce_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
+                           const int64_t *target, int64_t ignore_index, double smoothing, int reduction,
+                           const float *lse, const float *count, const float *grad, void *dx, void *dw, void *db,
+                           int64_t n, int vocab, int dim, int dtype, void *workspace, size_t workspace_bytes,
+                           bpt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
