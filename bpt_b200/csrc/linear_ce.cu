@@ -8,18 +8,24 @@
 //     d x = dZ W,   d W = dZ^T X,   d b = column sums of dZ
 // Tokens whose target is `ignore_index` have loss 0 and g = 0.
 //
-// All four products run in one kernel shape on the 5th-generation tensor cores: a persistent block per SM walks
-// 128 x 256 tiles; one warp brings operand tiles in by TMA (128-byte swizzle, four stages), one issues tcgen05.mma
-// into one of two accumulators in tensor memory, eight warps read the other accumulator and finish the tile.
-//   stats  Z tiles of consecutive vocabulary blocks of one block of tokens: a running maximum and sum per row stay in
-//          registers, a row's pieces (one per block that worked on it) are merged by the loss kernel;
-//   grad   Z tiles once more (cheaper than keeping them: at D = 512 a logit costs 0.7 ps of tensor time, its fp32
-//          copy 1.2 ps of HBM time), turned into dZ, which is kept for one piece of the vocabulary x tokens at a time;
-//   dx, dw dZ W and dZ^T X of the piece.  dZ is read K-major by the one and MN-major by the other.
+// All four products run in one kernel shape on the 5th-generation tensor cores: a persistent pair of blocks (a cluster
+// of two on one pair of SMs) walks 256 x 256 tiles, 128 rows of the result in each block.  In each block one warp brings
+// operand tiles in by TMA (128-byte swizzle, six stages of 32 KB; B's rows are shared, half in each block), one thread
+// of the pair issues tcgen05.mma.cta_group::2 into one of two accumulators in tensor memory, and eight warps read the
+// other accumulator and finish the tile.
+//   stats     Z tiles of consecutive vocabulary blocks of one block of tokens: a running maximum and sum per row stay in
+//             registers, a row's pieces (one per pair that worked on it) are merged by the loss kernel;
+//   grad      Z tiles once more (cheaper than keeping them: at D = 512 a logit costs 0.7 ps of tensor time, its fp32
+//             copy 1.2 ps of HBM time), turned into dZ, which is kept for one piece of tokens x vocabulary at a time.
+//             A pair walks the token blocks of one vocabulary block, so d b stays in registers, summed over the rows
+//             of a thread, before the rounding of dZ;
+//   products  dZ W and dZ^T X of the piece in one launch.  dZ is read K-major by the one and MN-major by the other.
 // dZ is rounded to the operands' 16-bit type, without g where all g_i are one number (the scale goes onto the fp32
 // results): a half-step error of each probability, the size of the rounding of the gradients themselves.
 // fp32 operands are split into three bf16 planes (8 + 8 + 8 significant bits, by truncation, exact) and each product
-// is run as the six products of planes whose weight is above 2^-24, smallest first.
+// is run as the six products of planes whose weight is above 2^-24, smallest first.  The tensor core rounds its running
+// sum towards zero, a bias that grows with K, so the fp32 kernels take the accumulator out every 512 of K and add
+// the runs up in registers.
 #include <algorithm>
 #include <type_traits>
 
@@ -31,22 +37,50 @@ namespace {
 
 using namespace tc5;
 
-constexpr int kBM = 128, kBN = 256, kBK = 64, kStages = 4;
-constexpr int kABytes = kBM * kBK * 2, kBBytes = kBN * kBK * 2, kStageBytes = kABytes + kBBytes;
+constexpr int kBM = 256, kBN = 256, kBK = 64;  // a pair's tile; each block has 128 of the rows
+constexpr int kRows = kBM / 2, kCols = kBN / 2;               // what a block loads of A and of B
+constexpr int kABytes = kRows * kBK * 2, kBBytes = kCols * kBK * 2, kStageBytes = kABytes + kBBytes;
 constexpr int kChunkBytes = 64 * 128;  // an MN-major tile: 64 rows along K of 64 elements
-constexpr int kFinishWarps = 8, kThreads = (kFinishWarps + 2) * 32;
-constexpr int kGrid = 148;             // blocks at most: one per SM
-constexpr int kSmemBytes = kStages * kStageBytes + 2 * kBN * 4 + 256 + 1024;
+// Eight warps finish tiles, one loads, one issues products (two more make its warpgroup whole).  The finishing warps take
+// registers that the others leave: 256 * 216 + 128 * 72 = 384 * 168, what the block is launched with.
+constexpr int kFinishWarps = 8, kThreads = (kFinishWarps + 4) * 32;
+constexpr int kFinishRegs = 216, kOtherRegs = 72;
+static_assert(kFinishWarps * 32 * kFinishRegs + 128 * kOtherRegs <= kThreads * 168, "the block's registers");
+constexpr int kPairs = 74;             // pairs of blocks at most: one block per SM
+constexpr int kRunTiles = 8;           // fp32: K blocks added up by the tensor core before the sum is taken out
 
-enum Kind { kStats, kGrad, kDx, kDw };
+enum Kind { kStats, kGrad, kProducts };
+// Shared memory: the bias of two tiles, barriers; from the next 1024-byte boundary on operand stages, and for grad two
+// tiles of 32 rows x 64 columns of dZ per finishing warp, on their way out (one stage less for them).
+constexpr int kOutBytes = 32 * 128;
+constexpr int stages(int kind) { return kind == kGrad ? 5 : 6; }
+constexpr int out_bytes(int kind) { return kind == kGrad ? 2 * kFinishWarps * kOutBytes : 0; }
+constexpr int kHeadBytes = 3072;
+constexpr int smem_bytes(int kind) { return kHeadBytes + stages(kind) * kStageBytes + out_bytes(kind); }
+static_assert(smem_bytes(kGrad) <= 227 * 1024 && smem_bytes(kStats) <= 227 * 1024, "a block's shared memory");
 enum { kReduceNone = 0, kReduceMean = 1, kReduceSum = 2 };
 
+// One of the two products of a piece.  A unit of work is a tile and a part of its K.
+struct Product {
+    int m_tiles, n_tiles, k_tiles, n_ext;
+    int parts, part_tiles;                 // K parts of a tile (each of part_tiles K blocks; sums go to `partial` if parts > 1)
+    int b0;                                // added to B's row coordinate
+    int64_t row_offset, row_end;           // rows of the output: row_offset + tile row, below row_end
+    float *acc;                            // fp32 sums of earlier pieces (leading dimension acc_ld), or null
+    float *partial;                        // [part][m_tiles * 256][acc_ld]
+    int64_t acc_ld;
+    int add, last;                         // acc holds earlier pieces; write `out`
+    void *out;
+    __host__ __device__ int64_t tiles() const { return static_cast<int64_t>(m_tiles) * n_tiles; }
+    __host__ __device__ int64_t units() const { return tiles() * parts; }
+};
+
 struct Params {
-    int m_tiles, n_tiles, k_tiles, n_ext;  // tiles; columns in all (the last tile may be narrower)
+    int m_tiles, n_tiles, k_tiles, n_ext;  // stats, grad: tiles; columns in all (the last tile may be narrower)
+    int m_ext;                             // grad: rows of the piece
     int n_pairs;                           // plane products: 1, or 6 for fp32
     int a0, b0;                            // added to the row coordinate of A and of B
     int *status;                           // set to 1 when a wait ran out
-    // stats, grad
     int64_t n_rows, ignore_index;          // tokens in all
     int vocab;
     const void *bias;
@@ -57,28 +91,28 @@ struct Params {
     const float *lse, *grad;               // grad
     float smoothing;
     int reduction;
-    uint16_t *dz;
-    int64_t dz_ld, dz_plane;
-    // dx, dw
-    float *acc;                            // fp32 sums of earlier pieces (leading dimension acc_ld), or null
-    int64_t acc_ld, row_offset, row_end;   // rows of the output: row_offset + tile row, below row_end
-    int add, last;                         // acc holds earlier pieces; write `out`
-    void *out;
+    float *col_sums;                       // grad: column sums of dZ, 8 rows a piece (a warp's rows each), or null
+    int64_t col_ld;
     const float *count;
     const unsigned *grad_top;              // none: bits of max |g|
-    const unsigned char *clean;            // dw: per 64 tokens, 1 = read the copy with ignored rows zeroed
+    const unsigned char *clean;            // d w: per 64 tokens, 1 = read the copy with ignored rows zeroed
+    // products: 0 = d x, 1 = d w.  The one with the longer units goes first, dealt in turn; pairs below `busy` have one
+    // more of them.  The shorter units follow in runs of `after_busy` and `after` per pair.
+    Product product[2];
+    int first, busy, after_busy, after;
 };
 
 __constant__ const int kPairA[6] = {2, 0, 1, 1, 0, 0}, kPairB[6] = {0, 2, 1, 0, 1, 0};
 
 template <typename T> constexpr bool kIsHalf = std::is_same<T, __half>::value;
+template <typename T> constexpr bool kIsFloat = std::is_same<T, float>::value;
 // fp16 dZ is kept times 2^14: |dz| <= 2, and probabilities down to 2^-28 stay normal numbers
 template <typename T> constexpr float kDzScale = kIsHalf<T> ? 16384.f : 1.f;
 
 template <typename T> __device__ constexpr uint32_t ce_instr(int n, bool a_mn, bool b_mn) {
     const uint32_t fmt = kIsHalf<T> ? 0u : 1u;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) |
-           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kBM >> 4) << 24);
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kBM >> 4) << 24);  // M = 256 over the pair
 }
 
 // Power of two at or below the largest |g| (its bits), so that g / scale is exact and below 2.
@@ -88,9 +122,9 @@ __device__ __forceinline__ float top_scale(unsigned bits) {
     return e == 0u ? (bits ? 1.17549435e-38f : 1.f) : __uint_as_float(e << 23);
 }
 
-// The first tile of block c when t tiles are dealt in order to g blocks; the block that has tile i.
+// The first tile of pair c when t tiles are dealt in order to g pairs; the pair that has tile i.
 __host__ __device__ __forceinline__ int first_tile(int64_t t, int g, int c) { return static_cast<int>(t * c / g); }
-__host__ __device__ __forceinline__ int block_of_tile(int64_t t, int g, int64_t i) {
+__host__ __device__ __forceinline__ int pair_of_tile(int64_t t, int g, int64_t i) {
     return static_cast<int>(((i + 1) * g + t - 1) / t) - 1;
 }
 
@@ -157,17 +191,64 @@ template <typename T> __device__ __forceinline__ void store_row(T *row, int64_t 
     }
 }
 
-// A block's tiles: stats has consecutive ones (a row's running sums go from tile to tile), the others every gridDim-th.
-template <int kKind> struct Tiles {
-    int64_t total;
-    int at, end, step;
-    __device__ explicit Tiles(const Params &p) {
-        total = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-        const int g = gridDim.x, c = blockIdx.x;
-        at = kKind == kStats ? first_tile(total, g, c) : c;
-        end = kKind == kStats ? first_tile(total, g, c + 1) : static_cast<int>(total);
-        step = kKind == kStats ? 1 : g;
+// The work of a pair, in the order in which all its warps take it: a tile, the K blocks of it, and for the products
+// which product and part.
+template <int kKind> struct Work {
+    const Params &p;
+    int64_t at, end;              // stats, grad: consecutive tiles
+    int pair, pairs, stage;       // products
+    int64_t stop_first;
+    int m, n, k0, k1, which, part;
+    __device__ explicit Work(const Params &p_) : p(p_) {
+        pair = blockIdx.x >> 1;
+        pairs = gridDim.x >> 1;
+        which = part = 0;
+        if constexpr (kKind != kProducts) {
+            const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+            at = first_tile(total, pairs, pair);
+            end = first_tile(total, pairs, pair + 1);
+            k0 = 0;
+            k1 = p.k_tiles;
+        } else {
+            stage = 0;
+            at = pair;
+            end = p.product[p.first].units();
+        }
     }
+    __device__ bool next() {
+        if constexpr (kKind != kProducts) {
+            if (at >= end) return false;
+            // stats: the vocabulary blocks of a token block in a row; grad: the token blocks of a vocabulary block
+            m = static_cast<int>(kKind == kStats ? at / p.n_tiles : at % p.m_tiles);
+            n = static_cast<int>(kKind == kStats ? at % p.n_tiles : at / p.m_tiles);
+            ++at;
+            return true;
+        } else {
+            if (stage == 0 && at >= end) {
+                stage = 1;
+                const int64_t units = p.product[1 - p.first].units();
+                const int64_t before = pair < p.busy ? static_cast<int64_t>(pair) * p.after_busy
+                                                     : static_cast<int64_t>(p.busy) * p.after_busy + static_cast<int64_t>(pair - p.busy) * p.after;
+                at = before;
+                end = before + (pair < p.busy ? p.after_busy : p.after);
+                if (end > units) end = units;
+            }
+            if (at >= end) return false;
+            which = stage == 0 ? p.first : 1 - p.first;
+            const Product &q = p.product[which];
+            part = static_cast<int>(at / q.tiles());
+            const int tile = static_cast<int>(at % q.tiles());
+            m = tile / q.n_tiles;
+            n = tile % q.n_tiles;
+            k0 = part * q.part_tiles;
+            k1 = min(k0 + q.part_tiles, q.k_tiles);
+            at += stage == 0 ? pairs : 1;
+            return true;
+        }
+    }
+    __device__ int n_ext() const { return kKind == kProducts ? p.product[which].n_ext : p.n_ext; }
+    // columns of the product instruction: whole 32s, half of them from each block's B
+    __device__ int width() const { return (min(kBN, n_ext() - n * kBN) + 31) / 32 * 32; }
 };
 
 // Barrier of the finishing warps that also says whether any of their threads gave up.
@@ -179,166 +260,223 @@ __device__ __forceinline__ bool finish_barrier_or(bool v) {
                  : "memory");
     return r;
 }
-static_assert(kFinishWarps * 32 == 256, "finish_barrier_or names its thread count");
+static_assert(kFinishWarps * 32 == 256 && kBN == 256, "finish_barrier_or names its thread count, a thread brings one bias");
 
+// Sums over the warp's lanes of 32 columns: lane l gets the sum of v[l].  v is used up.
+__device__ __forceinline__ float column_sum(float (&v)[32], int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float keep = upper ? v[i + o] : v[i], give = upper ? v[i] : v[i + o];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+    return v[0];
+}
+
+// What the gradients of w and b, and of x, are multiplied by: the one gradient of the loss, or the power of two that
+// the tokens' own ones were divided by.
+template <typename T> __device__ __forceinline__ float result_scale(const Params &p) {
+    float scale = p.reduction == kReduceNone ? top_scale(*p.grad_top) : *p.grad;
+    if (p.reduction == kReduceMean) scale = *p.count > 0.f ? scale / *p.count : 0.f;
+    return scale * (1.f / kDzScale<T>);
+}
+
+// map_a, map_b: stats, grad: X and W rows; products: dZ rows and W columns.  map_c, map_d, map_e: dZ columns, X columns,
+// the copy of X with ignored rows zeroed.
 template <typename T, int kKind>
-__global__ void __launch_bounds__(kThreads, 1)
-linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                 const __grid_constant__ CUtensorMap map_b2, const Params p) {
-    constexpr bool kAMn = kKind == kDw, kBMn = kKind == kDx || kKind == kDw;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
+                 const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_e, const __grid_constant__ Params p) {
     constexpr bool kPrecise = std::is_same<T, float>::value;
-    extern __shared__ unsigned char smem_raw[];
-    __shared__ int stop_flag;
-    volatile int *stop = &stop_flag;
-    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    unsigned char *sm = smem_raw + (base - raw);
-    float *s_bias = reinterpret_cast<float *>(sm + kStages * kStageBytes);  // [2][256]
-    const uint32_t bars = base + kStages * kStageBytes + 2 * kBN * 4;
-    const uint32_t bar_full = bars, bar_empty = bars + 8 * kStages, bar_tfull = bars + 16 * kStages,
-                   bar_tempty = bar_tfull + 16, bar_drain = bar_tempty + 16, tmem_slot = bar_drain + 8;
+    constexpr int kStages = stages(kKind);
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    float *s_bias = reinterpret_cast<float *>(smem_raw);  // [2][256]
+    // full (block 0's is used) and empty per stage, sums ready and sums read (block 0's) per accumulator
+    const uint32_t bars = smem_u32(smem_raw) + 2 * kBN * 4;
+    const uint32_t bar_full = bars, bar_empty = bars + 8 * kStages, bar_ready = bars + 16 * kStages, bar_read = bar_ready + 16,
+                   bar_drain = bar_read + 16, tmem_slot = bar_drain + 8;
+    constexpr int kWordsAt = 2 * kBN * 4 + 16 * kStages + 40;
+    volatile uint32_t *tmem_word = reinterpret_cast<volatile uint32_t *>(smem_raw + kWordsAt);
+    volatile int *stop = reinterpret_cast<volatile int *>(smem_raw + kWordsAt + 4);
+    const uint32_t base = (bars + 16 * kStages + 48 + 1023u) & ~1023u;  // the same offset in both blocks
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
 
     if (tid == 0) {
-        stop_flag = 0;
+        *stop = 0;
         for (int s = 0; s < kStages; ++s) {
             mbar_init(bar_full + 8 * s, 1);
             mbar_init(bar_empty + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(bar_tfull + 8 * b, 1);
-            mbar_init(bar_tempty + 8 * b, kFinishWarps);
+            mbar_init(bar_ready + 8 * b, 1);
+            mbar_init(bar_read + 8 * b, 2 * kFinishWarps);
         }
         mbar_init(bar_drain, 1);
         fence_mbar_init();
-        prefetch_map(&map_a);
-        prefetch_map(&map_b);
         if (kKind == kStats && blockIdx.x == 0) {
             *p.ticket = 0u;
             *p.status = 0;
         }
     }
-    if (warp == kFinishWarps + 1) tmem_alloc(tmem_slot, 512);
+    if (warp == kFinishWarps + 1) tmem_alloc_pair(tmem_slot, 512);
     fence_before_sync();
     __syncthreads();
+    cluster_sync();  // both blocks' barriers are set up
     fence_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + (tmem_slot - base));
-    Tiles<kKind> tiles(p);
-    const int steps = p.n_pairs * p.k_tiles;
-
+    const uint32_t tmem = *tmem_word;
+    Work<kKind> work(p);
+    const int first_pair = p.n_pairs == 1 ? 5 : 0;
+    if (warp >= kFinishWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
     if (warp == kFinishWarps) {
-        if (lane == 0) {  // ---- loads
+        if (lane == 0) {  // ---- loads of this block's rows of A and half of B
             int s = 0;
             uint32_t phase = 0, issued = 0;
             bool ok = true;
-            for (int t = tiles.at; ok && t < tiles.end; t += tiles.step) {
-                const int m = t / p.n_tiles, n = t % p.n_tiles;
-                const int cols = min(kBN, p.n_ext - n * kBN), chunks = (cols + 63) / 64;
-                for (int step = 0; step < steps; ++step) {
-                    const int pair = p.n_pairs == 1 ? 5 : step / p.k_tiles, k = step % p.k_tiles;
-                    const int pa = kPairA[pair], pb = kPairB[pair];
-                    ok = mbar_wait_or_stop(bar_empty + 8 * s, phase ^ 1u, stop);
-                    if (!ok) break;
-                    const uint32_t a = base + s * kStageBytes, b = a + kABytes, full = bar_full + 8 * s;
-                    mbar_expect(full, kABytes + (kBMn ? chunks * kChunkBytes : kBBytes));
-                    if constexpr (kAMn) {
-                        tma_load(a, &map_a, m * kBM, p.a0 + k * kBK, pa, full);
-                        tma_load(a + kChunkBytes, &map_a, m * kBM + 64, p.a0 + k * kBK, pa, full);
-                    } else {
-                        tma_load(a, &map_a, k * kBK, p.a0 + m * kBM, pa, full);
-                    }
-                    if constexpr (kBMn) {
-                        const bool copy = kKind == kDw && p.clean && p.clean[p.b0 / kBK + k];
-                        for (int c = 0; c < chunks; ++c)
-                            tma_load(b + c * kChunkBytes, copy ? &map_b2 : &map_b, n * kBN + 64 * c, p.b0 + k * kBK, pb, full);
-                    } else {
-                        tma_load(b, &map_b, k * kBK, p.b0 + n * kBN, pb, full);
-                    }
-                    ++issued;
-                    if (++s == kStages) {
-                        s = 0;
-                        phase ^= 1u;
+            while (ok && work.next()) {
+                const int m0 = work.m * kBM + static_cast<int>(rank) * kRows, half = work.width() / 2;
+                const int n0 = work.n * kBN + static_cast<int>(rank) * half, chunks = (half + 63) / 64;
+                const int run = kPrecise ? kRunTiles : work.k1;
+                for (int kr = work.k0; ok && kr < work.k1; kr += run) {
+                    for (int pair = first_pair; ok && pair < 6; ++pair) {
+                        const int pa = kPairA[pair], pb = kPairB[pair];
+                        for (int k = kr; k < min(kr + run, work.k1); ++k) {
+                            ok = mbar_wait_or_stop(bar_empty + 8 * s, phase ^ 1u, stop);
+                            if (!ok) break;
+                            const uint32_t a = base + s * kStageBytes, b = a + kABytes, full = map_to(bar_full + 8 * s, 0);
+                            const int b_bytes = kKind == kProducts ? chunks * kChunkBytes : kBBytes;
+                            if (rank == 0) mbar_expect(bar_full + 8 * s, 2 * (kABytes + b_bytes));
+                            if constexpr (kKind == kProducts) {
+                                const int b_row = p.product[work.which].b0 + k * kBK;
+                                if (work.which == 0) {
+                                    tma_load_pair(a, &map_a, k * kBK, m0, pa, full);
+                                    for (int c = 0; c < chunks; ++c) tma_load_pair(b + c * kChunkBytes, &map_b, n0 + 64 * c, b_row, pb, full);
+                                } else {
+                                    tma_load_pair(a, &map_c, m0, k * kBK, pa, full);
+                                    tma_load_pair(a + kChunkBytes, &map_c, m0 + 64, k * kBK, pa, full);
+                                    const CUtensorMap *map = p.clean && p.clean[b_row / kBK] ? &map_e : &map_d;
+                                    for (int c = 0; c < chunks; ++c) tma_load_pair(b + c * kChunkBytes, map, n0 + 64 * c, b_row, pb, full);
+                                }
+                            } else {
+                                tma_load_pair(a, &map_a, k * kBK, p.a0 + m0, pa, full);
+                                tma_load_pair(b, &map_b, k * kBK, p.b0 + n0, pb, full);
+                            }
+                            ++issued;
+                            if (++s == kStages) {
+                                s = 0;
+                                phase ^= 1u;
+                            }
+                        }
                     }
                 }
             }
-            if (!ok) {  // the last loads of every stage land before the block ends
-                for (int i = 0; i < kStages; ++i) {
-                    if (issued <= static_cast<uint32_t>(i)) break;
-                    const uint32_t last = (issued - 1 - i) / kStages;
-                    const uint32_t bar = bar_full + 8 * ((issued - 1 - i) % kStages);
+            if (!ok) {  // the last loads of every stage land before the block ends (block 0's barriers know)
+                for (uint32_t i = 0; i < kStages && i < issued; ++i) {
+                    const uint32_t load = issued - 1 - i, bar = bar_full + 8 * (load % kStages);
                     const long long start = clock64();
-                    while (!mbar_try(bar, last & 1u) && clock64() - start < kWaitCycles) {}
+                    while (clock64() - start < kWaitCycles / 8 && !(rank == 0 && mbar_try(bar, (load / kStages) & 1u))) {}
                 }
             }
         }
     } else if (warp == kFinishWarps + 1) {
-        if (lane == 0) {  // ---- products
+        if (lane == 0 && rank == 0) {  // ---- products
             int s = 0, buf = 0;
-            uint32_t phase = 0, tphase = 0;
+            uint32_t phase = 0, read_phase = 0;
             bool ok = true;
-            for (int t = tiles.at; ok && t < tiles.end; t += tiles.step) {
-                const int n = t % p.n_tiles;
-                const int cols = (min(kBN, p.n_ext - n * kBN) + 31) / 32 * 32;
-                const uint32_t instr = ce_instr<T>(cols, kAMn, kBMn), d = tmem + buf * kBN;
-                ok = mbar_wait_or_stop(bar_tempty + 8 * buf, tphase ^ 1u, stop);
-                if (!ok) break;
-                fence_after_sync();
-                for (int step = 0; step < steps; ++step) {
-                    ok = mbar_wait_or_stop(bar_full + 8 * s, phase, stop);
+            while (ok && work.next()) {
+                const bool a_mn = kKind == kProducts && work.which == 1, b_mn = kKind == kProducts;
+                const uint32_t instr = ce_instr<T>(work.width(), a_mn, b_mn);
+                const int run = kPrecise ? kRunTiles : work.k1;
+                for (int kr = work.k0; ok && kr < work.k1; kr += run) {
+                    const uint32_t d = tmem + buf * kBN;
+                    ok = mbar_wait_or_stop(bar_read + 8 * buf, read_phase ^ 1u, stop);
                     if (!ok) break;
                     fence_after_sync();
-                    const uint32_t a = base + s * kStageBytes, b = a + kABytes;
+                    uint32_t accumulate = 0;
+                    const int steps = (6 - first_pair) * (min(kr + run, work.k1) - kr);
+                    for (int step = 0; step < steps; ++step) {
+                        ok = mbar_wait_or_stop(bar_full + 8 * s, phase, stop);
+                        if (!ok) break;
+                        fence_after_sync();
+                        const uint32_t a = base + s * kStageBytes, b = a + kABytes;
 #pragma unroll
-                    for (int ks = 0; ks < kBK / 16; ++ks)
-                        mma_ss(d, kAMn ? desc_mnmajor(a, ks) : desc_kmajor(a, ks), kBMn ? desc_mnmajor(b, ks) : desc_kmajor(b, ks),
-                               instr, step > 0 || ks > 0);
-                    mma_commit(bar_empty + 8 * s);
-                    if (++s == kStages) {
-                        s = 0;
-                        phase ^= 1u;
+                        for (int ks = 0; ks < kBK / 16; ++ks) {
+                            mma_pair(d, a_mn ? desc_mnmajor(a, ks) : desc_kmajor(a, ks), b_mn ? desc_mnmajor(b, ks) : desc_kmajor(b, ks), instr,
+                                     accumulate);
+                            accumulate = 1;
+                        }
+                        mma_commit_pair(bar_empty + 8 * s);
+                        if (++s == kStages) {
+                            s = 0;
+                            phase ^= 1u;
+                        }
                     }
-                }
-                if (!ok) break;
-                mma_commit(bar_tfull + 8 * buf);
-                if (++buf == 2) {
-                    buf = 0;
-                    tphase ^= 1u;
+                    if (!ok) break;
+                    mma_commit_pair(bar_ready + 8 * buf);
+                    if (++buf == 2) {
+                        buf = 0;
+                        read_phase ^= 1u;
+                    }
                 }
             }
             if (!ok) {  // products under way end before the tensor memory is freed
-                mma_commit(bar_drain);
+                mma_commit_pair(bar_drain);
                 const long long start = clock64();
                 while (!mbar_try(bar_drain, 0u) && clock64() - start < kWaitCycles) {}
             }
         }
-    } else {  // ---- finishing: warp % 4 names the tile's 32 rows, warp / 4 its half of the columns
-        const int quarter = warp & 3, half = warp >> 2, trow = quarter * 32 + lane;
+    }
+    } else {  // ---- finishing: warp % 4 names the 32 of this block's rows, warp / 4 the half of the columns
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kFinishRegs));
+        const int quarter = warp & 3, half = warp >> 2, trow = static_cast<int>(rank) * kRows + quarter * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        int buf = 0, parity = 0, row_m = -1;
-        uint32_t tphase = 0;
+        const uint32_t bar_read_0 = map_to(bar_read, 0);
+        int buf = 0, parity = 0, row_m = -1, col_n = -1;
+        uint32_t ready_phase = 0;
         float run_max = -INFINITY, run_sum = 0.f, run_z = 0.f;
         int tgt = -1;
-        float row_lse = 0.f, row_g = 0.f;
+        float row_lse = 0.f, row_l2 = 0.f, row_g = 0.f, uniform = 0.f;
+        bool row_plain = true, row_skips = false;  // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0
         float scale = 1.f;
-        if constexpr (kKind == kDx || kKind == kDw) {
-            if (p.last) {
-                if (p.reduction == kReduceNone) scale = top_scale(*p.grad_top);
-                else scale = *p.grad;
-                if (p.reduction == kReduceMean) scale = *p.count > 0.f ? scale / *p.count : 0.f;
-                scale *= 1.f / kDzScale<T>;
-            }
+        if constexpr (kKind == kProducts) scale = result_scale<T>(p);
+        // grad, 16-bit: column sums over the pair's token blocks of one vocabulary block
+        constexpr bool kKeepSums = kKind == kGrad && !kPrecise;
+        const uint32_t out_tile = base + kStages * kStageBytes + warp * 2 * kOutBytes;
+        int out_at = 0;
+        float col_sum[kKeepSums ? 4 : 1][32];
+        if constexpr (kKeepSums) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) col_sum[j][i] = 0.f;
         }
-        for (int t = tiles.at; t < tiles.end; t += tiles.step) {
-            const int m = t / p.n_tiles, n = t % p.n_tiles;
-            const int cols = min(kBN, p.n_ext - n * kBN);
-            bool ok;
+        auto store_col_sums = [&](float (&v)[32], int j, int n, int piece) {
+            const float total = column_sum(v, lane);
+            p.col_sums[(static_cast<int64_t>(piece) * 8 + rank * 4 + quarter) * p.col_ld + n * kBN + half * (kBN / 2) + j * 32 + lane] = total;
+        };
+        auto release = [&] {  // this warp has read the accumulator
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(bar_read_0 + 8 * buf);
+            if (++buf == 2) {
+                buf = 0;
+                ready_phase ^= 1u;
+            }
+        };
+        while (work.next()) {
+            const int m = work.m, n = work.n, cols = min(kBN, work.n_ext() - n * kBN);
             const float *bias = s_bias + parity * kBN;
-            if constexpr (kKind == kStats || kKind == kGrad) {
+            if constexpr (kKind != kProducts) {
                 const int col = n * kBN + tid;  // 256 finishing threads, 256 columns
                 float b = -INFINITY;
                 if (col < p.n_ext) {
                     const int64_t v = p.b0 + col;
-                    if constexpr (kPrecise) b = p.bias ? static_cast<const float *>(p.bias)[v] : 0.f;
-                    else b = p.bias ? to_acc<T>(static_cast<const T *>(p.bias)[v]) : 0.f;
+                    b = p.bias ? to_acc<T>(static_cast<const T *>(p.bias)[v]) : 0.f;
+                    if constexpr (!kPrecise) b *= kLog2e;
                 }
                 s_bias[parity * kBN + tid] = b;
                 parity ^= 1;
@@ -361,122 +499,267 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             if (tgt < 0) row_g = __int_as_float(0x7fffffff);  // no such class: the gradients say so
                             row_g *= kDzScale<T>;
                         }
+                        uniform = p.smoothing / static_cast<float>(p.vocab) * row_g;
+                        row_skips = __any_sync(0xffffffffu, row_g == 0.f);
+                        row_plain = p.smoothing == 0.f && __all_sync(0xffffffffu, row_g == kDzScale<T> || row_g == 0.f);
+                        row_l2 = row_lse * kLog2e - (row_plain && kIsHalf<T> ? 14.f : 0.f);
                     }
                 }
-                ok = mbar_wait_or_stop(bar_tfull + 8 * buf, tphase, stop);
-                ok = !finish_barrier_or(!ok);  // s_bias is whole, and all these warps go on or none does
-            } else {
-                ok = mbar_wait_or_stop(bar_tfull + 8 * buf, tphase, stop);
-                ok = __all_sync(0xffffffffu, ok);
-            }
-            if (!ok) break;
-            fence_after_sync();
-            const uint32_t acc = tmem + lanes + buf * kBN;
-            for (int c0 = half * (kBN / 2); c0 < (half + 1) * (kBN / 2) && c0 < cols; c0 += 32) {
-                uint32_t r[32];
-                __syncwarp();
-                tmem_ld32(acc + c0, r);
-                tmem_ld_wait();
-                if constexpr (kKind == kStats || kKind == kGrad) {
-                    float z[32];
+                if constexpr (kKeepSums) {
+                    if (n != col_n && col_n >= 0 && p.col_sums) {
+                        const int piece = work.pair - pair_of_tile(static_cast<int64_t>(p.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(col_n) * p.m_tiles);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + i);
-                        z[i] = __uint_as_float(r[i]) + b.x;
-                        z[i + 1] = __uint_as_float(r[i + 1]) + b.y;
-                        z[i + 2] = __uint_as_float(r[i + 2]) + b.z;
-                        z[i + 3] = __uint_as_float(r[i + 3]) + b.w;
+                        for (int j = 0; j < 4; ++j) {
+                            store_col_sums(col_sum[j], j, col_n, piece);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) col_sum[j][i] = 0.f;
+                        }
                     }
+                    col_n = n;
+                }
+            }
+            // finishes 32 neighbouring columns from c0 on; v: the products, left as what went out (grad)
+            auto finish = [&](float (&v)[32], int c0) {
+                if constexpr (kKind != kProducts) {
                     const int local = tgt - (p.b0 + n * kBN + c0);  // the target's place in these 32, if it is there
                     const bool here = tgt >= 0 && local >= 0 && local < 32;
-                    if constexpr (kKind == kStats) {
-                        float top = z[0];
+                    if constexpr (kPrecise) {  // logits; probabilities from differences of logits
 #pragma unroll
-                        for (int i = 1; i < 32; ++i) top = fmaxf(top, z[i]);
-                        if (top > run_max) {
-                            run_sum *= ex2((run_max - top) * kLog2e);
-                            run_max = top;
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + i);
+                            v[i] += b.x;
+                            v[i + 1] += b.y;
+                            v[i + 2] += b.z;
+                            v[i + 3] += b.w;
                         }
-                        const float m0 = run_max == -INFINITY ? 0.f : run_max, m2 = m0 * kLog2e;
-                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    } else {  // logits times log2(e)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            sum[i & 3] += kPrecise ? ex2((z[i] - m0) * kLog2e) : ex2(fmaf(z[i], kLog2e, -m2));
-                        run_sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + i);
+                            const float2 lo = fma2(make_float2(v[i], v[i + 1]), make_float2(kLog2e, kLog2e), make_float2(b.x, b.y));
+                            const float2 hi = fma2(make_float2(v[i + 2], v[i + 3]), make_float2(kLog2e, kLog2e), make_float2(b.z, b.w));
+                            v[i] = lo.x;
+                            v[i + 1] = lo.y;
+                            v[i + 2] = hi.x;
+                            v[i + 3] = hi.y;
+                        }
+                    }
+                    constexpr float kUnit = kPrecise ? 1.f : kLn2;  // of v, in logits
+                    if constexpr (kKind == kStats) {
                         if (p.smoothed) {
-                            float total = 0.f;
+                            if (cols == kBN) {
+                                float2 total = make_float2(0.f, 0.f);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) total += c0 + i < cols ? z[i] : 0.f;
-                            run_z += total;
+                                for (int i = 0; i < 32; i += 2) total = add2(total, make_float2(v[i], v[i + 1]));
+                                run_z += (total.x + total.y) * kUnit;
+                            } else {
+                                float total = 0.f;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) total += c0 + i < cols ? v[i] : 0.f;
+                                run_z += total * kUnit;
+                            }
                         }
                         if (here) {
                             float zt = 0.f;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) zt = i == local ? z[i] : zt;
-                            p.z_target[p.a0 + static_cast<int64_t>(m) * kBM + trow] = zt;
+                            for (int i = 0; i < 32; ++i) zt = i == local ? v[i] : zt;
+                            p.z_target[p.a0 + static_cast<int64_t>(m) * kBM + trow] = zt * kUnit;
                         }
-                    } else {
-                        const float l2 = row_lse * kLog2e, uniform = p.smoothing / static_cast<float>(p.vocab) * row_g;
+                        // Sums of exp(v - run_max), where run_max is a number near the largest so far: it moves only when
+                        // a sum gets large (or is not a number), which saves looking for the maximum of every 32.
+                        float2 sum = make_float2(0.f, 0.f);
+                        if constexpr (!kPrecise) {
+                            const float2 from = make_float2(-run_max, -run_max);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float prob = kPrecise ? ex2((z[i] - row_lse) * kLog2e) : ex2(fmaf(z[i], kLog2e, -l2));
-                            z[i] = row_g == 0.f ? 0.f : fmaf(prob, row_g, -uniform);
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 d = add2(make_float2(v[i], v[i + 1]), from);
+                                sum = add2(sum, make_float2(ex2(d.x), ex2(d.y)));
+                            }
+                        }
+                        float more = sum.x + sum.y;
+                        if (kPrecise || !(more < 1e18f) || run_max == -INFINITY) {
+                            float top = v[0];
+#pragma unroll
+                            for (int i = 1; i < 32; ++i) top = fmaxf(top, v[i]);
+                            if (top > run_max) {
+                                run_sum *= ex2((run_max - top) * (kPrecise ? kLog2e : 1.f));
+                                run_max = top;
+                            }
+                            const float m0 = run_max == -INFINITY ? 0.f : run_max;
+                            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) part[i & 3] += ex2((v[i] - m0) * (kPrecise ? kLog2e : 1.f));
+                            more = (part[0] + part[1]) + (part[2] + part[3]);
+                        }
+                        run_sum += more;
+                    } else {
+                        // p g - e / V g, with p = exp(z - lse); where every g of the warp is 1 and nothing is smoothed,
+                        // the type's scale rides in the exponent
+                        if constexpr (kPrecise) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = fmaf(ex2((v[i] - row_lse) * kLog2e), row_g, -uniform);
+                        } else {
+                            const float2 from = make_float2(-row_l2, -row_l2);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 d = add2(make_float2(v[i], v[i + 1]), from);
+                                v[i] = ex2(d.x);
+                                v[i + 1] = ex2(d.y);
+                            }
+                            if (!row_plain) {
+                                const float2 g2 = make_float2(row_g, row_g), u2 = make_float2(-uniform, -uniform);
+#pragma unroll
+                                for (int i = 0; i < 32; i += 2) {
+                                    const float2 d = fma2(make_float2(v[i], v[i + 1]), g2, u2);
+                                    v[i] = d.x;
+                                    v[i + 1] = d.y;
+                                }
+                            }
+                        }
+                        if (row_skips) {  // some row of the warp is ignored: zeros there, whatever its logits are
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = row_g == 0.f ? 0.f : v[i];
                         }
                         if (here) {
                             const float sub = (1.f - p.smoothing) * row_g;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) z[i] -= i == local ? sub : 0.f;
+                            for (int i = 0; i < 32; ++i) v[i] -= i == local ? sub : 0.f;
                         }
-                        // the buffer's rows and columns are padded to whole tiles
-                        uint16_t *at = p.dz + (static_cast<int64_t>(m) * kBM + trow) * p.dz_ld + n * kBN + c0;
+                        // Out through shared memory, 64 columns of the warp's 32 rows at a time: whole 128-byte lines.
+                        constexpr int kPlanes = kPrecise ? 3 : 1;
+                        float left[kPrecise ? 32 : 1];
+                        if constexpr (kPrecise) {
 #pragma unroll
-                        for (int plane = 0; plane < (kPrecise ? 3 : 1); ++plane) {
+                            for (int i = 0; i < 32; ++i) left[i] = v[i];
+                        }
+                        // 16-bit: 32 columns into one half of the tile, out after the second; fp32: a tile a plane
 #pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                uint32_t w[8];
+                        for (int plane = 0; plane < kPlanes; ++plane) {
+                            const int at = kPrecise ? 0 : (c0 >> 5) & 1;  // which half of the tile's 64 columns
+                            const uint32_t tile = out_tile + out_at * kOutBytes;
+                            if (kPrecise || at == 0) {
+                                if (lane == 0) store_wait_read<1>();  // the other tile may still be on its way
+                                __syncwarp();
+                            }
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    if constexpr (kPrecise) w[i] = take_plane(z[16 * u + 2 * i], z[16 * u + 2 * i + 1]);
-                                    else w[i] = pack2<T>(z[16 * u + 2 * i], z[16 * u + 2 * i + 1]);
+                            for (int u = 0; u < 4; ++u) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    if constexpr (kPrecise) w[i] = take_plane(left[8 * u + 2 * i], left[8 * u + 2 * i + 1]);
+                                    else w[i] = pack2<T>(v[8 * u + 2 * i], v[8 * u + 2 * i + 1]);
                                 }
-                                st_global_v8(at + plane * p.dz_plane + 16 * u, w);
+                                if constexpr (kPrecise) st_shared_v4(tile + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4), w[0], w[1], w[2], w[3]);
+                                else st_shared_v4(tile + swz(lane, at * 4 + u), w[0], w[1], w[2], w[3]);
+                            }
+                            if (kPrecise || at == 1 || c0 + 32 >= cols) {
+                                fence_async_smem();
+                                __syncwarp();
+                                const int x = n * kBN + (kPrecise ? c0 : c0 & ~63), y = m * kBM + trow - lane;
+                                if (lane == 0) {
+                                    if (y < p.m_ext) tma_store(&map_c, x, y, plane, tile);
+                                    store_commit();
+                                }
+                                out_at ^= 1;
                             }
                         }
                     }
                 } else {
-                    const int64_t row = p.row_offset + static_cast<int64_t>(m) * kBM + trow;
-                    if (row < p.row_end) {
-                        float v[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                        const int col = n * kBN + c0, left = p.n_ext - col;
-                        float *sums = p.acc ? p.acc + row * p.acc_ld + col : nullptr;
-                        if (p.add) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] += i < left ? sums[i] : 0.f;
-                        }
-                        if (p.last) {
-                            const bool ignored = kKind == kDx && p.target[row] == p.ignore_index;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = ignored ? 0.f : v[i] * scale;
-                            store_row(static_cast<T *>(p.out) + row * p.n_ext, p.n_ext * static_cast<int64_t>(sizeof(T)), col, left, v);
+                    const Product &q = p.product[work.which];
+                    const int64_t in_piece = static_cast<int64_t>(m) * kBM + trow, row = q.row_offset + in_piece;
+                    const int col = n * kBN + c0, left = q.n_ext - col;
+                    if (row < q.row_end) {
+                        if (q.parts > 1) {
+                            store_row(q.partial + (static_cast<int64_t>(work.part) * q.m_tiles * kBM + in_piece) * q.acc_ld, q.acc_ld * 4, col, left, v);
                         } else {
-                            store_row(p.acc + row * p.acc_ld, p.acc_ld * 4, col, left, v);
+                            if (q.add) {
+                                const float *sums = q.acc + row * q.acc_ld + col;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) v[i] += i < left ? sums[i] : 0.f;
+                            }
+                            if (q.last) {
+                                const bool ignored = work.which == 0 && p.target[row] == p.ignore_index;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) v[i] = ignored ? 0.f : v[i] * scale;
+                                store_row(static_cast<T *>(q.out) + row * q.n_ext, q.n_ext * static_cast<int64_t>(sizeof(T)), col, left, v);
+                            } else {
+                                store_row(q.acc + row * q.acc_ld, q.acc_ld * 4, col, left, v);
+                            }
                         }
                     }
                 }
-            }
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
-            if (++buf == 2) {
-                buf = 0;
-                tphase ^= 1u;
+            };
+            const int first = half * (kBN / 2);
+            bool ok;
+            if constexpr (kPrecise) {  // add the runs up in registers, then finish
+                float sum[4][32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
+                ok = true;
+                for (int kr = work.k0; ok && kr < work.k1; kr += kRunTiles) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_or_stop(bar_ready + 8 * buf, ready_phase, stop));
+                    if (!ok) break;
+                    fence_after_sync();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (first + 32 * j < cols) {
+                            uint32_t r[32];
+                            tmem_ld32(tmem + lanes + buf * kBN + first + 32 * j, r);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sum[j][i] += __uint_as_float(r[i]);
+                        }
+                    }
+                    release();
+                }
+                if constexpr (kKind != kProducts) ok = !finish_barrier_or(!ok);  // s_bias is whole, and all these warps go on or none does
+                if (!ok) break;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (first + 32 * j < cols) {
+                        finish(sum[j], first + 32 * j);
+                        __syncwarp();
+                        if constexpr (kKind == kGrad) {
+                            if (p.col_sums) store_col_sums(sum[j], j, n, m);
+                        }
+                    }
+                }
+            } else {
+                ok = mbar_wait_or_stop(bar_ready + 8 * buf, ready_phase, stop);
+                if constexpr (kKind != kProducts) ok = !finish_barrier_or(!ok);
+                else ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                fence_after_sync();
+                // (loading the next 32 columns ahead was slower: 1.4 times for grad, whose sums then spill, 1.03 for stats)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (first + 32 * j < cols) {
+                        uint32_t r[32];
+                        float v[32];
+                        tmem_ld32(tmem + lanes + buf * kBN + first + 32 * j, r);
+                        tmem_ld_wait_for(r);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                        finish(v, first + 32 * j);
+                        if constexpr (kKeepSums) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 sum = add2(make_float2(col_sum[j][i], col_sum[j][i + 1]), make_float2(v[i], v[i + 1]));
+                                col_sum[j][i] = sum.x;
+                                col_sum[j][i + 1] = sum.y;
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+                release();
             }
             if constexpr (kKind == kStats) {
-                if (n == p.n_tiles - 1 || t + 1 == tiles.end) {  // the last tile of these rows in this block
+                if (n == p.n_tiles - 1 || work.at == work.end) {  // the last tile of these rows in this pair
                     const int64_t rows_padded = static_cast<int64_t>(p.m_tiles) * kBM;
-                    const int piece = blockIdx.x - block_of_tile(tiles.total, gridDim.x, static_cast<int64_t>(m) * p.n_tiles);
+                    const int piece = work.pair - pair_of_tile(static_cast<int64_t>(p.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(m) * p.n_tiles);
                     float *at = p.partial + (static_cast<int64_t>(piece) * 2 + half) * 3 * rows_padded + static_cast<int64_t>(m) * kBM + trow;
                     at[0] = run_max;
                     at[rows_padded] = run_sum;
@@ -484,13 +767,24 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 }
             }
         }
+        if constexpr (kKeepSums) {
+            if (col_n >= 0 && p.col_sums) {
+                const int piece = work.pair - pair_of_tile(static_cast<int64_t>(p.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(col_n) * p.m_tiles);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) store_col_sums(col_sum[j], j, col_n, piece);
+            }
+        }
+        if constexpr (kKind == kGrad) {
+            if (lane == 0) store_wait();
+        }
     }
     __syncwarp();
     fence_before_sync();
     __syncthreads();
+    cluster_sync();  // nothing of the pair is under way any more
     if (warp == kFinishWarps + 1) {
         fence_after_sync();
-        tmem_free(tmem, 512);
+        tmem_free_pair(tmem, 512);
     }
     if (tid == 0 && *stop) *p.status = 1;
 }
@@ -501,8 +795,8 @@ struct LossParams {
     const float *partial, *z_target;
     const int64_t *target;
     int64_t n_rows, ignore_index;
-    int m_tiles, n_tiles, grid, vocab, reduction;
-    float smoothing;
+    int m_tiles, n_tiles, pairs, vocab, reduction;
+    float smoothing, unit;  // unit: of a piece's maximum, in logits
     float *loss, *lse, *count;
     double *block_sums;  // [blocks][sum, count]
     unsigned *ticket;
@@ -516,7 +810,7 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
     bool counted = false;
     if (row < p.n_rows) {
         const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles, m = row / kBM, rows_padded = static_cast<int64_t>(p.m_tiles) * kBM;
-        const int pieces = 2 * (block_of_tile(total, p.grid, (m + 1) * p.n_tiles - 1) - block_of_tile(total, p.grid, m * p.n_tiles) + 1);
+        const int pieces = 2 * (pair_of_tile(total, p.pairs, (m + 1) * p.n_tiles - 1) - pair_of_tile(total, p.pairs, m * p.n_tiles) + 1);
         float top = -INFINITY, sum = 0.f, z = 0.f;
         for (int i = lane; i < pieces; i += kLanes) top = fmaxf(top, p.partial[static_cast<int64_t>(i) * 3 * rows_padded + row]);
 #pragma unroll
@@ -524,7 +818,7 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
         for (int i = lane; i < pieces; i += kLanes) {
             const float *at = p.partial + static_cast<int64_t>(i) * 3 * rows_padded + row;
             const float s = at[rows_padded];
-            if (!(s == 0.f)) sum += s * exp2f((at[0] - top) * kLog2e);  // a piece without any finite logit has sum 0
+            if (!(s == 0.f)) sum += s * exp2f((at[0] - top) * (p.unit * kLog2e));  // a piece without any finite logit has sum 0
             z += at[2 * rows_padded];
         }
 #pragma unroll
@@ -533,7 +827,7 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
             z += __shfl_xor_sync(0xffffffffu, z, o);
         }
         if (lane == 0) {
-            const float lse = top + logf(sum);
+            const float lse = top * p.unit + logf(sum);
             const int64_t target = p.target[row];
             counted = target != p.ignore_index;
             if (counted) {
@@ -666,58 +960,61 @@ __global__ void linear_ce_top_kernel(const float *__restrict__ grad, const int64
     if ((threadIdx.x & 31) == 0) atomicMax(top, best);
 }
 
-// Column sums of a dZ piece over each 128 rows: thread per pair of columns.
+// Sums of a product's K parts (and of earlier pieces), in their order: a thread has 4 neighbouring columns.
 template <typename T>
-__global__ void __launch_bounds__(128) linear_ce_colsum_kernel(const uint16_t *__restrict__ dz, int64_t ld, int64_t plane, int rows,
-                                                               int cols, float *__restrict__ out, int64_t out_ld) {
-    const int c = (blockIdx.x * 128 + threadIdx.x) * 2;
-    if (c >= cols) return;
-    float a = 0.f, b = 0.f;
-    for (int r = blockIdx.y * 128; r < min(rows, static_cast<int>(blockIdx.y) * 128 + 128); ++r) {
-        constexpr int kPlanes = std::is_same<T, float>::value ? 3 : 1;
-        float va = 0.f, vb = 0.f;
+__global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_constant__ Params p, int which) {
+    const Product &q = p.product[which];
+    const int64_t pieces = q.acc_ld / 4, rows = q.row_end - q.row_offset, total = rows * pieces, plane = static_cast<int64_t>(q.m_tiles) * kBM * q.acc_ld;
+    const float scale = result_scale<T>(p);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t in_piece = i / pieces, row = q.row_offset + in_piece;
+        const int col = static_cast<int>(i % pieces) * 4, left = min(4, q.n_ext - col);
+        const float *from = q.partial + in_piece * q.acc_ld + col;
+        float4 s = *reinterpret_cast<const float4 *>(from);
+        for (int k = 1; k < q.parts; ++k) {
+            const float4 t = *reinterpret_cast<const float4 *>(from + k * plane);
+            s.x += t.x;
+            s.y += t.y;
+            s.z += t.z;
+            s.w += t.w;
+        }
+        float v[4] = {s.x, s.y, s.z, s.w};
+        float *sums = q.acc + row * q.acc_ld + col;
 #pragma unroll
-        for (int q = kPlanes - 1; q >= 0; --q) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(dz + q * plane + r * ld + c);
-            if constexpr (kIsHalf<T>) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-                va += f.x;
-                vb += f.y;
+        for (int j = 0; j < 4; ++j) {
+            if (j >= left) break;
+            if (q.add) v[j] += sums[j];
+            if (!q.last) {
+                sums[j] = v[j];
             } else {
-                va += __uint_as_float(w << 16);
-                vb += __uint_as_float(w & 0xFFFF0000u);
+                const bool ignored = which == 0 && p.target[row] == p.ignore_index;
+                static_cast<T *>(q.out)[row * q.n_ext + col + j] = from_acc<T>(ignored ? 0.f : v[j] * scale);
             }
         }
-        a += va;
-        b += vb;
     }
-    out[blockIdx.y * out_ld + c] = a;
-    if (c + 1 < cols) out[blockIdx.y * out_ld + c + 1] = b;
 }
 
-// d b of a piece: sums over its blocks of rows, added to those of earlier rows; the last one is scaled and stored.
+// d b of a piece: the column sums that the pairs (or, each_m, the token blocks) left, added to those of earlier rows;
+// the last one is scaled and stored.
 template <typename T>
-__global__ void __launch_bounds__(256) linear_ce_bias_kernel(const float *__restrict__ sums, int64_t ld, int blocks, int cols, float *acc,
-                                                             int add, int last, T *__restrict__ out, Params p) {
+__global__ void __launch_bounds__(256) linear_ce_bias_kernel(const __grid_constant__ Params p, int pairs, int each_m, float *acc, int add,
+                                                             int last, T *__restrict__ out) {
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
     __shared__ float s_part[8][32];
+    const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles, n = blockIdx.x * 32 / kBN;
+    const int pieces = each_m ? p.m_tiles : pair_of_tile(total, pairs, (n + 1) * p.m_tiles - 1) - pair_of_tile(total, pairs, n * p.m_tiles) + 1;
     float s = 0.f;
-    if (c < cols)
-        for (int r = part; r < blocks; r += 8) s += sums[r * ld + c];
+    if (c < p.n_ext)
+        for (int r = part; r < pieces * 8; r += 8) s += p.col_sums[r * p.col_ld + c];
     s_part[part][threadIdx.x & 31] = s;
     __syncthreads();
-    if (part > 0 || c >= cols) return;
+    if (part > 0 || c >= p.n_ext) return;
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += s_part[i][threadIdx.x];
     if (add) s += acc[c];
-    if (!last) {
-        acc[c] = s;
-        return;
-    }
-    float scale = p.reduction == kReduceNone ? top_scale(*p.grad_top) : *p.grad;
-    if (p.reduction == kReduceMean) scale = *p.count > 0.f ? scale / *p.count : 0.f;
-    out[c] = from_acc<T>(s * (scale / kDzScale<T>));
+    if (!last) acc[c] = s;
+    else out[c] = from_acc<T>(s * result_scale<T>(p));
 }
 
 // A wait that ran out leaves results that mean nothing: say so in them.
@@ -741,6 +1038,13 @@ bool tma_ready(const void *p, int64_t ld, int dtype) {
 }
 int64_t ce_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+int pairs_for(int64_t tiles) { return static_cast<int>(std::min<int64_t>(kPairs, tiles)); }
+// Pairs that get a share of `run` consecutive tiles of `total`, at most.
+int64_t shared_pieces(int64_t run, int64_t total) {
+    const int64_t pairs = pairs_for(total);
+    return std::min<int64_t>(pairs, run * pairs / total + 2);
+}
+
 struct Shape {
     int64_t n;
     int vocab, dim, dtype, planes;
@@ -752,10 +1056,8 @@ struct Shape {
     int64_t m_tiles() const { return ce_div(n, kBM); }
     int v_tiles() const { return static_cast<int>(ce_div(vocab, kBN)); }
     int64_t packed(int64_t rows) const { return align_up(rows * packed_ld, 64) * planes; }
-    int stats_grid() const { return static_cast<int>(std::min<int64_t>(kGrid, m_tiles() * v_tiles())); }
-    int64_t pieces() const {  // blocks that share one block of rows, at most
-        return std::min<int64_t>(stats_grid(), static_cast<int64_t>(v_tiles()) * stats_grid() / (m_tiles() * v_tiles()) + 2);
-    }
+    // pairs that share one block of rows in the forward, at most
+    int64_t pieces() const { return shared_pieces(v_tiles(), m_tiles() * v_tiles()); }
 };
 
 struct ForwardSpace {
@@ -775,8 +1077,71 @@ struct ForwardSpace {
     }
 };
 
-// Bytes of dZ kept at a time.  It is written by one product and read by two, so it should stay in the 126 MB L2.
-constexpr int64_t kDzBytes = 64 << 20;
+// Bytes of dZ kept at a time.  More than the L2 holds: the products read it at 3 TB/s, which HBM has to spare, and larger
+// pieces leave fewer pairs of blocks idle at their ends.  28701 x 8000 x 512 / 8192 x 50000 x 512, forward + backward:
+// 64 MB 1340 / 1987 us, 128 MB 1075 / 1744, 256 MB 892 / 1557, 512 MB 866 / 1533.
+constexpr int64_t kDzBytes = 256 << 20;
+
+// How the two products of a piece are dealt to the pairs of blocks.
+struct Deal {
+    int pairs, first, busy, after_busy, after;
+    int64_t steps;  // of the pair with the most work
+};
+// Unit lengths l0, l1 (in K blocks, with what a unit costs besides) and numbers u0, u1: the longer units in turn, then
+// runs of the shorter ones so that the pair with the most work has as little as possible.
+Deal deal(int64_t l0, int64_t u0, int64_t l1, int64_t u1) {
+    Deal d;
+    d.pairs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kPairs, u0 + u1)));
+    d.first = u0 > 0 && (l0 >= l1 || u1 == 0) ? 0 : 1;
+    const int64_t long_l = d.first == 0 ? l0 : l1, long_u = d.first == 0 ? u0 : u1, short_l = d.first == 0 ? l1 : l0, short_u = d.first == 0 ? u1 : u0;
+    const int64_t each = long_u / d.pairs;
+    d.busy = static_cast<int>(long_u % d.pairs);
+    auto room = [&](int64_t t, int64_t units) { return t < units * long_l ? 0 : (t - units * long_l) / short_l; };
+    int64_t low = d.busy ? (each + 1) * long_l : each * long_l, high = low + (short_u / d.pairs + 1) * short_l + long_l;
+    while (short_u > 0 && low < high) {
+        const int64_t t = (low + high) / 2;
+        if (d.busy * room(t, each + 1) + (d.pairs - d.busy) * room(t, each) >= short_u) high = t;
+        else low = t + 1;
+    }
+    d.steps = low;
+    d.after_busy = short_u > 0 ? static_cast<int>(room(low, each + 1)) : 0;
+    d.after = short_u > 0 ? static_cast<int>(room(low, each)) : 0;
+    return d;
+}
+// A unit's fixed cost, and that of its sums through memory where a tile has several parts, in K blocks of one product
+// (0.3 us): measured.
+constexpr int64_t kUnitSteps = 4, kPartSteps = 20;
+// What a launch costs in K blocks, and the elements of a sum that is read and written once more in the time of one.
+constexpr int64_t kLaunchSteps = 15, kStepElements = 200000;
+// Splits the longer tiles along K where that shortens the work of the pair with the most of it: few tiles, long K.
+Deal split_and_deal(Product &x, Product &w, int n_pairs) {
+    auto steps = [&](const Product &q, int parts) {
+        return ce_div(q.k_tiles, parts) * n_pairs + kUnitSteps + (parts > 1 ? kPartSteps : 0);
+    };
+    Product &longer = w.tiles() == 0 || (x.tiles() > 0 && x.k_tiles >= w.k_tiles) ? x : w;
+    Product &other = &longer == &x ? w : x;
+    Deal best{};
+    int best_parts = 0;
+    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 36, 72}) {
+        if (parts > 1 && (longer.k_tiles < 4 * parts || longer.tiles() * parts > 2 * kPairs)) break;
+        const int64_t l = steps(longer, parts), u = longer.tiles() * parts;
+        const Deal d = &longer == &x ? deal(l, u, steps(other, 1), other.tiles()) : deal(steps(other, 1), other.tiles(), l, u);
+        if (best_parts == 0 || d.steps < best.steps) {
+            best = d;
+            best_parts = parts;
+        }
+    }
+    x.parts = w.parts = 1;
+    x.part_tiles = x.k_tiles;
+    w.part_tiles = w.k_tiles;
+    longer.part_tiles = static_cast<int>(ce_div(longer.k_tiles, best_parts));
+    longer.parts = static_cast<int>(ce_div(longer.k_tiles, std::max(1, longer.part_tiles)));
+    if (longer.parts != best_parts) {  // rounding left fewer parts
+        const int64_t l = steps(longer, longer.parts), u = longer.units();
+        best = &longer == &x ? deal(l, u, steps(other, 1), other.tiles()) : deal(steps(other, 1), other.tiles(), l, u);
+    }
+    return best;
+}
 
 struct BackwardSpace {
     int64_t rows, cols;  // tokens x vocabulary of a piece
@@ -785,35 +1150,9 @@ struct BackwardSpace {
     unsigned *grad_top;
     uint16_t *dz, *x, *w, *x_clean;
     unsigned char *clean;
-    float *dx_acc, *dw_acc, *col_sums, *db_acc;
+    float *dx_acc, *dw_acc, *col_sums, *db_acc, *partial;
     BackwardSpace(Workspace &ws, const Shape &s, bool want_dx, bool want_dw, bool want_db) {
-        // Pieces of rows x cols cells.  Cutting the vocabulary has dX pass through memory once a cut, cutting the
-        // tokens dW: take the cheaper of the two, whole tiles, at least 1024 each way.
-        const int64_t cells = kDzBytes / (2 * s.planes), n_pad = ce_div(s.n, kBM) * kBM, v_pad = ce_div(s.vocab, kBN) * kBN;
-        rows = n_pad;
-        cols = v_pad;
-        if (n_pad * v_pad > cells) {
-            int64_t best = -1;
-            for (int64_t r = std::min<int64_t>(n_pad, 1024);; r = std::min(r * 2, n_pad)) {
-                int64_t c = std::max<int64_t>(cells / r / kBN * kBN, 1024);
-                c = std::min(c, v_pad);
-                const int64_t row_cuts = ce_div(n_pad, r), col_cuts = ce_div(v_pad, c);
-                const int64_t cost = (col_cuts - 1) * s.n + (row_cuts - 1) * s.vocab;
-                if (r * c <= cells + cells / 8 && (best < 0 || cost < best)) {
-                    best = cost;
-                    rows = r;
-                    cols = c;
-                }
-                if (r == n_pad) break;
-            }
-            if (best < 0) {
-                rows = std::min<int64_t>(n_pad, 1024);
-                cols = std::min<int64_t>(v_pad, std::max<int64_t>(1024, cells / rows / kBN * kBN));
-            }
-            // pieces of one size instead of a small last one
-            rows = ce_div(ce_div(n_pad, kBM), ce_div(n_pad, rows)) * kBM;
-            cols = ce_div(ce_div(v_pad, kBN), ce_div(v_pad, cols)) * kBN;
-        }
+        choose_pieces(s, want_dx, want_dw);
         dz_ld = cols;
         dz_plane = rows * cols;
         acc_ld = ce_div(s.dim, 8) * 8;
@@ -827,16 +1166,86 @@ struct BackwardSpace {
         clean = !s.pack_x && want_dw ? ws.take<unsigned char>(ce_div(s.n, 64)) : nullptr;
         dx_acc = want_dx && !own_acc && cols < s.vocab ? ws.take<float>(s.n * acc_ld) : nullptr;
         dw_acc = want_dw && !own_acc && rows < s.n ? ws.take<float>(s.vocab * acc_ld) : nullptr;
-        col_sums = want_db ? ws.take<float>(rows / kBM * cols) : nullptr;
         db_acc = want_db && rows < s.n ? ws.take<float>(s.vocab) : nullptr;
+        // the rows of column sums and the parts that any of the pieces may need (the last ones are smaller)
+        int64_t sum_rows = 0, parts = 0;
+        for (int64_t r : {rows, s.n - (ce_div(s.n, rows) - 1) * rows}) {
+            for (int64_t c : {cols, s.vocab - (ce_div(s.vocab, cols) - 1) * cols}) {
+                const int64_t m = ce_div(r, kBM), n = ce_div(c, kBN);
+                sum_rows = std::max(sum_rows, 8 * (s.planes == 3 ? m : shared_pieces(m, m * n)));
+                Product px, pw;
+                products(s, want_dx, want_dw, r, c, &px, &pw);
+                split_and_deal(px, pw, s.planes == 3 ? 6 : 1);
+                for (const Product &q : {px, pw})
+                    if (q.parts > 1) parts = std::max(parts, static_cast<int64_t>(q.parts) * q.m_tiles * kBM * acc_ld);
+            }
+        }
+        col_sums = want_db ? ws.take<float>(sum_rows * cols) : nullptr;
+        partial = parts ? ws.take<float>(parts) : nullptr;
+    }
+    // Pieces of rows x cols cells, whole tiles, that fit kDzBytes: as few K blocks' time as possible on the pair of
+    // blocks with the most work, over all pieces, with a launch's cost for each piece and with what passes through
+    // memory more than once (dX once more a cut of the vocabulary, dW a cut of the tokens).
+    void choose_pieces(const Shape &s, bool want_dx, bool want_dw) {
+        const int64_t cells = kDzBytes / (2 * s.planes), m = ce_div(s.n, kBM), n = ce_div(s.vocab, kBN);
+        const int n_pairs = s.planes == 3 ? 6 : 1;
+        rows = m * kBM;
+        cols = n * kBN;
+        if (rows * cols <= cells) return;
+        const int64_t least = ce_div(rows * cols, cells);  // pieces at least
+        int64_t best = -1;
+        auto consider = [&](int64_t row_cuts, int64_t col_cuts) {
+            const int64_t pm = ce_div(m, row_cuts), pn = ce_div(n, col_cuts);
+            if (pm * kBM * pn * kBN > cells) return;
+            row_cuts = ce_div(m, pm);
+            col_cuts = ce_div(n, pn);
+            Product x, w;
+            products(s, want_dx, want_dw, pm * kBM, pn * kBN, &x, &w);
+            const int64_t steps = split_and_deal(x, w, n_pairs).steps +
+                                  ce_div(pm * pn, kPairs) * (ce_div(s.dim, kBK) * n_pairs + 1) + 2 * kLaunchSteps;
+            const int64_t again = ((col_cuts - 1) * s.n + (row_cuts - 1) * s.vocab) * s.dim / kStepElements;
+            const int64_t cost = row_cuts * col_cuts * steps + again;
+            if (best < 0 || cost < best) {
+                best = cost;
+                rows = pm * kBM;
+                cols = pn * kBN;
+            }
+        };
+        for (int64_t cuts = least; cuts < least + least / 2 + 6; ++cuts) {
+            if (cuts <= m) consider(cuts, 1);
+            if (cuts <= n) consider(1, cuts);
+        }
+        // both ways, where one way leaves a piece too narrow to keep the products busy
+        for (int64_t r = 2; r * r <= 4 * least && r <= m; r *= 2) {
+            const int64_t c = ce_div(least, r) + 1;
+            if (c > 1 && c <= n) consider(r, c);
+        }
+        for (int64_t r = m; best < 0; r = ce_div(r, 2)) {  // nothing fitted: smaller and smaller
+            consider(ce_div(m, r), n);
+            if (r == 1) break;
+        }
+    }
+    // Tiles of the products of a piece of r x c cells.
+    static void products(const Shape &s, bool want_dx, bool want_dw, int64_t r, int64_t c, Product *x, Product *w) {
+        *x = Product{};
+        *w = Product{};
+        x->n_ext = w->n_ext = s.dim;
+        x->n_tiles = w->n_tiles = static_cast<int>(ce_div(s.dim, kBN));
+        x->m_tiles = want_dx ? static_cast<int>(ce_div(r, kBM)) : 0;
+        w->m_tiles = want_dw ? static_cast<int>(ce_div(c, kBM)) : 0;
+        x->k_tiles = static_cast<int>(ce_div(c, kBK));
+        w->k_tiles = static_cast<int>(ce_div(r, kBK));
+        x->parts = w->parts = 1;
     }
 };
 
-template <typename T, int kKind>
-int launch_ce(const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &b2, const Params &p, cudaStream_t stream) {
-    const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-    BPT_CUDA(cudaFuncSetAttribute(linear_ce_kernel<T, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
-    linear_ce_kernel<T, kKind><<<static_cast<unsigned>(std::min<int64_t>(kGrid, total)), kThreads, kSmemBytes, stream>>>(a, b, b2, p);
+struct Maps {
+    CUtensorMap a, b, c, d, e;
+};
+
+template <typename T, int kKind> int launch_ce(const Maps &m, const Params &p, int pairs, cudaStream_t stream) {
+    BPT_CUDA(cudaFuncSetAttribute(linear_ce_kernel<T, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kKind)));
+    linear_ce_kernel<T, kKind><<<2 * pairs, kThreads, smem_bytes(kKind), stream>>>(m.a, m.b, m.c, m.d, m.e, p);
     BPT_LAUNCH_CHECK();
     return BPT_OK;
 }
@@ -874,9 +1283,10 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     Operand x{c.x, c.ldx, 0}, w{c.w, c.ldw, 0};
     if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, f.x, nullptr, 0, stream, &x));
     if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, f.w, nullptr, 0, stream, &w));
-    CUtensorMap ma, mb;
-    BPT_TRY(make_map(&ma, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kBM));
-    BPT_TRY(make_map(&mb, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kBN));
+    Maps maps;
+    BPT_TRY(make_map(&maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
+    BPT_TRY(make_map(&maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));
+    maps.c = maps.d = maps.e = maps.a;
     Params p{};
     p.m_tiles = static_cast<int>(s.m_tiles());
     p.n_tiles = s.v_tiles();
@@ -893,7 +1303,8 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     p.z_target = f.z_target;
     p.ticket = f.ticket;
     p.smoothed = c.smoothing != 0.f;
-    BPT_TRY((launch_ce<T, kStats>(ma, mb, mb, p, stream)));
+    const int pairs = pairs_for(s.m_tiles() * s.v_tiles());
+    BPT_TRY((launch_ce<T, kStats>(maps, p, pairs, stream)));
     LossParams l{};
     l.partial = f.partial;
     l.z_target = f.z_target;
@@ -902,10 +1313,11 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     l.ignore_index = c.ignore_index;
     l.m_tiles = p.m_tiles;
     l.n_tiles = p.n_tiles;
-    l.grid = s.stats_grid();
+    l.pairs = pairs;
     l.vocab = s.vocab;
     l.reduction = c.reduction;
     l.smoothing = c.smoothing;
+    l.unit = kIsFloat<T> ? 1.f : kLn2;
     l.loss = loss;
     l.lse = lse;
     l.count = count;
@@ -940,13 +1352,14 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
                                                                                                                c.ignore_index, f.grad_top);
         BPT_LAUNCH_CHECK();
     }
-    CUtensorMap x_rows, w_rows, w_cols, x_cols, x_clean;
-    BPT_TRY(make_map(&x_rows, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kBM));
-    BPT_TRY(make_map(&w_rows, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kBN));
-    BPT_TRY(make_map(&w_cols, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, 64));
-    BPT_TRY(make_map(&x_cols, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, 64));
-    x_clean = x_cols;
-    if (f.clean) BPT_TRY(make_map(&x_clean, kHalf, f.x_clean, s.n, s.dim, clean_ld, 1, 0, 64));
+    Maps grad_maps, maps;
+    BPT_TRY(make_map(&grad_maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
+    BPT_TRY(make_map(&grad_maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));
+    grad_maps.d = grad_maps.e = grad_maps.a;
+    BPT_TRY(make_map(&maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, 64));
+    BPT_TRY(make_map(&maps.d, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, 64));
+    maps.e = maps.d;
+    if (f.clean) BPT_TRY(make_map(&maps.e, kHalf, f.x_clean, s.n, s.dim, clean_ld, 1, 0, 64));
     Params p{};
     p.n_pairs = s.planes == 3 ? 6 : 1;
     p.status = f.status;
@@ -961,9 +1374,9 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     p.count = count;
     p.smoothing = c.smoothing;
     p.reduction = c.reduction;
-    p.dz = f.dz;
-    p.dz_ld = f.dz_ld;
-    p.dz_plane = f.dz_plane;
+    p.col_sums = f.col_sums;
+    p.col_ld = f.cols;
+    p.clean = f.clean;
     const bool own_acc = kFloat && s.dim == f.acc_ld;
     for (int64_t n0 = 0; n0 < s.n; n0 += f.rows) {
         const int64_t rows = std::min(f.rows, s.n - n0);
@@ -971,58 +1384,55 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
         for (int64_t v0 = 0; v0 < s.vocab; v0 += f.cols) {
             const int64_t cols = std::min<int64_t>(f.cols, s.vocab - v0);
             const bool last_cols = v0 + f.cols >= s.vocab;
-            CUtensorMap dz_rows, dz_cols;
-            BPT_TRY(make_map(&dz_rows, kHalf, f.dz, rows, cols, f.dz_ld, s.planes, f.dz_plane, kBM));
-            BPT_TRY(make_map(&dz_cols, kHalf, f.dz, rows, cols, f.dz_ld, s.planes, f.dz_plane, 64));
             Params g = p;
             g.m_tiles = static_cast<int>(ce_div(rows, kBM));
             g.n_tiles = static_cast<int>(ce_div(cols, kBN));
             g.k_tiles = static_cast<int>(ce_div(s.dim, kBK));
             g.n_ext = static_cast<int>(cols);
+            g.m_ext = static_cast<int>(rows);
             g.a0 = static_cast<int>(n0);
             g.b0 = static_cast<int>(v0);
-            BPT_TRY((launch_ce<T, kGrad>(x_rows, w_rows, w_rows, g, stream)));
-            if (dx) {
-                Params q = p;
-                q.m_tiles = g.m_tiles;
-                q.n_tiles = static_cast<int>(ce_div(s.dim, kBN));
-                q.k_tiles = static_cast<int>(ce_div(cols, kBK));
-                q.n_ext = s.dim;
-                q.b0 = static_cast<int>(v0);
-                q.acc = own_acc ? static_cast<float *>(dx) : f.dx_acc;
-                q.acc_ld = f.acc_ld;
-                q.row_offset = n0;
-                q.row_end = n0 + rows;
-                q.add = v0 > 0;
-                q.last = last_cols;
-                q.out = dx;
-                BPT_TRY((launch_ce<T, kDx>(dz_rows, w_cols, w_cols, q, stream)));
-            }
-            if (dw) {
-                Params q = p;
-                q.m_tiles = static_cast<int>(ce_div(cols, kBM));
-                q.n_tiles = static_cast<int>(ce_div(s.dim, kBN));
-                q.k_tiles = static_cast<int>(ce_div(rows, kBK));
-                q.n_ext = s.dim;
-                q.b0 = static_cast<int>(n0);
-                q.acc = own_acc ? static_cast<float *>(dw) : f.dw_acc;
-                q.acc_ld = f.acc_ld;
-                q.row_offset = v0;
-                q.row_end = v0 + cols;
-                q.add = n0 > 0;
-                q.last = last_rows;
-                q.out = dw;
-                q.clean = f.clean;
-                BPT_TRY((launch_ce<T, kDw>(dz_cols, x_cols, x_clean, q, stream)));
-            }
+            BPT_TRY(make_map(&grad_maps.c, kHalf, f.dz, rows, cols, f.dz_ld, s.planes, f.dz_plane, 32, kFloat ? 32 : 64));
+            const int pairs = pairs_for(static_cast<int64_t>(g.m_tiles) * g.n_tiles);
+            BPT_TRY((launch_ce<T, kGrad>(grad_maps, g, pairs, stream)));
             if (db) {
-                const int blocks = static_cast<int>(ce_div(rows, kBM));
-                linear_ce_colsum_kernel<T><<<dim3(static_cast<unsigned>(ce_div(cols, 256)), blocks), 128, 0, stream>>>(
-                    f.dz, f.dz_ld, f.dz_plane, static_cast<int>(rows), static_cast<int>(cols), f.col_sums, f.cols);
-                BPT_LAUNCH_CHECK();
                 linear_ce_bias_kernel<T><<<static_cast<unsigned>(ce_div(cols, 32)), 256, 0, stream>>>(
-                    f.col_sums, f.cols, blocks, static_cast<int>(cols), f.db_acc ? f.db_acc + v0 : nullptr, n0 > 0, last_rows,
-                    static_cast<T *>(db) + v0, p);
+                    g, pairs, kFloat, f.db_acc ? f.db_acc + v0 : nullptr, n0 > 0, last_rows, static_cast<T *>(db) + v0);
+                BPT_LAUNCH_CHECK();
+            }
+            if (!dx && !dw) continue;
+            BPT_TRY(make_map(&maps.a, kHalf, f.dz, rows, cols, f.dz_ld, s.planes, f.dz_plane, kRows));
+            BPT_TRY(make_map(&maps.c, kHalf, f.dz, rows, cols, f.dz_ld, s.planes, f.dz_plane, 64));
+            Params q = p;
+            BackwardSpace::products(s, dx, dw, rows, cols, &q.product[0], &q.product[1]);
+            Product &px = q.product[0], &pw = q.product[1];
+            const Deal d = split_and_deal(px, pw, p.n_pairs);
+            q.first = d.first;
+            q.busy = d.busy;
+            q.after_busy = d.after_busy;
+            q.after = d.after;
+            px.b0 = static_cast<int>(v0);
+            px.row_offset = n0;
+            px.row_end = n0 + rows;
+            px.acc = own_acc ? static_cast<float *>(dx) : f.dx_acc;
+            px.add = v0 > 0;
+            px.last = last_cols;
+            px.out = dx;
+            pw.b0 = static_cast<int>(n0);
+            pw.row_offset = v0;
+            pw.row_end = v0 + cols;
+            pw.acc = own_acc ? static_cast<float *>(dw) : f.dw_acc;
+            pw.add = n0 > 0;
+            pw.last = last_rows;
+            pw.out = dw;
+            px.acc_ld = pw.acc_ld = f.acc_ld;
+            px.partial = pw.partial = f.partial;  // at most one of them has parts
+            BPT_TRY((launch_ce<T, kProducts>(maps, q, d.pairs, stream)));
+            for (int which = 0; which < 2; ++which) {
+                const Product &r = q.product[which];
+                if (r.parts <= 1) continue;
+                const int64_t blocks = std::min<int64_t>(ce_div((r.row_end - r.row_offset) * (r.acc_ld / 4), 256), 148 * 8);
+                linear_ce_parts_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(q, which);
                 BPT_LAUNCH_CHECK();
             }
         }

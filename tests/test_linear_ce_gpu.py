@@ -119,7 +119,8 @@ def test_values_and_gradients(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", [(2100, 20000, 64), (20000, 2100, 64), (34000, 4000, 32), (12000, 12000, 40)])
+@pytest.mark.parametrize("shape", [(2100, 20000, 64), (20000, 2100, 64), (34000, 4000, 32), (12000, 12000, 40), (6000, 40000, 32),
+                                   (40000, 6000, 32), (20, 300000, 16), (300000, 20, 16)])
 def test_pieces(shape, dtype):
     """More cells than are kept at a time: the vocabulary is cut, the tokens are, and both."""
     check(*inputs(*shape, dtype, padded=0.1), smoothing=0.1)
