@@ -27,6 +27,7 @@
 // sum towards zero, a bias that grows with K, so the fp32 kernels take the accumulator out every 512 of K and add
 // the runs up in registers.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "fused_common.cuh"
@@ -78,7 +79,8 @@ struct Product {
 struct Params {
     int m_tiles, n_tiles, k_tiles, n_ext;  // stats, grad: tiles; columns in all (the last tile may be narrower)
     int m_ext;                             // grad: rows of the piece
-    int n_pairs;                           // plane products: 1, or 6 for fp32
+    int n_pairs;                           // plane products: 1, 2 or 6
+    int dz_planes;                         // grad: planes of dZ that are written
     int a0, b0;                            // added to the row coordinate of A and of B
     int *status;                           // set to 1 when a wait ran out
     int64_t n_rows, ignore_index;          // tokens in all
@@ -86,7 +88,9 @@ struct Params {
     const void *bias;
     const int64_t *target;
     float *partial, *z_target;             // stats: [piece][max, sum, sum of z][row], z of the target
-    unsigned *ticket;                      // stats: zeroed here for the loss kernel
+    unsigned *ticket;                      // zeroed by stats and grad for what follows them: its last block speaks for all
+    int starts;                            // the call's first kernel: status is cleared
+    void *spoilt;                          // db, where a wait that ran out is made known when its kernel has written it
     int smoothed;
     const float *lse, *grad;               // grad
     float smoothing;
@@ -102,7 +106,8 @@ struct Params {
     int first, busy, after_busy, after;
 };
 
-__constant__ const int kPairA[6] = {2, 0, 1, 1, 0, 0}, kPairB[6] = {0, 2, 1, 0, 1, 0};
+// Plane products, smallest first.  All six: fp32 by fp32; the last two: dZ in two planes by a 16-bit operand; the last: 16-bit.
+__constant__ const int kPairA[6] = {2, 0, 1, 0, 1, 0}, kPairB[6] = {0, 2, 1, 1, 0, 0};
 
 template <typename T> constexpr bool kIsHalf = std::is_same<T, __half>::value;
 template <typename T> constexpr bool kIsFloat = std::is_same<T, float>::value;
@@ -141,6 +146,14 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t *>(&h);
     }
+}
+template <typename T> __device__ __forceinline__ float unpack_low(uint32_t w) {
+    if constexpr (kIsHalf<T>) return __half2float(__ushort_as_half(static_cast<unsigned short>(w & 0xFFFFu)));
+    else return __uint_as_float(w << 16);
+}
+template <typename T> __device__ __forceinline__ float unpack_high(uint32_t w) {
+    if constexpr (kIsHalf<T>) return __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16)));
+    else return __uint_as_float(w & 0xFFFF0000u);
 }
 // The next bf16 plane of a, b (truncated, so what is left is exact); a and b become what is left.
 __device__ __forceinline__ uint32_t take_plane(float &a, float &b) {
@@ -317,9 +330,9 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         mbar_init(bar_drain, 1);
         fence_mbar_init();
-        if (kKind == kStats && blockIdx.x == 0) {
+        if (kKind != kProducts && blockIdx.x == 0) {
             *p.ticket = 0u;
-            *p.status = 0;
+            if (p.starts) *p.status = 0;
         }
     }
     if (warp == kFinishWarps + 1) tmem_alloc_pair(tmem_slot, 512);
@@ -329,7 +342,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     fence_after_sync();
     const uint32_t tmem = *tmem_word;
     Work<kKind> work(p);
-    const int first_pair = p.n_pairs == 1 ? 5 : 0;
+    const int first_pair = 6 - p.n_pairs;
     if (warp >= kFinishWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
     if (warp == kFinishWarps) {
@@ -625,42 +638,64 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] -= i == local ? sub : 0.f;
                         }
-                        // Out through shared memory, 64 columns of the warp's 32 rows at a time: whole 128-byte lines.
-                        constexpr int kPlanes = kPrecise ? 3 : 1;
-                        float left[kPrecise ? 32 : 1];
+                        // Out through shared memory: with one plane 64 columns of the warp's 32 rows at a time (whole
+                        // 128-byte lines, sent after the second 32), else 32 columns of each plane.
+                        const int y = m * kBM + trow - lane;
+                        auto send = [&](int x, int plane, uint32_t tile) {
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (y < p.m_ext) tma_store(&map_c, x, y, plane, tile);
+                                store_commit();
+                            }
+                            out_at ^= 1;
+                        };
+                        auto next_tile = [&] {  // the other one may still be on its way
+                            if (lane == 0) store_wait_read<1>();
+                            __syncwarp();
+                            return out_tile + out_at * kOutBytes;
+                        };
+                        const uint32_t narrow = lane * 64, turn = lane >> 1 & 3;  // a row of a 64-byte-swizzled tile
                         if constexpr (kPrecise) {
+                            float left[32];
 #pragma unroll
                             for (int i = 0; i < 32; ++i) left[i] = v[i];
-                        }
-                        // 16-bit: 32 columns into one half of the tile, out after the second; fp32: a tile a plane
 #pragma unroll
-                        for (int plane = 0; plane < kPlanes; ++plane) {
-                            const int at = kPrecise ? 0 : (c0 >> 5) & 1;  // which half of the tile's 64 columns
-                            const uint32_t tile = out_tile + out_at * kOutBytes;
-                            if (kPrecise || at == 0) {
-                                if (lane == 0) store_wait_read<1>();  // the other tile may still be on its way
-                                __syncwarp();
-                            }
+                            for (int plane = 0; plane < 3; ++plane) {
+                                const uint32_t tile = next_tile();
 #pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                uint32_t w[4];
+                                for (int u = 0; u < 4; ++u) {
+                                    uint32_t w[4];
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    if constexpr (kPrecise) w[i] = take_plane(left[8 * u + 2 * i], left[8 * u + 2 * i + 1]);
-                                    else w[i] = pack2<T>(v[8 * u + 2 * i], v[8 * u + 2 * i + 1]);
+                                    for (int i = 0; i < 4; ++i) w[i] = take_plane(left[8 * u + 2 * i], left[8 * u + 2 * i + 1]);
+                                    st_shared_v4(tile + narrow + ((u ^ turn) << 4), w[0], w[1], w[2], w[3]);
                                 }
-                                if constexpr (kPrecise) st_shared_v4(tile + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4), w[0], w[1], w[2], w[3]);
-                                else st_shared_v4(tile + swz(lane, at * 4 + u), w[0], w[1], w[2], w[3]);
+                                send(n * kBN + c0, plane, tile);
                             }
-                            if (kPrecise || at == 1 || c0 + 32 >= cols) {
-                                fence_async_smem();
-                                __syncwarp();
-                                const int x = n * kBN + (kPrecise ? c0 : c0 & ~63), y = m * kBM + trow - lane;
-                                if (lane == 0) {
-                                    if (y < p.m_ext) tma_store(&map_c, x, y, plane, tile);
-                                    store_commit();
+                        } else if (p.dz_planes == 1) {
+                            const int at = (c0 >> 5) & 1;  // which half of the tile's 64 columns
+                            const uint32_t tile = at == 0 ? next_tile() : out_tile + out_at * kOutBytes;
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+                                st_shared_v4(tile + swz(lane, at * 4 + u), pack2<T>(v[8 * u], v[8 * u + 1]), pack2<T>(v[8 * u + 2], v[8 * u + 3]),
+                                             pack2<T>(v[8 * u + 4], v[8 * u + 5]), pack2<T>(v[8 * u + 6], v[8 * u + 7]));
+                            if (at == 1 || c0 + 32 >= cols) send(n * kBN + (c0 & ~63), 0, tile);
+                        } else {
+#pragma unroll
+                            for (int plane = 0; plane < 2; ++plane) {
+                                const uint32_t tile = next_tile();
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) {
+                                    uint32_t w[4];
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const float a = v[8 * u + 2 * i], b = v[8 * u + 2 * i + 1];
+                                        w[i] = pack2<T>(a, b);
+                                        if (plane == 1) w[i] = pack2<T>(a - unpack_low<T>(w[i]), b - unpack_high<T>(w[i]));
+                                    }
+                                    st_shared_v4(tile + narrow + ((u ^ turn) << 4), w[0], w[1], w[2], w[3]);
                                 }
-                                out_at ^= 1;
+                                send(n * kBN + c0, plane, tile);
                             }
                         }
                     }
@@ -786,7 +821,21 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         fence_after_sync();
         tmem_free_pair(tmem, 512);
     }
-    if (tid == 0 && *stop) *p.status = 1;
+    if (tid == 0) {
+        if (*stop) *p.status = 1;
+        if constexpr (kKind == kProducts) {  // a wait that ran out leaves results that mean nothing: the last block says so in them
+            __threadfence();
+            if (atomicAdd(p.ticket, 1u) == gridDim.x - 1) {
+                __threadfence();
+                if (*static_cast<volatile int *>(p.status)) {
+                    const T nan = from_acc<T>(__int_as_float(0x7fffffff));
+                    if (p.product[0].tiles() && p.product[0].last) static_cast<T *>(p.product[0].out)[p.product[0].row_offset * p.product[0].n_ext] = nan;
+                    if (p.product[1].tiles() && p.product[1].last) static_cast<T *>(p.product[1].out)[p.product[1].row_offset * p.product[1].n_ext] = nan;
+                    if (p.spoilt) *static_cast<T *>(p.spoilt) = nan;
+                }
+            }
+        }
+    }
 }
 
 // ---- the loss from the pieces: kLanes threads a row, one row or many pieces a thread.
@@ -965,7 +1014,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_constant__ Params p, int which) {
     const Product &q = p.product[which];
     const int64_t pieces = q.acc_ld / 4, rows = q.row_end - q.row_offset, total = rows * pieces, plane = static_cast<int64_t>(q.m_tiles) * kBM * q.acc_ld;
-    const float scale = result_scale<T>(p);
+    const float scale = *p.status ? __int_as_float(0x7fffffff) : result_scale<T>(p);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t in_piece = i / pieces, row = q.row_offset + in_piece;
         const int col = static_cast<int>(i % pieces) * 4, left = min(4, q.n_ext - col);
@@ -1014,17 +1063,7 @@ __global__ void __launch_bounds__(256) linear_ce_bias_kernel(const __grid_consta
     for (int i = 0; i < 8; ++i) s += s_part[i][threadIdx.x];
     if (add) s += acc[c];
     if (!last) acc[c] = s;
-    else out[c] = from_acc<T>(s * result_scale<T>(p));
-}
-
-// A wait that ran out leaves results that mean nothing: say so in them.
-template <typename T> __global__ void linear_ce_poison_kernel(const int *status, T *dx, T *dw, T *db) {
-    if (*status) {
-        const T nan = from_acc<T>(__int_as_float(0x7fffffff));
-        if (dx) *dx = nan;
-        if (dw) *dw = nan;
-        if (db) *db = nan;
-    }
+    else out[c] = *p.status ? from_acc<T>(__int_as_float(0x7fffffff)) : from_acc<T>(s * result_scale<T>(p));
 }
 
 // ---- host side
@@ -1045,14 +1084,22 @@ int64_t shared_pieces(int64_t run, int64_t total) {
     return std::min<int64_t>(pairs, run * pairs / total + 2);
 }
 
+// Up to so many tokens the 16-bit kernels keep dZ in two planes, 16 significant bits of it: the rounding of a handful of
+// probabilities does not average out (a single token's gradients were off by up to 4e-3), and the products of a single
+// block of tokens wait for memory, not for the second product.
+constexpr int64_t kFewTokens = 256;
+
 struct Shape {
     int64_t n;
-    int vocab, dim, dtype, planes;
+    int vocab, dim, dtype, planes, dz_planes;
     int64_t packed_ld;
     bool pack_x, pack_w;
     Shape(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t n_, int vocab_, int dim_, int dtype_)
-        : n(n_), vocab(vocab_), dim(dim_), dtype(dtype_), planes(dtype_ == BPT_F32 ? 3 : 1), packed_ld(ce_div(dim_, 8) * 8),
+        : n(n_), vocab(vocab_), dim(dim_), dtype(dtype_), planes(dtype_ == BPT_F32 ? 3 : 1),
+          dz_planes(dtype_ == BPT_F32 ? 3 : n_ <= kFewTokens ? 2 : 1), packed_ld(ce_div(dim_, 8) * 8),
           pack_x(!tma_ready(x, ldx, dtype_)), pack_w(!tma_ready(w, ldw, dtype_)) {}
+    int logit_pairs() const { return planes == 3 ? 6 : 1; }                          // plane products of the logits
+    int product_pairs() const { return planes == 3 ? 6 : dz_planes == 2 ? 2 : 1; }  // and of the gradients
     int64_t m_tiles() const { return ce_div(n, kBM); }
     int v_tiles() const { return static_cast<int>(ce_div(vocab, kBN)); }
     int64_t packed(int64_t rows) const { return align_up(rows * packed_ld, 64) * planes; }
@@ -1147,7 +1194,7 @@ struct BackwardSpace {
     int64_t rows, cols;  // tokens x vocabulary of a piece
     int64_t dz_ld, dz_plane, acc_ld;
     int *status;
-    unsigned *grad_top;
+    unsigned *ticket, *grad_top;
     uint16_t *dz, *x, *w, *x_clean;
     unsigned char *clean;
     float *dx_acc, *dw_acc, *col_sums, *db_acc, *partial;
@@ -1158,8 +1205,9 @@ struct BackwardSpace {
         acc_ld = ce_div(s.dim, 8) * 8;
         const bool own_acc = s.dtype == BPT_F32 && s.dim == acc_ld;  // fp32 sums can live in the output itself
         status = ws.take<int>(1);
+        ticket = ws.take<unsigned>(1);
         grad_top = ws.take<unsigned>(1);
-        dz = ws.take<uint16_t>(dz_plane * s.planes);
+        dz = ws.take<uint16_t>(dz_plane * s.dz_planes);
         x = s.pack_x ? ws.take<uint16_t>(s.packed(s.n)) : nullptr;
         w = s.pack_w ? ws.take<uint16_t>(s.packed(s.vocab)) : nullptr;
         x_clean = !s.pack_x && want_dw ? ws.take<uint16_t>(s.n * ce_div(s.dim, 8) * 8) : nullptr;
@@ -1175,7 +1223,7 @@ struct BackwardSpace {
                 sum_rows = std::max(sum_rows, 8 * (s.planes == 3 ? m : shared_pieces(m, m * n)));
                 Product px, pw;
                 products(s, want_dx, want_dw, r, c, &px, &pw);
-                split_and_deal(px, pw, s.planes == 3 ? 6 : 1);
+                split_and_deal(px, pw, s.product_pairs());
                 for (const Product &q : {px, pw})
                     if (q.parts > 1) parts = std::max(parts, static_cast<int64_t>(q.parts) * q.m_tiles * kBM * acc_ld);
             }
@@ -1187,8 +1235,7 @@ struct BackwardSpace {
     // blocks with the most work, over all pieces, with a launch's cost for each piece and with what passes through
     // memory more than once (dX once more a cut of the vocabulary, dW a cut of the tokens).
     void choose_pieces(const Shape &s, bool want_dx, bool want_dw) {
-        const int64_t cells = kDzBytes / (2 * s.planes), m = ce_div(s.n, kBM), n = ce_div(s.vocab, kBN);
-        const int n_pairs = s.planes == 3 ? 6 : 1;
+        const int64_t cells = kDzBytes / (2 * s.dz_planes), m = ce_div(s.n, kBM), n = ce_div(s.vocab, kBN);
         rows = m * kBM;
         cols = n * kBN;
         if (rows * cols <= cells) return;
@@ -1201,8 +1248,8 @@ struct BackwardSpace {
             col_cuts = ce_div(n, pn);
             Product x, w;
             products(s, want_dx, want_dw, pm * kBM, pn * kBN, &x, &w);
-            const int64_t steps = split_and_deal(x, w, n_pairs).steps +
-                                  ce_div(pm * pn, kPairs) * (ce_div(s.dim, kBK) * n_pairs + 1) + 2 * kLaunchSteps;
+            const int64_t steps = split_and_deal(x, w, s.product_pairs()).steps +
+                                  ce_div(pm * pn, kPairs) * (ce_div(s.dim, kBK) * s.logit_pairs() + 1) + 2 * kLaunchSteps;
             const int64_t again = ((col_cuts - 1) * s.n + (row_cuts - 1) * s.vocab) * s.dim / kStepElements;
             const int64_t cost = row_cuts * col_cuts * steps + again;
             if (best < 0 || cost < best) {
@@ -1244,7 +1291,14 @@ struct Maps {
 };
 
 template <typename T, int kKind> int launch_ce(const Maps &m, const Params &p, int pairs, cudaStream_t stream) {
-    BPT_CUDA(cudaFuncSetAttribute(linear_ce_kernel<T, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kKind)));
+    // once per device; two threads that meet here do it twice
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    BPT_CUDA(cudaGetDevice(&device));
+    if (device >= 64 || !(done.load(std::memory_order_relaxed) >> device & 1)) {
+        BPT_CUDA(cudaFuncSetAttribute(linear_ce_kernel<T, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kKind)));
+        if (device < 64) done.fetch_or(uint64_t(1) << device);
+    }
     linear_ce_kernel<T, kKind><<<2 * pairs, kThreads, smem_bytes(kKind), stream>>>(m.a, m.b, m.c, m.d, m.e, p);
     BPT_LAUNCH_CHECK();
     return BPT_OK;
@@ -1292,7 +1346,8 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     p.n_tiles = s.v_tiles();
     p.k_tiles = static_cast<int>(ce_div(s.dim, kBK));
     p.n_ext = s.vocab;
-    p.n_pairs = s.planes == 3 ? 6 : 1;
+    p.n_pairs = s.logit_pairs();
+    p.dz_planes = s.dz_planes;
     p.status = f.status;
     p.n_rows = s.n;
     p.ignore_index = c.ignore_index;
@@ -1302,6 +1357,7 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     p.partial = f.partial;
     p.z_target = f.z_target;
     p.ticket = f.ticket;
+    p.starts = 1;
     p.smoothed = c.smoothing != 0.f;
     const int pairs = pairs_for(s.m_tiles() * s.v_tiles());
     BPT_TRY((launch_ce<T, kStats>(maps, p, pairs, stream)));
@@ -1337,7 +1393,6 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     constexpr bool kHalf = kIsHalf<T>;
     constexpr bool kFloat = std::is_same<T, float>::value;
     Operand x{c.x, c.ldx, 0}, w{c.w, c.ldw, 0};
-    BPT_CUDA(cudaMemsetAsync(f.status, 0, sizeof(int), stream));
     if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, f.x, c.target, c.ignore_index, stream, &x));
     if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, f.w, nullptr, 0, stream, &w));
     const int64_t clean_ld = ce_div(s.dim, 8) * 8;
@@ -1361,8 +1416,11 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     maps.e = maps.d;
     if (f.clean) BPT_TRY(make_map(&maps.e, kHalf, f.x_clean, s.n, s.dim, clean_ld, 1, 0, 64));
     Params p{};
-    p.n_pairs = s.planes == 3 ? 6 : 1;
+    p.n_pairs = s.logit_pairs();
+    p.dz_planes = s.dz_planes;
     p.status = f.status;
+    p.ticket = f.ticket;
+    p.spoilt = db;
     p.n_rows = s.n;
     p.ignore_index = c.ignore_index;
     p.vocab = s.vocab;
@@ -1391,8 +1449,9 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             g.n_ext = static_cast<int>(cols);
             g.m_ext = static_cast<int>(rows);
             g.a0 = static_cast<int>(n0);
+            g.starts = n0 == 0 && v0 == 0;
             g.b0 = static_cast<int>(v0);
-            BPT_TRY(make_map(&grad_maps.c, kHalf, f.dz, rows, cols, f.dz_ld, s.planes, f.dz_plane, 32, kFloat ? 32 : 64));
+            BPT_TRY(make_map(&grad_maps.c, kHalf, f.dz, rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, 32, s.dz_planes == 1 ? 64 : 32));
             const int pairs = pairs_for(static_cast<int64_t>(g.m_tiles) * g.n_tiles);
             BPT_TRY((launch_ce<T, kGrad>(grad_maps, g, pairs, stream)));
             if (db) {
@@ -1401,12 +1460,13 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
                 BPT_LAUNCH_CHECK();
             }
             if (!dx && !dw) continue;
-            BPT_TRY(make_map(&maps.a, kHalf, f.dz, rows, cols, f.dz_ld, s.planes, f.dz_plane, kRows));
-            BPT_TRY(make_map(&maps.c, kHalf, f.dz, rows, cols, f.dz_ld, s.planes, f.dz_plane, 64));
+            BPT_TRY(make_map(&maps.a, kHalf, f.dz, rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, kRows));
+            BPT_TRY(make_map(&maps.c, kHalf, f.dz, rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, 64));
             Params q = p;
             BackwardSpace::products(s, dx, dw, rows, cols, &q.product[0], &q.product[1]);
             Product &px = q.product[0], &pw = q.product[1];
-            const Deal d = split_and_deal(px, pw, p.n_pairs);
+            const Deal d = split_and_deal(px, pw, s.product_pairs());
+            q.n_pairs = s.product_pairs();
             q.first = d.first;
             q.busy = d.busy;
             q.after_busy = d.after_busy;
@@ -1437,8 +1497,6 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             }
         }
     }
-    linear_ce_poison_kernel<T><<<1, 1, 0, stream>>>(f.status, static_cast<T *>(dx), static_cast<T *>(dw), static_cast<T *>(db));
-    BPT_LAUNCH_CHECK();
     return BPT_OK;
 }
 
