@@ -19,6 +19,16 @@ def graphop_extension():
     return _graphop_ext
 
 
+def train_extension():
+    """The torch C++ extension with the differentiable training operators (csrc_torch/train_ext.cpp) that norm.py and
+    loss.py call.  Raises ImportError with the build command when it has not been built."""
+    try:
+        from . import _train_ext
+    except ImportError as e:
+        raise ImportError("bpt_b200._train_ext is not built (%s); run `python -m bpt_b200.build`" % e)
+    return _train_ext
+
+
 def install_dropin(binding=None):
     """Registers this package's `graphop` and `graphbuilder` under the top-level module
     names the reference imports (`from graphop import *`, modules/op.py:2;

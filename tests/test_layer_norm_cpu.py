@@ -7,6 +7,7 @@ import torch
 def lib():
     from bpt_b200 import _lib, build
     build.build()
+    build.build_torch_ext(name="_train_ext")
     return _lib.lib()
 
 

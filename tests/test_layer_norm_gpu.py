@@ -275,3 +275,18 @@ def test_blocks_train_through_it():
             models.add_layer_norm = kept
         for k, p in blk.named_parameters():
             assert float((p.grad - got[k]).abs().max()) <= 1e-4 * float(p.grad.abs().max()), k
+
+
+def test_second_derivative_is_refused():
+    """create_graph may be asked for (other parts of a model may need it); the derivative of this backward is an error."""
+    from bpt_b200.loss import linear_cross_entropy
+    from bpt_b200.norm import layer_norm
+    x, r, w, b, _ = inputs(4, 16, torch.float32, True)
+    x.requires_grad_(True)
+    t = torch.zeros(4, dtype=torch.long, device="cuda")
+    for f in (lambda: layer_norm(x, w, b, residual=r).square().sum(), lambda: linear_cross_entropy(x, r.detach(), t)):
+        plain, = torch.autograd.grad(f(), x)
+        g, = torch.autograd.grad(f(), x, create_graph=True)
+        assert torch.equal(g.detach(), plain)
+        with pytest.raises(RuntimeError, match="once"):
+            g.sum().backward()
