@@ -11,186 +11,94 @@
 //     d gamma = sum over rows of gy n,   d beta = sum over rows of gy
 // so one pass that reads x, r and gy and writes d a has everything; the sums over rows stay in the registers of
 // the threads that own a column, then go through one partial row per block (no atomics: the order is fixed).
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
+#include "tma.cuh"
 
 namespace bpt {
 namespace {
 
-constexpr int kLnWarps = 8;
-
-// load8 / store8: 8 elements = one 16-byte piece (bf16, fp16) or two (fp32), widened to fp32.
-__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&f)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4 *>(p);
-    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = __bfloat1622float2(h[i]);
-        f[2 * i] = v.x;
-        f[2 * i + 1] = v.y;
-    }
-}
-__device__ __forceinline__ void load8(const __half *p, float (&f)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4 *>(p);
-    const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = __half22float2(h[i]);
-        f[2 * i] = v.x;
-        f[2 * i + 1] = v.y;
-    }
-}
-__device__ __forceinline__ void load8(const float *p, float (&f)[8]) {
-    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&f)[8]) {
-    uint4 raw;
-    __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4 *>(p) = raw;
-}
-__device__ __forceinline__ void store8(__half *p, const float (&f)[8]) {
-    uint4 raw;
-    __half2 *h = reinterpret_cast<__half2 *>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4 *>(p) = raw;
-}
-__device__ __forceinline__ void store8(float *p, const float (&f)[8]) {
-    *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4 *>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
-}
-
-// kVecs pieces of 8 elements per lane: dim <= 256 * kVecs.  A warp per row.
-template <typename T, int kVecs>
-__global__ void __launch_bounds__(kLnWarps * 32)
-add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma,
-                      const T *__restrict__ beta, float eps, T *__restrict__ y, float *__restrict__ mean_out,
-                      float *__restrict__ rstd_out, int64_t n_rows, int dim) {
-    const int lane = threadIdx.x & 31;
-    const int64_t row = blockIdx.x * static_cast<int64_t>(kLnWarps) + (threadIdx.x >> 5);
-    if (row >= n_rows) return;
-    const T *xr = x + row * dim;
-    const T *rr = r ? r + row * dim : nullptr;
-    float v[kVecs][8];
-    float sum = 0.f;
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        const int c = (u * 32 + lane) * 8;
-        if (c < dim) {
-            load8(xr + c, v[u]);
-            if (rr) {
-                float t[8];
-                load8(rr + c, t);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] += t[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum += v[u][i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-        }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float mean = sum / static_cast<float>(dim);
-    float sq = 0.f;
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        const int c = (u * 32 + lane) * 8;
-        if (c < dim) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = v[u][i] - mean;
-                sq = fmaf(d, d, sq);
-            }
-        }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-    const float rstd = rsqrtf(sq / static_cast<float>(dim) + eps);  // biased variance, as torch.nn.LayerNorm
-    if (mean_out && lane == 0) {
-        mean_out[row] = mean;
-        rstd_out[row] = rstd;
-    }
-    T *yr = y + row * dim;
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        const int c = (u * 32 + lane) * 8;
-        if (c < dim) {
-            float g[8], b[8], out[8];
-            if (gamma) load8(gamma + c, g);
-            if (beta) load8(beta + c, b);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float n = (v[u][i] - mean) * rstd;
-                out[i] = fmaf(n, gamma ? g[i] : 1.f, beta ? b[i] : 0.f);
-            }
-            store8(yr + c, out);
-        }
-    }
-}
-
-template <typename T>
-int launch_add_layer_norm(const void *x, const void *r, const void *gamma, const void *beta, float eps, void *y,
-                          float *mean, float *rstd, int64_t n_rows, int dim, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>((n_rows + kLnWarps - 1) / kLnWarps);
-    const int vecs = (dim + 255) / 256;
-#define BPT_LN_LAUNCH(V)                                                                                      \
-    add_layer_norm_kernel<T, V><<<grid, kLnWarps * 32, 0, stream>>>(                                          \
-        static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(gamma),                  \
-        static_cast<const T *>(beta), eps, static_cast<T *>(y), mean, rstd, n_rows, dim)
-    if (vecs <= 1) BPT_LN_LAUNCH(1);
-    else if (vecs <= 2) BPT_LN_LAUNCH(2);
-    else if (vecs <= 4) BPT_LN_LAUNCH(4);
-    else if (vecs <= 8) BPT_LN_LAUNCH(8);
-    else BPT_LN_LAUNCH(16);
-#undef BPT_LN_LAUNCH
-    BPT_LAUNCH_CHECK();
-    return BPT_OK;
-}
-
-// ---- any width: a row belongs to `tpr` threads of a block (a power of two from 32 to 512), each with kVecs pieces
-// of kVec neighbouring elements, at most kPerThread elements in all, so the column sums of the backward fit in
+// A row belongs to `tpr` threads of a block (a power of two from 32 to 512), each with kVecs pieces of kVec
+// neighbouring elements, at most kPerThread elements in all, so that a row (and the backward's column sums) stays in
 // registers.  kVec is the widest of 8, 4, 1 that the width and the pointers allow.
 constexpr int kPerThread = 16;
 constexpr int kMaxDim = 512 * kPerThread;
 constexpr int kMaxGrid = 148 * 4;  // blocks of the backward = partial rows of d gamma and d beta
 
-template <typename T, int kVec> __device__ __forceinline__ void load_vec(const T *p, float (&f)[kVec]) {
-    if constexpr (kVec == 8) {
-        load8(p, f);
-    } else if constexpr (kVec == 4 && sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(p);
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    } else if constexpr (kVec == 4) {
-        const uint2 raw = *reinterpret_cast<const uint2 *>(p);
-        const T *h = reinterpret_cast<const T *>(&raw);
+// kVec elements as they lie in memory, in whole words (16-bit elements held one by one would take a register each).
+template <typename T, int kVec> struct Raw {
+    static constexpr int kWords = kVec * sizeof(T) >= 4 ? kVec * sizeof(T) / 4 : 1;
+    uint32_t w[kWords];
+};
+template <typename T, int kVec> __device__ __forceinline__ Raw<T, kVec> load_raw(const T *p) {
+    Raw<T, kVec> r;
+    if constexpr (kVec * sizeof(T) >= 16) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = to_acc<T>(h[i]);
+        for (int i = 0; i < Raw<T, kVec>::kWords; i += 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
+            r.w[i] = v.x;
+            r.w[i + 1] = v.y;
+            r.w[i + 2] = v.z;
+            r.w[i + 3] = v.w;
+        }
+    } else if constexpr (kVec * sizeof(T) == 8) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        r.w[0] = v.x;
+        r.w[1] = v.y;
+    } else if constexpr (sizeof(T) == 4) {
+        r.w[0] = *reinterpret_cast<const uint32_t *>(p);
     } else {
-        f[0] = to_acc<T>(*p);
+        r.w[0] = *reinterpret_cast<const uint16_t *>(p);
+    }
+    return r;
+}
+template <typename T, int kVec> __device__ __forceinline__ void widen(const Raw<T, kVec> &r, float (&f)[kVec]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) f[i] = __uint_as_float(r.w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; i += 2) {
+            const uint32_t w = r.w[i / 2];
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                f[i] = v.x;
+                if (kVec > 1) f[i + 1 < kVec ? i + 1 : 0] = kVec > 1 ? v.y : v.x;
+            } else {
+                f[i] = __uint_as_float(w << 16);
+                if (kVec > 1) f[i + 1 < kVec ? i + 1 : 0] = __uint_as_float(w & 0xFFFF0000u);
+            }
+        }
     }
 }
 template <typename T, int kVec> __device__ __forceinline__ void store_vec(T *p, const float (&f)[kVec]) {
-    if constexpr (kVec == 8) {
-        store8(p, f);
-    } else if constexpr (kVec == 4 && sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    } else if constexpr (kVec == 4) {
-        uint2 raw;
-        T *h = reinterpret_cast<T *>(&raw);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = from_acc<T>(f[i]);
-        *reinterpret_cast<uint2 *>(p) = raw;
-    } else {
+    if constexpr (kVec == 1) {
         *p = from_acc<T>(f[0]);
+    } else {
+        constexpr int kWords = Raw<T, kVec>::kWords;
+        uint32_t w[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                w[i] = __float_as_uint(f[i]);
+            } else if constexpr (std::is_same<T, __half>::value) {
+                const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        if constexpr (kWords == 2) {
+            *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4)
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint32_t *>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
     }
 }
 
@@ -213,154 +121,60 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float *slot) {
     return v;
 }
 
-template <typename T, int kVec, int kVecs>
-__global__ void __launch_bounds__(512)
-layer_norm_any_kernel(const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma,
-                      const T *__restrict__ beta, float eps, T *__restrict__ y, float *__restrict__ mean_out,
-                      float *__restrict__ rstd_out, int64_t n_rows, int dim, int tpr) {
-    __shared__ float slots[2][16];
-    const int t = threadIdx.x & (tpr - 1);
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
-    const bool live = row < n_rows;  // every thread of the block takes part in the barriers
-    const int64_t base = live ? row * dim : 0;
-    float v[kVecs][kVec];
-    float sum = 0.f;
+// Elementwise arithmetic of a piece, two elements an instruction where there are two (the same roundings).
+template <int n> __device__ __forceinline__ void add(float (&a)[n], const float (&b)[n]) {
+    if constexpr (n == 1) {
+        a[0] += b[0];
+    } else {
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        const int c = (u * tpr + t) * kVec;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) v[u][i] = 0.f;
-        if (live && c < dim) {
-            load_vec<T, kVec>(x + base + c, v[u]);
-            if (r) {
-                float w[kVec];
-                load_vec<T, kVec>(r + base + c, w);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) v[u][i] += w[i];
-            }
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) sum += v[u][i];
-        }
-    }
-    const float mean = row_sum(sum, tpr, slots[0]) / static_cast<float>(dim);
-    float sq = 0.f;
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        if ((u * tpr + t) * kVec < dim) {
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                const float d = v[u][i] - mean;
-                sq = fmaf(d, d, sq);
-            }
-        }
-    }
-    const float rstd = rsqrtf(row_sum(sq, tpr, slots[1]) / static_cast<float>(dim) + eps);
-    if (!live) return;
-    if (mean_out && t == 0) {
-        mean_out[row] = mean;
-        rstd_out[row] = rstd;
-    }
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        const int c = (u * tpr + t) * kVec;
-        if (c < dim) {
-            float g[kVec], b[kVec], out[kVec];
-            if (gamma) load_vec<T, kVec>(gamma + c, g);
-            if (beta) load_vec<T, kVec>(beta + c, b);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i)
-                out[i] = fmaf((v[u][i] - mean) * rstd, gamma ? g[i] : 1.f, beta ? b[i] : 0.f);
-            store_vec<T, kVec>(y + base + c, out);
+        for (int i = 0; i < n; i += 2) {
+            const float2 s = tc5::add2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+            a[i] = s.x;
+            a[i + 1] = s.y;
         }
     }
 }
-
-template <typename T, int kVec, int kVecs>
-__global__ void __launch_bounds__(512)
-layer_norm_backward_kernel(const T *__restrict__ gy, const T *__restrict__ x, const T *__restrict__ r,
-                           const T *__restrict__ gamma, const float *__restrict__ mean_in,
-                           const float *__restrict__ rstd_in, T *__restrict__ da, float *__restrict__ partial,
-                           int64_t n_rows, int dim, int tpr) {
-    __shared__ float slots[2][2][16];
-    extern __shared__ float sums[];  // [rows of the block][dim]
-    const int t = threadIdx.x & (tpr - 1), rows_here = blockDim.x / tpr, mine = threadIdx.x / tpr;
-    const float inv_dim = 1.f / static_cast<float>(dim);
-    float g[kVecs][kVec], acc_g[kVecs][kVec], acc_b[kVecs][kVec];
+template <int n> __device__ __forceinline__ void add(float (&a)[n], float b) {
+    float all[n];
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
+    for (int i = 0; i < n; ++i) all[i] = b;
+    add(a, all);
+}
+template <int n> __device__ __forceinline__ void multiply(float (&a)[n], const float (&b)[n]) {
+    if constexpr (n == 1) {
+        a[0] *= b[0];
+    } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            g[u][i] = 1.f;
-            acc_g[u][i] = acc_b[u][i] = 0.f;
-        }
-        const int c = (u * tpr + t) * kVec;
-        if (gamma && c < dim) load_vec<T, kVec>(gamma + c, g[u]);
-    }
-    int parity = 0;
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_here; row0 < n_rows;
-         row0 += static_cast<int64_t>(gridDim.x) * rows_here) {
-        const int64_t row = row0 + mine;
-        const bool live = row < n_rows;
-        const int64_t base = live ? row * dim : 0;
-        const float mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
-        float n[kVecs][kVec], q[kVecs][kVec];
-        float sq = 0.f, sqn = 0.f;
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            const int c = (u * tpr + t) * kVec;
-            if (live && c < dim) {
-                load_vec<T, kVec>(x + base + c, n[u]);
-                load_vec<T, kVec>(gy + base + c, q[u]);
-                if (r) {
-                    float w[kVec];
-                    load_vec<T, kVec>(r + base + c, w);
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) n[u][i] += w[i];
-                }
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    n[u][i] = (n[u][i] - mean) * rstd;
-                    acc_g[u][i] = fmaf(q[u][i], n[u][i], acc_g[u][i]);
-                    acc_b[u][i] += q[u][i];
-                    q[u][i] *= g[u][i];
-                    sq += q[u][i];
-                    sqn = fmaf(q[u][i], n[u][i], sqn);
-                }
-            }
-        }
-        if (da) {
-            // both sums, then one barrier for the pair when a row spans warps
-            sq = warp_sum(sq);
-            sqn = warp_sum(sqn);
-            if (tpr > 32) {
-                const int warp = threadIdx.x >> 5, per_row = tpr >> 5, first = warp / per_row * per_row;
-                if ((threadIdx.x & 31) == 0) {
-                    slots[parity][0][warp] = sq;
-                    slots[parity][1][warp] = sqn;
-                }
-                __syncthreads();  // the other parity's slots were last read before this barrier
-                sq = sqn = 0.f;
-                for (int i = 0; i < per_row; ++i) {
-                    sq += slots[parity][0][first + i];
-                    sqn += slots[parity][1][first + i];
-                }
-                parity ^= 1;
-            }
-            const float mq = sq * inv_dim, mqn = sqn * inv_dim;
-#pragma unroll
-            for (int u = 0; u < kVecs; ++u) {
-                const int c = (u * tpr + t) * kVec;
-                if (live && c < dim) {
-                    float out[kVec];
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) out[i] = rstd * (q[u][i] - mq - n[u][i] * mqn);
-                    store_vec<T, kVec>(da + base + c, out);
-                }
-            }
+        for (int i = 0; i < n; i += 2) {
+            const float2 s = tc5::mul2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+            a[i] = s.x;
+            a[i + 1] = s.y;
         }
     }
-    if (!partial) return;
-    // the block's rows of sums -> one partial row: [block][d gamma, d beta][dim]
+}
+template <int n> __device__ __forceinline__ void multiply(float (&a)[n], float b) {
+    float all[n];
+#pragma unroll
+    for (int i = 0; i < n; ++i) all[i] = b;
+    multiply(a, all);
+}
+// c += a b
+template <int n> __device__ __forceinline__ void multiply_add(float (&c)[n], const float (&a)[n], const float (&b)[n]) {
+    if constexpr (n == 1) {
+        c[0] = fmaf(a[0], b[0], c[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < n; i += 2) {
+            const float2 s = tc5::fma2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), make_float2(c[i], c[i + 1]));
+            c[i] = s.x;
+            c[i + 1] = s.y;
+        }
+    }
+}
+// The sums of a block's rows -> one partial row: [block][d gamma, d beta][dim].
+template <int kVec, int kVecs>
+__device__ __forceinline__ void store_partial(const float (&acc_g)[kVecs][kVec], const float (&acc_b)[kVecs][kVec], float *sums, float *partial,
+                                              int t, int tpr, int rows_here, int mine, int dim) {
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
@@ -379,6 +193,184 @@ layer_norm_backward_kernel(const T *__restrict__ gy, const T *__restrict__ x, co
             partial[(static_cast<int64_t>(blockIdx.x) * 2 + which) * dim + c] = s;
         }
     }
+}
+
+template <typename T, int kVec, int kVecs, bool kHasR>
+__global__ void __launch_bounds__(512)
+layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma, const T *__restrict__ beta, float eps,
+                  T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int64_t n_rows, int dim, int tpr) {
+    __shared__ float slots[2][16];
+    const int t = threadIdx.x & (tpr - 1);
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
+    const bool live = row < n_rows;  // every thread of the block takes part in the barriers
+    const int64_t at = row * dim + t * kVec;
+    const int step = tpr * kVec;
+    float v[kVecs][kVec];
+    float sum = 0.f;
+    Raw<T, kVec> a[kVecs], b[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        if (live && u * step + t * kVec < dim) {
+            a[u] = load_raw<T, kVec>(x + at + u * step);
+            if constexpr (kHasR) b[u] = load_raw<T, kVec>(r + at + u * step);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        if (live && u * step + t * kVec < dim) {
+            widen(a[u], v[u]);
+            if constexpr (kHasR) {
+                float w[kVec];
+                widen(b[u], w);
+                add(v[u], w);
+            }
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) sum += v[u][i];
+        }
+    }
+    // gamma and beta travel while the sums are made
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        if (u * step + t * kVec < dim) {
+            if (gamma) a[u] = load_raw<T, kVec>(gamma + t * kVec + u * step);
+            if (beta) b[u] = load_raw<T, kVec>(beta + t * kVec + u * step);
+        }
+    }
+    const float mean = row_sum(sum, tpr, slots[0]) / static_cast<float>(dim);
+    float sq = 0.f;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        if (live && u * step + t * kVec < dim) {
+            add(v[u], -mean);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) sq = fmaf(v[u][i], v[u][i], sq);
+        }
+    }
+    const float rstd = rsqrtf(row_sum(sq, tpr, slots[1]) / static_cast<float>(dim) + eps);  // biased variance, as torch.nn.LayerNorm
+    if (!live) return;
+    if (mean_out && t == 0) {
+        mean_out[row] = mean;
+        rstd_out[row] = rstd;
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        if (u * step + t * kVec < dim) {
+            multiply(v[u], rstd);
+            float g[kVec], c[kVec];
+            if (gamma) {
+                widen(a[u], g);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) g[i] = 1.f;
+            }
+            if (beta) {
+                widen(b[u], c);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) c[i] = 0.f;
+            }
+            multiply_add(c, v[u], g);
+            store_vec<T, kVec>(y + at + u * step, c);
+        }
+    }
+}
+
+template <typename T, int kVec, int kVecs, bool kHasR, int kBlock>
+__global__ void __launch_bounds__(kBlock, kBlock == 256 ? 2 : 1)
+layer_norm_backward_kernel(const T *__restrict__ gy, const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma,
+                           const float *__restrict__ mean_in, const float *__restrict__ rstd_in, T *__restrict__ da,
+                           float *__restrict__ partial, int64_t n_rows, int dim, int tpr) {
+    __shared__ float slots[2][2][16];
+    extern __shared__ float sums[];  // [rows of the block][dim]
+    const int t = threadIdx.x & (tpr - 1), rows_here = kBlock / tpr, mine = threadIdx.x / tpr, step = tpr * kVec;
+    const float inv_dim = 1.f / static_cast<float>(dim);
+    Raw<T, kVec> gm[kVecs];
+    float acc_g[kVecs][kVec], acc_b[kVecs][kVec];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) acc_g[u][i] = acc_b[u][i] = 0.f;
+        if (gamma && u * step + t * kVec < dim) gm[u] = load_raw<T, kVec>(gamma + t * kVec + u * step);
+    }
+    int parity = 0;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_here; row0 < n_rows; row0 += static_cast<int64_t>(gridDim.x) * rows_here) {
+        const int64_t row = row0 + mine, at = row * dim + t * kVec;
+        const bool live = row < n_rows;
+        Raw<T, kVec> xv[kVecs], rv[kHasR ? kVecs : 1], gv[kVecs];
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            if (live && u * step + t * kVec < dim) {
+                xv[u] = load_raw<T, kVec>(x + at + u * step);
+                if constexpr (kHasR) rv[u] = load_raw<T, kVec>(r + at + u * step);
+                gv[u] = load_raw<T, kVec>(gy + at + u * step);
+            }
+        }
+        const float mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
+        float n[kVecs][kVec], q[kVecs][kVec], sq[kVec], sqn[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) sq[i] = sqn[i] = 0.f;
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            if (live && u * step + t * kVec < dim) {
+                widen(xv[u], n[u]);
+                float w[kVec];
+                if constexpr (kHasR) {
+                    widen(rv[u], w);
+                    add(n[u], w);
+                }
+                add(n[u], -mean);
+                multiply(n[u], rstd);
+                widen(gv[u], q[u]);
+                multiply_add(acc_g[u], q[u], n[u]);
+                add(acc_b[u], q[u]);
+                if (gamma) {
+                    widen(gm[u], w);
+                    multiply(q[u], w);
+                }
+                add(sq, q[u]);
+                multiply_add(sqn, q[u], n[u]);
+            }
+        }
+        if (da) {
+            // both sums, then one barrier for the pair when a row spans warps
+            float s = 0.f, sn = 0.f;
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                s += sq[i];
+                sn += sqn[i];
+            }
+            s = warp_sum(s);
+            sn = warp_sum(sn);
+            if (tpr > 32) {
+                const int warp = threadIdx.x >> 5, per_row = tpr >> 5, first = warp / per_row * per_row;
+                if ((threadIdx.x & 31) == 0) {
+                    slots[parity][0][warp] = s;
+                    slots[parity][1][warp] = sn;
+                }
+                __syncthreads();  // the other parity's slots were last read before this barrier
+                s = sn = 0.f;
+                for (int i = 0; i < per_row; ++i) {
+                    s += slots[parity][0][first + i];
+                    sn += slots[parity][1][first + i];
+                }
+                parity ^= 1;
+            }
+            const float mq = -s * inv_dim, mqn = -sn * inv_dim;
+#pragma unroll
+            for (int u = 0; u < kVecs; ++u) {
+                if (live && u * step + t * kVec < dim) {
+                    float w[kVec];
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) w[i] = mqn;
+                    add(q[u], mq);
+                    multiply_add(q[u], n[u], w);
+                    multiply(q[u], rstd);
+                    store_vec<T, kVec>(da + at + u * step, q[u]);
+                }
+            }
+        }
+    }
+    if (partial) store_partial(acc_g, acc_b, sums, partial, t, tpr, rows_here, mine, dim);
 }
 
 // d gamma and d beta from the partial rows, in block order within a thread and thread order within a column.
@@ -435,25 +427,28 @@ template <typename F> int ln_dispatch(const LnLayout &l, int dim, F f) {
                   : f(std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
 }
 
-template <typename T>
-int launch_layer_norm_any(const void *x, const void *r, const void *gamma, const void *beta, float eps, void *y,
-                          float *mean, float *rstd, int64_t n_rows, int dim, cudaStream_t stream) {
-    const LnLayout l = ln_layout(dim, ln_vec(dim, sizeof(T), {x, r, gamma, beta, y}));
-    const int64_t rows_here = l.block / l.tpr;
-    const unsigned grid = static_cast<unsigned>((n_rows + rows_here - 1) / rows_here);
-    return ln_dispatch(l, dim, [&](auto vec, auto vecs) -> int {
-        layer_norm_any_kernel<T, vec.value, vecs.value><<<grid, l.block, 0, stream>>>(
-            static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(gamma),
-            static_cast<const T *>(beta), eps, static_cast<T *>(y), mean, rstd, n_rows, dim, l.tpr);
-        BPT_LAUNCH_CHECK();
-        return BPT_OK;
-    });
-}
-
 int64_t ln_backward_grid(int64_t n_rows, int dim) {
     const LnLayout l = ln_layout(dim, 1);
     const int64_t blocks = (n_rows + l.block / l.tpr - 1) / (l.block / l.tpr);
     return blocks < kMaxGrid ? blocks : kMaxGrid;
+}
+
+template <typename T>
+int launch_layer_norm(const void *x, const void *r, const void *gamma, const void *beta, float eps, void *y, float *mean, float *rstd,
+                      int64_t n_rows, int dim, cudaStream_t stream) {
+    const LnLayout l = ln_layout(dim, ln_vec(dim, sizeof(T), {x, r, gamma, beta, y}));
+    const int64_t rows_here = l.block / l.tpr;
+    const unsigned grid = static_cast<unsigned>((n_rows + rows_here - 1) / rows_here);
+    return ln_dispatch(l, dim, [&](auto vec, auto vecs) -> int {
+        auto go = [&](auto has_r) -> int {
+            layer_norm_kernel<T, vec.value, vecs.value, has_r.value><<<grid, l.block, 0, stream>>>(
+                static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(gamma), static_cast<const T *>(beta), eps,
+                static_cast<T *>(y), mean, rstd, n_rows, dim, l.tpr);
+            BPT_LAUNCH_CHECK();
+            return BPT_OK;
+        };
+        return r ? go(std::true_type()) : go(std::false_type());
+    });
 }
 
 template <typename T>
@@ -463,16 +458,18 @@ int launch_layer_norm_backward(const void *gy, const void *x, const void *r, con
     const LnLayout l = ln_layout(dim, ln_vec(dim, sizeof(T), {gy, x, r, gamma, da}));
     const unsigned grid = static_cast<unsigned>(ln_backward_grid(n_rows, dim));
     const size_t smem = sizeof(float) * static_cast<size_t>(l.block / l.tpr) * dim;  // at most 512 * 16 floats
-    if (n_rows > 0) {
-        const int rc = ln_dispatch(l, dim, [&](auto vec, auto vecs) -> int {
-            layer_norm_backward_kernel<T, vec.value, vecs.value><<<grid, l.block, smem, stream>>>(
-                static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const T *>(r),
-                static_cast<const T *>(gamma), mean, rstd, static_cast<T *>(da), partial, n_rows, dim, l.tpr);
+    const int rc = ln_dispatch(l, dim, [&](auto vec, auto vecs) -> int {
+        auto go = [&](auto has_r) -> int {
+            auto kernel = l.block == 256 ? layer_norm_backward_kernel<T, vec.value, vecs.value, has_r.value, 256>
+                                         : layer_norm_backward_kernel<T, vec.value, vecs.value, has_r.value, 512>;
+            kernel<<<grid, l.block, smem, stream>>>(static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const T *>(r),
+                                                    static_cast<const T *>(gamma), mean, rstd, static_cast<T *>(da), partial, n_rows, dim, l.tpr);
             BPT_LAUNCH_CHECK();
             return BPT_OK;
-        });
-        if (rc != BPT_OK) return rc;
-    }
+        };
+        return r ? go(std::true_type()) : go(std::false_type());
+    });
+    if (rc != BPT_OK) return rc;
     if (partial) {
         layer_norm_reduce_kernel<T><<<(2 * dim + 31) / 32, dim3(32, kReduceRows), 0, stream>>>(
             partial, static_cast<int>(grid), dim, static_cast<T *>(dgamma), static_cast<T *>(dbeta));
@@ -490,7 +487,6 @@ extern "C" int bpt_add_layer_norm(const void *x, const void *r, const void *gamm
                                   void *y, int64_t n_rows, int dim, int dtype, bpt_stream_t stream_) {
     BPT_CHECK_ARG(n_rows >= 0 && dim >= 8 && dim % 8 == 0 && dim <= 4096,
                   "add_layer_norm: dim must be a multiple of 8 in [8, 4096] (got %d)", dim);
-    BPT_CHECK_ARG(n_rows < (int64_t(1) << 31) * kLnWarps, "add_layer_norm: too many rows");
     if (n_rows == 0) return BPT_OK;
     BPT_CHECK_ARG(x && y, "add_layer_norm: null tensor");
     BPT_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(r) | reinterpret_cast<uintptr_t>(gamma) |
@@ -508,12 +504,7 @@ extern "C" int bpt_layer_norm_forward(const void *x, const void *r, const void *
     BPT_CHECK_ARG(x && y, "layer_norm: null tensor");
     cudaStream_t stream = as_stream(stream_);
     const float e = static_cast<float>(eps);
-    // multiples of 8 up to 4096 keep the kernel of a warp per row
-    const bool warp_rows = dim <= 4096 && ln_vec(dim, 2, {x, r, gamma, beta, y}) == 8;
-    BPT_CHECK_ARG(n_rows < (int64_t(1) << 31) * (warp_rows ? kLnWarps : 1), "layer_norm: too many rows");
-#define BPT_LN_FORWARD(T)                                                                                       \
-    return warp_rows ? launch_add_layer_norm<T>(x, r, gamma, beta, e, y, mean, rstd, n_rows, dim, stream)        \
-                     : launch_layer_norm_any<T>(x, r, gamma, beta, e, y, mean, rstd, n_rows, dim, stream)
+#define BPT_LN_FORWARD(T) return launch_layer_norm<T>(x, r, gamma, beta, e, y, mean, rstd, n_rows, dim, stream)
     switch (dtype) {
         case BPT_F32: BPT_LN_FORWARD(float);
         case BPT_BF16: BPT_LN_FORWARD(__nv_bfloat16);

@@ -488,8 +488,8 @@ int bpt_add_layer_norm(const void *x, const void *r, const void *gamma, const vo
                        int64_t n_rows, int dim, int dtype, bpt_stream_t stream);
 
 /* The same for any dim from 1 to 8192 and any alignment, for training: mean and rstd (fp32, one per row; both or
- * neither may be NULL) are what bpt_layer_norm_backward reads.  Where bpt_add_layer_norm takes the arguments too,
- * y is the same bit for bit.  No counterpart in the reference, which spells it with torch operators.
+ * neither may be NULL) are what bpt_layer_norm_backward reads; y is that of bpt_add_layer_norm where both take the
+ * arguments.  No counterpart in the reference, which spells it with torch operators.
  *
  * bpt_layer_norm_backward: gy: gradient of y; x, r (may be NULL), gamma (may be NULL: ones), mean, rstd as in the
  * forward.  da: gradient of x + r, that is of x and of r; dgamma, dbeta (dim): sums over the rows.  Each of the three
