@@ -26,7 +26,7 @@ namespace {
 // registers.  kVec is the widest of 8, 4, 1 that the width and the pointers allow.
 constexpr int kPerThread = 16;
 constexpr int kMaxDim = 512 * kPerThread;
-constexpr int kMaxGrid = 148 * 4;  // blocks of the backward = partial rows of d gamma and d beta
+constexpr int kMaxGrid = 148 * 2;  // blocks of the backward = partial rows of d gamma and d beta
 
 // kVec elements as they lie in memory, in whole words (16-bit elements held one by one would take a register each).
 template <typename T, int kVec> struct Raw {
@@ -195,142 +195,215 @@ __device__ __forceinline__ void store_partial(const float (&acc_g)[kVecs][kVec],
     }
 }
 
-template <typename T, int kVec, int kVecs, bool kHasR>
-__global__ void __launch_bounds__(512)
+// Blocks are persistent (the backward's column sums then stay in registers).  Where pieces are 16 bytes or more, a
+// thread's pieces of the kAhead rows to come travel to shared memory by cp.async, into places that only this thread
+// reads: no barrier, no registers, and two or three rows a warp under way instead of one.
+template <typename T, int kVec, int kVecs, int kArrays, int kBlock, int kAhead> struct Rows {
+    static constexpr int kBytes = kVec * sizeof(T);
+    static constexpr int kSmem = kAhead * kArrays * kVecs * kBlock * kBytes;
+    const T *arrays[kArrays];
+    unsigned char *smem;
+    int64_t n_rows;
+    int dim, first, step, ahead;  // this thread's first column, columns from piece to piece
+
+    __device__ bool in(int u) const { return u * step + first < dim; }
+    __device__ unsigned char *place(int slot, int array, int u) const {
+        return smem + ((slot * kArrays + array) * kVecs + u) * (kBlock * kBytes) + threadIdx.x * kBytes;
+    }
+    __device__ void send(int64_t row, int slot) const {
+        if (row < n_rows) {
+#pragma unroll
+            for (int u = 0; u < kVecs; ++u) {
+                if (in(u)) {
+#pragma unroll
+                    for (int k = 0; k < kArrays; ++k)
+#pragma unroll
+                        for (int b = 0; b < kBytes; b += 16)
+                            tc5::cp_async16(tc5::smem_u32(place(slot, k, u) + b),
+                                            reinterpret_cast<const char *>(arrays[k] + row * dim + first + u * step) + b);
+                }
+            }
+        }
+        tc5::cp_async_commit();
+    }
+    __device__ void start(int64_t row, int64_t stride) {
+        ahead = 0;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) send(row + k * stride, k);
+    }
+    __device__ void get(int64_t row, Raw<T, kVec> (&v)[kArrays][kVecs]) const {
+        if constexpr (kAhead > 0) asm volatile("cp.async.wait_group %0;\n" ::"n"(kAhead > 0 ? kAhead - 1 : 0) : "memory");
+        if (row >= n_rows) return;
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            if (in(u)) {
+#pragma unroll
+                for (int k = 0; k < kArrays; ++k) {
+                    if constexpr (kAhead > 0) v[k][u] = load_raw<T, kVec>(reinterpret_cast<const T *>(place(ahead, k, u)));
+                    else v[k][u] = load_raw<T, kVec>(arrays[k] + row * dim + first + u * step);
+                }
+            }
+        }
+    }
+    // The places of the row that get() brought are free once its values have been used: the row kAhead further on.
+    __device__ void next(int64_t row, int64_t stride) {
+        if constexpr (kAhead > 0) {
+            send(row + kAhead * stride, ahead);
+            if (++ahead == kAhead) ahead = 0;
+        }
+    }
+};
+
+template <typename T, int kVec, int kVecs, bool kHasR, int kBlock, int kAhead>
+__global__ void __launch_bounds__(kBlock)
 layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma, const T *__restrict__ beta, float eps,
                   T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int64_t n_rows, int dim, int tpr) {
     __shared__ float slots[2][16];
-    const int t = threadIdx.x & (tpr - 1);
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
-    const bool live = row < n_rows;  // every thread of the block takes part in the barriers
-    const int64_t at = row * dim + t * kVec;
-    const int step = tpr * kVec;
-    float v[kVecs][kVec];
-    float sum = 0.f;
-    Raw<T, kVec> a[kVecs], b[kVecs];
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kArrays = kHasR ? 2 : 1;
+    const int t = threadIdx.x & (tpr - 1), rows_here = kBlock / tpr, step = tpr * kVec;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * rows_here;
+    Rows<T, kVec, kVecs, kArrays, kBlock, kAhead> rows;
+    rows.arrays[0] = x;
+    if constexpr (kHasR) rows.arrays[1] = r;
+    rows.smem = smem;
+    rows.n_rows = n_rows;
+    rows.dim = dim;
+    rows.first = t * kVec;
+    rows.step = step;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * rows_here + threadIdx.x / tpr;
+    rows.start(row, stride);
+    // every thread of the block takes part in the barriers: the loop ends for all when the block's first row is past the end
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_here; row0 < n_rows; row0 += stride, row += stride) {
+        const bool live = row < n_rows;
+        Raw<T, kVec> a[kArrays][kVecs];
+        rows.get(row, a);
+        float v[kVecs][kVec];
+        float sum = 0.f;
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        if (live && u * step + t * kVec < dim) {
-            a[u] = load_raw<T, kVec>(x + at + u * step);
-            if constexpr (kHasR) b[u] = load_raw<T, kVec>(r + at + u * step);
-        }
-    }
+        for (int u = 0; u < kVecs; ++u) {
+            if (live && rows.in(u)) {
+                widen(a[0][u], v[u]);
+                if constexpr (kHasR) {
+                    float w[kVec];
+                    widen(a[kArrays - 1][u], w);
+                    add(v[u], w);
+                }
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        if (live && u * step + t * kVec < dim) {
-            widen(a[u], v[u]);
-            if constexpr (kHasR) {
-                float w[kVec];
-                widen(b[u], w);
-                add(v[u], w);
+                for (int i = 0; i < kVec; ++i) sum += v[u][i];
             }
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) sum += v[u][i];
         }
-    }
-    // gamma and beta travel while the sums are made
+        rows.next(row, stride);
+        const float mean = row_sum(sum, tpr, slots[0]) / static_cast<float>(dim);
+        float sq = 0.f;
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        if (u * step + t * kVec < dim) {
-            if (gamma) a[u] = load_raw<T, kVec>(gamma + t * kVec + u * step);
-            if (beta) b[u] = load_raw<T, kVec>(beta + t * kVec + u * step);
-        }
-    }
-    const float mean = row_sum(sum, tpr, slots[0]) / static_cast<float>(dim);
-    float sq = 0.f;
+        for (int u = 0; u < kVecs; ++u) {
+            if (live && rows.in(u)) {
+                add(v[u], -mean);
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        if (live && u * step + t * kVec < dim) {
-            add(v[u], -mean);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) sq = fmaf(v[u][i], v[u][i], sq);
-        }
-    }
-    const float rstd = rsqrtf(row_sum(sq, tpr, slots[1]) / static_cast<float>(dim) + eps);  // biased variance, as torch.nn.LayerNorm
-    if (!live) return;
-    if (mean_out && t == 0) {
-        mean_out[row] = mean;
-        rstd_out[row] = rstd;
-    }
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        if (u * step + t * kVec < dim) {
-            multiply(v[u], rstd);
-            float g[kVec], c[kVec];
-            if (gamma) {
-                widen(a[u], g);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) g[i] = 1.f;
+                for (int i = 0; i < kVec; ++i) sq = fmaf(v[u][i], v[u][i], sq);
             }
-            if (beta) {
-                widen(b[u], c);
-            } else {
+        }
+        const float rstd = rsqrtf(row_sum(sq, tpr, slots[1]) / static_cast<float>(dim) + eps);  // biased variance, as torch.nn.LayerNorm
+        if (!live) continue;
+        if (mean_out && t == 0) {
+            mean_out[row] = mean;
+            rstd_out[row] = rstd;
+        }
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) c[i] = 0.f;
+        for (int u = 0; u < kVecs; ++u) {
+            if (rows.in(u)) {
+                multiply(v[u], rstd);
+                float g[kVec], c[kVec];
+                if (gamma) {
+                    widen(load_raw<T, kVec>(gamma + t * kVec + u * step), g);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) g[i] = 1.f;
+                }
+                if (beta) {
+                    widen(load_raw<T, kVec>(beta + t * kVec + u * step), c);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) c[i] = 0.f;
+                }
+                multiply_add(c, v[u], g);
+                store_vec<T, kVec>(y + row * dim + t * kVec + u * step, c);
             }
-            multiply_add(c, v[u], g);
-            store_vec<T, kVec>(y + at + u * step, c);
         }
     }
+    if constexpr (kAhead > 0) tc5::cp_async_wait_all();
 }
 
-template <typename T, int kVec, int kVecs, bool kHasR, int kBlock>
+template <typename T, int kVec, int kVecs, bool kHasR, int kBlock, int kAhead>
 __global__ void __launch_bounds__(kBlock, kBlock == 256 ? 2 : 1)
 layer_norm_backward_kernel(const T *__restrict__ gy, const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma,
                            const float *__restrict__ mean_in, const float *__restrict__ rstd_in, T *__restrict__ da,
                            float *__restrict__ partial, int64_t n_rows, int dim, int tpr) {
     __shared__ float slots[2][2][16];
-    extern __shared__ float sums[];  // [rows of the block][dim]
+    extern __shared__ __align__(16) unsigned char smem[];  // rows ahead; at the end the sums, [rows of the block][dim]
     const int t = threadIdx.x & (tpr - 1), rows_here = kBlock / tpr, mine = threadIdx.x / tpr, step = tpr * kVec;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * rows_here;
     const float inv_dim = 1.f / static_cast<float>(dim);
-    Raw<T, kVec> gm[kVecs];
+    constexpr int kArrays = kHasR ? 3 : 2;
+    Rows<T, kVec, kVecs, kArrays, kBlock, kAhead> rows;
+    rows.arrays[0] = x;
+    rows.arrays[1] = gy;
+    if constexpr (kHasR) rows.arrays[2] = r;
+    rows.smem = smem;
+    rows.n_rows = n_rows;
+    rows.dim = dim;
+    rows.first = t * kVec;
+    rows.step = step;
     float acc_g[kVecs][kVec], acc_b[kVecs][kVec];
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) acc_g[u][i] = acc_b[u][i] = 0.f;
-        if (gamma && u * step + t * kVec < dim) gm[u] = load_raw<T, kVec>(gamma + t * kVec + u * step);
     }
+    int64_t row = static_cast<int64_t>(blockIdx.x) * rows_here + mine;
+    float next_mean = 0.f, next_rstd = 0.f;  // a row ahead
+    if (row < n_rows) {
+        next_mean = mean_in[row];
+        next_rstd = rstd_in[row];
+    }
+    rows.start(row, stride);
     int parity = 0;
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_here; row0 < n_rows; row0 += static_cast<int64_t>(gridDim.x) * rows_here) {
-        const int64_t row = row0 + mine, at = row * dim + t * kVec;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_here; row0 < n_rows; row0 += stride, row += stride) {
         const bool live = row < n_rows;
-        Raw<T, kVec> xv[kVecs], rv[kHasR ? kVecs : 1], gv[kVecs];
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            if (live && u * step + t * kVec < dim) {
-                xv[u] = load_raw<T, kVec>(x + at + u * step);
-                if constexpr (kHasR) rv[u] = load_raw<T, kVec>(r + at + u * step);
-                gv[u] = load_raw<T, kVec>(gy + at + u * step);
-            }
+        Raw<T, kVec> v[kArrays][kVecs];
+        rows.get(row, v);
+        const float mean = next_mean, rstd = next_rstd;
+        if (row + stride < n_rows) {
+            next_mean = mean_in[row + stride];
+            next_rstd = rstd_in[row + stride];
         }
-        const float mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
         float n[kVecs][kVec], q[kVecs][kVec], sq[kVec], sqn[kVec];
 #pragma unroll
         for (int i = 0; i < kVec; ++i) sq[i] = sqn[i] = 0.f;
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
-            if (live && u * step + t * kVec < dim) {
-                widen(xv[u], n[u]);
+            if (live && rows.in(u)) {
+                widen(v[0][u], n[u]);
                 float w[kVec];
                 if constexpr (kHasR) {
-                    widen(rv[u], w);
+                    widen(v[kArrays - 1][u], w);
                     add(n[u], w);
                 }
                 add(n[u], -mean);
                 multiply(n[u], rstd);
-                widen(gv[u], q[u]);
+                widen(v[1][u], q[u]);
                 multiply_add(acc_g[u], q[u], n[u]);
                 add(acc_b[u], q[u]);
                 if (gamma) {
-                    widen(gm[u], w);
+                    widen(load_raw<T, kVec>(gamma + t * kVec + u * step), w);  // from L1: registers for it spilled
                     multiply(q[u], w);
                 }
                 add(sq, q[u]);
                 multiply_add(sqn, q[u], n[u]);
             }
         }
+        rows.next(row, stride);
         if (da) {
             // both sums, then one barrier for the pair when a row spans warps
             float s = 0.f, sn = 0.f;
@@ -358,18 +431,20 @@ layer_norm_backward_kernel(const T *__restrict__ gy, const T *__restrict__ x, co
             const float mq = -s * inv_dim, mqn = -sn * inv_dim;
 #pragma unroll
             for (int u = 0; u < kVecs; ++u) {
-                if (live && u * step + t * kVec < dim) {
+                if (live && rows.in(u)) {
                     float w[kVec];
 #pragma unroll
                     for (int i = 0; i < kVec; ++i) w[i] = mqn;
                     add(q[u], mq);
                     multiply_add(q[u], n[u], w);
                     multiply(q[u], rstd);
-                    store_vec<T, kVec>(da + at + u * step, q[u]);
+                    store_vec<T, kVec>(da + row * dim + t * kVec + u * step, q[u]);
                 }
             }
         }
     }
+    if constexpr (kAhead > 0) tc5::cp_async_wait_all();
+    float *sums = reinterpret_cast<float *>(smem);
     if (partial) store_partial(acc_g, acc_b, sums, partial, t, tpr, rows_here, mine, dim);
 }
 
@@ -427,27 +502,42 @@ template <typename F> int ln_dispatch(const LnLayout &l, int dim, F f) {
                   : f(std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
 }
 
+// Blocks of a kernel that run at once; its shared memory is allowed on the way.
+template <typename K> int ln_resident(K kernel, int block, size_t smem) {
+    int per_sm = 1;
+    if (smem > (40 << 10)) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
+    return per_sm * 148;
+}
+
+// Blocks of the backward: as many as run at once.
 int64_t ln_backward_grid(int64_t n_rows, int dim) {
     const LnLayout l = ln_layout(dim, 1);
     const int64_t blocks = (n_rows + l.block / l.tpr - 1) / (l.block / l.tpr);
-    return blocks < kMaxGrid ? blocks : kMaxGrid;
+    return std::min<int64_t>(blocks, l.block == 256 ? kMaxGrid : kMaxGrid / 2);
 }
 
 template <typename T>
 int launch_layer_norm(const void *x, const void *r, const void *gamma, const void *beta, float eps, void *y, float *mean, float *rstd,
                       int64_t n_rows, int dim, cudaStream_t stream) {
     const LnLayout l = ln_layout(dim, ln_vec(dim, sizeof(T), {x, r, gamma, beta, y}));
-    const int64_t rows_here = l.block / l.tpr;
-    const unsigned grid = static_cast<unsigned>((n_rows + rows_here - 1) / rows_here);
+    const int64_t rows_here = l.block / l.tpr, blocks = (n_rows + rows_here - 1) / rows_here;
     return ln_dispatch(l, dim, [&](auto vec, auto vecs) -> int {
-        auto go = [&](auto has_r) -> int {
-            layer_norm_kernel<T, vec.value, vecs.value, has_r.value><<<grid, l.block, 0, stream>>>(
+        auto go = [&](auto has_r, auto block) -> int {
+            constexpr int kPiece = vec.value * sizeof(T), kAhead = kPiece >= 16 ? 2 : 0;
+            using R = Rows<T, vec.value, vecs.value, has_r.value ? 2 : 1, block.value, kAhead>;
+            auto kernel = layer_norm_kernel<T, vec.value, vecs.value, has_r.value, block.value, kAhead>;
+            static const int resident = ln_resident(kernel, block.value, R::kSmem);  // one wave of persistent blocks
+            kernel<<<static_cast<unsigned>(std::min<int64_t>(blocks, resident)), block.value, R::kSmem, stream>>>(
                 static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(gamma), static_cast<const T *>(beta), eps,
                 static_cast<T *>(y), mean, rstd, n_rows, dim, l.tpr);
             BPT_LAUNCH_CHECK();
             return BPT_OK;
         };
-        return r ? go(std::true_type()) : go(std::false_type());
+        auto with_block = [&](auto has_r) -> int {
+            return l.block == 256 ? go(has_r, std::integral_constant<int, 256>()) : go(has_r, std::integral_constant<int, 512>());
+        };
+        return r ? with_block(std::true_type()) : with_block(std::false_type());
     });
 }
 
@@ -455,13 +545,18 @@ template <typename T>
 int launch_layer_norm_backward(const void *gy, const void *x, const void *r, const void *gamma, const float *mean,
                                const float *rstd, void *da, void *dgamma, void *dbeta, float *partial,
                                int64_t n_rows, int dim, cudaStream_t stream) {
-    const LnLayout l = ln_layout(dim, ln_vec(dim, sizeof(T), {gy, x, r, gamma, da}));
+    const LnLayout l = ln_layout(dim, std::min<int>(ln_vec(dim, sizeof(T), {gy, x, r, gamma, da}), 16 / sizeof(T)));
     const unsigned grid = static_cast<unsigned>(ln_backward_grid(n_rows, dim));
-    const size_t smem = sizeof(float) * static_cast<size_t>(l.block / l.tpr) * dim;  // at most 512 * 16 floats
     const int rc = ln_dispatch(l, dim, [&](auto vec, auto vecs) -> int {
         auto go = [&](auto has_r) -> int {
-            auto kernel = l.block == 256 ? layer_norm_backward_kernel<T, vec.value, vecs.value, has_r.value, 256>
-                                         : layer_norm_backward_kernel<T, vec.value, vecs.value, has_r.value, 512>;
+            // three rows ahead where two blocks a SM have the room, else two; pieces that are not 16 bytes come directly
+            constexpr int kRow = 256 * 16 * vecs.value * (has_r.value ? 3 : 2);
+            constexpr int kAhead = vec.value * sizeof(T) != 16 ? 0 : 3 * kRow <= (100 << 10) ? 3 : 2;
+            auto kernel = l.block == 256 ? layer_norm_backward_kernel<T, vec.value, vecs.value, has_r.value, 256, kAhead>
+                                         : layer_norm_backward_kernel<T, vec.value, vecs.value, has_r.value, 512, kAhead>;
+            const size_t sums = sizeof(float) * static_cast<size_t>(l.block / l.tpr) * dim;  // at most 512 * 16 floats
+            const size_t smem = std::max<size_t>(kAhead * kRow * (l.block / 256), partial ? sums : 0);
+            if (smem > (40 << 10)) BPT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10));
             kernel<<<grid, l.block, smem, stream>>>(static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const T *>(r),
                                                     static_cast<const T *>(gamma), mean, rstd, static_cast<T *>(da), partial, n_rows, dim, l.tpr);
             BPT_LAUNCH_CHECK();
