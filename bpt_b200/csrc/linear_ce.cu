@@ -838,6 +838,146 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     }
 }
 
+// ---- forward of a handful of tokens: there is nothing to compute, the weight has to pass by once.  A warp takes eight rows
+// of W at a time, 16 bytes a lane and piece, against all the tokens (fp32 in shared memory).  Adding up over the lanes
+// halves the rows a lane has at each of the first three steps, so a lane ends with one row's logit (four lanes with the
+// same one) and keeps its own running maximum and sum; a block leaves one piece.
+template <typename T, int kTokens>
+__global__ void __launch_bounds__(256, 2) linear_ce_few_kernel(const T *__restrict__ x, int64_t ldx, const T *__restrict__ w, int64_t ldw,
+                                                            const T *__restrict__ bias, const int64_t *__restrict__ target, int n, int vocab,
+                                                            int dim, float *__restrict__ partial, float *__restrict__ z_target,
+                                                            unsigned *ticket, int *status) {
+    constexpr int kVec = 16 / sizeof(T), kFew = 8;
+    extern __shared__ float xs[];  // [kTokens][dim]
+    __shared__ float s_max[8][kTokens], s_sum[8][kTokens], s_z[8][kTokens];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *ticket = 0u;
+        *status = 0;
+    }
+    for (int i = threadIdx.x; i < kTokens * dim; i += 256) xs[i] = i / dim < n ? to_acc<T>(x[i / dim * ldx + i % dim]) : 0.f;
+    __syncthreads();
+    float top[kTokens], sum[kTokens], total[kTokens];
+    int tgt[kTokens];
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+        top[k] = -INFINITY;
+        sum[k] = total[k] = 0.f;
+        const int64_t t = k < n ? target[k] : -1;
+        tgt[k] = t >= 0 && t < vocab ? static_cast<int>(t) : -1;
+    }
+    for (int64_t v0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * kFew; v0 < vocab; v0 += static_cast<int64_t>(gridDim.x) * 8 * kFew) {
+        float acc[kFew][kTokens];
+#pragma unroll
+        for (int r = 0; r < kFew; ++r)
+#pragma unroll
+            for (int k = 0; k < kTokens; ++k) acc[r][k] = 0.f;
+#pragma unroll(kTokens <= 2 ? 2 : 1)
+        for (int c = lane * kVec; c < dim; c += 32 * kVec) {
+            uint4 raw[kFew];
+#pragma unroll
+            for (int r = 0; r < kFew; ++r) {  // rows past the end read the last one; they are left out below
+                const int64_t v = v0 + r < vocab ? v0 + r : vocab - 1;
+                raw[r] = __ldg(reinterpret_cast<const uint4 *>(w + v * ldw + c));
+            }
+            float wf[kFew][kVec];
+#pragma unroll
+            for (int r = 0; r < kFew; ++r) {
+                const uint32_t words[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (kVec == 4) {
+                        wf[r][i] = __uint_as_float(words[i]);
+                    } else {
+                        wf[r][2 * i] = unpack_low<T>(words[i]);
+                        wf[r][2 * i + 1] = unpack_high<T>(words[i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kTokens; ++k) {
+#pragma unroll
+                for (int i = 0; i < kVec; i += 4) {
+                    const float4 xv = *reinterpret_cast<const float4 *>(xs + k * dim + c + i);
+#pragma unroll
+                    for (int r = 0; r < kFew; ++r) {
+                        acc[r][k] = fmaf(wf[r][i], xv.x, acc[r][k]);
+                        acc[r][k] = fmaf(wf[r][i + 1], xv.y, acc[r][k]);
+                        acc[r][k] = fmaf(wf[r][i + 2], xv.z, acc[r][k]);
+                        acc[r][k] = fmaf(wf[r][i + 3], xv.w, acc[r][k]);
+                    }
+                }
+            }
+        }
+        const int64_t v = v0 + (lane >> 4) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);  // the row this lane ends with
+        const float b = bias && v < vocab ? to_acc<T>(bias[v]) : 0.f;
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+#pragma unroll
+            for (int o = 16, half = kFew / 2; o >= 4; o >>= 1, half >>= 1) {
+#pragma unroll
+                for (int r = 0; r < half; ++r) {
+                    const bool upper = lane & o;
+                    const float keep = upper ? acc[r + half][k] : acc[r][k], give = upper ? acc[r][k] : acc[r + half][k];
+                    acc[r][k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+            }
+            float z = acc[0][k];
+            z += __shfl_xor_sync(0xffffffffu, z, 2);
+            z += __shfl_xor_sync(0xffffffffu, z, 1);
+            if (v >= vocab) continue;
+            z += b;
+            if (z > top[k]) {
+                sum[k] *= ex2((top[k] - z) * kLog2e);
+                top[k] = z;
+            }
+            sum[k] += ex2((z - (top[k] == -INFINITY ? 0.f : top[k])) * kLog2e);
+            total[k] += z;
+            if (tgt[k] == v && (lane & 3) == 0) z_target[k] = z;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {  // one of the four lanes of a row counts
+        if (lane & 3) {
+            sum[k] = total[k] = 0.f;
+            top[k] = -INFINITY;
+        }
+        float m = top[k];
+#pragma unroll
+        for (int o = 16; o >= 4; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = __shfl_sync(0xffffffffu, m, 0);
+        if (!(sum[k] == 0.f)) sum[k] *= ex2((top[k] - m) * kLog2e);
+        top[k] = m;
+#pragma unroll
+        for (int o = 16; o >= 4; o >>= 1) {
+            sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+            total[k] += __shfl_xor_sync(0xffffffffu, total[k], o);
+        }
+    }
+    if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+            s_max[warp][k] = top[k];
+            s_sum[warp][k] = sum[k];
+            s_z[warp][k] = total[k];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < n) {
+        const int k = threadIdx.x;
+        float m = -INFINITY, s = 0.f, z = 0.f;
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, s_max[i][k]);
+        for (int i = 0; i < 8; ++i) {
+            if (!(s_sum[i][k] == 0.f)) s += s_sum[i][k] * ex2((s_max[i][k] - m) * kLog2e);
+            z += s_z[i][k];
+        }
+        float *at = partial + static_cast<int64_t>(blockIdx.x) * 3 * n + k;
+        at[0] = m;
+        at[n] = s;
+        at[2 * n] = z;
+    }
+}
+
 // ---- the loss from the pieces: kLanes threads a row, one row or many pieces a thread.
 constexpr int kLossThreads = 256;
 struct LossParams {
@@ -845,6 +985,8 @@ struct LossParams {
     const int64_t *target;
     int64_t n_rows, ignore_index;
     int m_tiles, n_tiles, pairs, vocab, reduction;
+    int pieces;            // of every row, or 0: what the tiles' dealing gives
+    int64_t rows_padded;   // between a piece's numbers
     float smoothing, unit;  // unit: of a piece's maximum, in logits
     float *loss, *lse, *count;
     double *block_sums;  // [blocks][sum, count]
@@ -858,8 +1000,9 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
     float loss = 0.f;
     bool counted = false;
     if (row < p.n_rows) {
-        const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles, m = row / kBM, rows_padded = static_cast<int64_t>(p.m_tiles) * kBM;
-        const int pieces = 2 * (pair_of_tile(total, p.pairs, (m + 1) * p.n_tiles - 1) - pair_of_tile(total, p.pairs, m * p.n_tiles) + 1);
+        const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles, m = row / kBM, rows_padded = p.rows_padded;
+        const int pieces = p.pieces ? p.pieces
+                                    : 2 * (pair_of_tile(total, p.pairs, (m + 1) * p.n_tiles - 1) - pair_of_tile(total, p.pairs, m * p.n_tiles) + 1);
         float top = -INFINITY, sum = 0.f, z = 0.f;
         for (int i = lane; i < pieces; i += kLanes) top = fmaxf(top, p.partial[static_cast<int64_t>(i) * 3 * rows_padded + row]);
 #pragma unroll
@@ -1089,15 +1232,25 @@ int64_t shared_pieces(int64_t run, int64_t total) {
 // block of tokens wait for memory, not for the second product.
 constexpr int64_t kFewTokens = 256;
 
+// Up to so many tokens the forward reads W on the CUDA cores (rows of whole 16-byte pieces, the tokens' features in
+// shared memory).  W of 50000 x 512, both kernels of the forward: bf16, 1 / 2 / 4 tokens 16 / 18 / 27 us against 27 / 24 /
+// 25 on the tiles; fp32, whose tiles need W split into planes first, 1 / 4 / 8 tokens 23 / 33 / 48 us against 140 / 113 / 118.
+constexpr int64_t few_tokens(int dtype) { return dtype == BPT_F32 ? 8 : 2; }
+constexpr int kFewBlocks = 148 * 2;
+
 struct Shape {
     int64_t n;
     int vocab, dim, dtype, planes, dz_planes;
     int64_t packed_ld;
-    bool pack_x, pack_w;
+    bool pack_x, pack_w, few;
     Shape(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t n_, int vocab_, int dim_, int dtype_)
         : n(n_), vocab(vocab_), dim(dim_), dtype(dtype_), planes(dtype_ == BPT_F32 ? 3 : 1),
           dz_planes(dtype_ == BPT_F32 ? 3 : n_ <= kFewTokens ? 2 : 1), packed_ld(ce_div(dim_, 8) * 8),
-          pack_x(!tma_ready(x, ldx, dtype_)), pack_w(!tma_ready(w, ldw, dtype_)) {}
+          pack_x(!tma_ready(x, ldx, dtype_)), pack_w(!tma_ready(w, ldw, dtype_)) {
+        const int vec = dtype_ == BPT_F32 ? 4 : 8;
+        const int tokens = n_ <= 1 ? 1 : n_ <= 2 ? 2 : n_ <= 4 ? 4 : 8;  // whose features fit in 40 KB
+        few = n_ <= few_tokens(dtype_) && int64_t(tokens) * dim_ <= 10000 && dim_ % vec == 0 && ldw % vec == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+    }
     int logit_pairs() const { return planes == 3 ? 6 : 1; }                          // plane products of the logits
     int product_pairs() const { return planes == 3 ? 6 : dz_planes == 2 ? 2 : 1; }  // and of the gradients
     int64_t m_tiles() const { return ce_div(n, kBM); }
@@ -1118,9 +1271,9 @@ struct ForwardSpace {
         ticket = ws.take<unsigned>(1);
         block_sums = ws.take<double>(2 * ce_div(s.n * 32, kLossThreads));
         z_target = ws.take<float>(s.n);
-        partial = ws.take<float>(s.pieces() * 2 * 3 * s.m_tiles() * kBM);
-        x = s.pack_x ? ws.take<uint16_t>(s.packed(s.n)) : nullptr;
-        w = s.pack_w ? ws.take<uint16_t>(s.packed(s.vocab)) : nullptr;
+        partial = ws.take<float>(s.few ? static_cast<int64_t>(kFewBlocks) * 3 * s.n : s.pieces() * 2 * 3 * s.m_tiles() * kBM);
+        x = s.pack_x && !s.few ? ws.take<uint16_t>(s.packed(s.n)) : nullptr;
+        w = s.pack_w && !s.few ? ws.take<uint16_t>(s.packed(s.vocab)) : nullptr;
     }
 };
 
@@ -1332,48 +1485,73 @@ struct Call {
     int reduction;
 };
 
+template <typename T> int launch_few(const Shape &s, const Call &c, ForwardSpace &f, cudaStream_t stream) {
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(kFewBlocks, ce_div(s.vocab, 64)));
+    auto go = [&](auto tokens) -> int {
+        linear_ce_few_kernel<T, tokens.value><<<grid, 256, tokens.value * s.dim * sizeof(float), stream>>>(
+            static_cast<const T *>(c.x), c.ldx, static_cast<const T *>(c.w), c.ldw, static_cast<const T *>(c.bias), c.target,
+            static_cast<int>(s.n), s.vocab, s.dim, f.partial, f.z_target, f.ticket, f.status);
+        BPT_LAUNCH_CHECK();
+        return BPT_OK;
+    };
+    if (s.n <= 1) return go(std::integral_constant<int, 1>());
+    if constexpr (kIsFloat<T>) {
+        if (s.n > 4) return go(std::integral_constant<int, 8>());
+        if (s.n > 2) return go(std::integral_constant<int, 4>());
+    }
+    return go(std::integral_constant<int, 2>());
+}
+
 template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace &f, float *loss, float *lse, float *count, cudaStream_t stream) {
     constexpr bool kHalf = kIsHalf<T>;
     Operand x{c.x, c.ldx, 0}, w{c.w, c.ldw, 0};
-    if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, f.x, nullptr, 0, stream, &x));
-    if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, f.w, nullptr, 0, stream, &w));
-    Maps maps;
-    BPT_TRY(make_map(&maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
-    BPT_TRY(make_map(&maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));
-    maps.c = maps.d = maps.e = maps.a;
-    Params p{};
-    p.m_tiles = static_cast<int>(s.m_tiles());
-    p.n_tiles = s.v_tiles();
-    p.k_tiles = static_cast<int>(ce_div(s.dim, kBK));
-    p.n_ext = s.vocab;
-    p.n_pairs = s.logit_pairs();
-    p.dz_planes = s.dz_planes;
-    p.status = f.status;
-    p.n_rows = s.n;
-    p.ignore_index = c.ignore_index;
-    p.vocab = s.vocab;
-    p.bias = c.bias;
-    p.target = c.target;
-    p.partial = f.partial;
-    p.z_target = f.z_target;
-    p.ticket = f.ticket;
-    p.starts = 1;
-    p.smoothed = c.smoothing != 0.f;
-    const int pairs = pairs_for(s.m_tiles() * s.v_tiles());
-    BPT_TRY((launch_ce<T, kStats>(maps, p, pairs, stream)));
     LossParams l{};
+    const int pairs = pairs_for(s.m_tiles() * s.v_tiles());
+    if (s.few) {
+        BPT_TRY(launch_few<T>(s, c, f, stream));
+        l.pieces = static_cast<int>(std::min<int64_t>(kFewBlocks, ce_div(s.vocab, 64)));
+        l.rows_padded = s.n;
+        l.unit = 1.f;
+    } else {
+        if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, f.x, nullptr, 0, stream, &x));
+        if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, f.w, nullptr, 0, stream, &w));
+        Maps maps;
+        BPT_TRY(make_map(&maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
+        BPT_TRY(make_map(&maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));
+        maps.c = maps.d = maps.e = maps.a;
+        Params p{};
+        p.m_tiles = static_cast<int>(s.m_tiles());
+        p.n_tiles = s.v_tiles();
+        p.k_tiles = static_cast<int>(ce_div(s.dim, kBK));
+        p.n_ext = s.vocab;
+        p.n_pairs = s.logit_pairs();
+        p.dz_planes = s.dz_planes;
+        p.status = f.status;
+        p.n_rows = s.n;
+        p.ignore_index = c.ignore_index;
+        p.vocab = s.vocab;
+        p.bias = c.bias;
+        p.target = c.target;
+        p.partial = f.partial;
+        p.z_target = f.z_target;
+        p.ticket = f.ticket;
+        p.starts = 1;
+        p.smoothed = c.smoothing != 0.f;
+        BPT_TRY((launch_ce<T, kStats>(maps, p, pairs, stream)));
+        l.rows_padded = s.m_tiles() * kBM;
+        l.unit = kIsFloat<T> ? 1.f : kLn2;
+    }
     l.partial = f.partial;
     l.z_target = f.z_target;
     l.target = c.target;
     l.n_rows = s.n;
     l.ignore_index = c.ignore_index;
-    l.m_tiles = p.m_tiles;
-    l.n_tiles = p.n_tiles;
+    l.m_tiles = static_cast<int>(s.m_tiles());
+    l.n_tiles = s.v_tiles();
     l.pairs = pairs;
     l.vocab = s.vocab;
     l.reduction = c.reduction;
     l.smoothing = c.smoothing;
-    l.unit = kIsFloat<T> ? 1.f : kLn2;
     l.loss = loss;
     l.lse = lse;
     l.count = count;
@@ -1381,7 +1559,7 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     l.ticket = f.ticket;
     l.status = f.status;
     // a row of many pieces (few rows, so many blocks shared each) is merged by a warp
-    if (s.pieces() > 8) linear_ce_loss_kernel<32><<<static_cast<unsigned>(ce_div(s.n * 32, kLossThreads)), kLossThreads, 0, stream>>>(l);
+    if (l.pieces > 8 || s.pieces() > 8) linear_ce_loss_kernel<32><<<static_cast<unsigned>(ce_div(s.n * 32, kLossThreads)), kLossThreads, 0, stream>>>(l);
     else linear_ce_loss_kernel<1><<<static_cast<unsigned>(ce_div(s.n, kLossThreads)), kLossThreads, 0, stream>>>(l);
     BPT_LAUNCH_CHECK();
     return BPT_OK;
