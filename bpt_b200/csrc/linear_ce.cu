@@ -22,10 +22,13 @@
 //   products  dZ W and dZ^T X of the piece in one launch.  dZ is read K-major by the one and MN-major by the other.
 // dZ is rounded to the operands' 16-bit type, without g where all g_i are one number (the scale goes onto the fp32
 // results): a half-step error of each probability, the size of the rounding of the gradients themselves.
-// fp32 operands are split into three bf16 planes (8 + 8 + 8 significant bits, by truncation, exact) and each product
-// is run as the six products of planes whose weight is above 2^-24, smallest first.  The tensor core rounds its running
-// sum towards zero, a bias that grows with K, so the fp32 kernels take the accumulator out every 512 of K and add
-// the runs up in registers.
+// fp32 operands are split into 16-bit planes, and each product of matrices is run as the products of planes whose weight
+// is above 2^-24.  Scaled by a power of two to the top of fp16's range, an operand is two fp16 planes, the second kept
+// times 2^11: 22 significant bits by rounding, down to 2^-29 of the largest number, and good to 2^-51 of that number
+// below; three products.  That is taken where no row's largest is below 2^-24 of the matrix's largest.  Otherwise three
+// bf16 planes (24 bits by truncation, exact, any range), six products.  A first pass over X and W finds which, on the
+// device.  The tensor core rounds its running sum towards zero, a bias that grows with K, so the fp32 kernels take the
+// accumulator out every 512 of K, and between products of different scales, and add these runs up in registers.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -79,7 +82,8 @@ struct Product {
 struct Params {
     int m_tiles, n_tiles, k_tiles, n_ext;  // stats, grad: tiles; columns in all (the last tile may be narrower)
     int m_ext;                             // grad: rows of the piece
-    int n_pairs;                           // plane products: 1, 2 or 6
+    int n_pairs;                           // plane products: 1 or 2; fp32: 3 or 6, as `split` says
+    const unsigned *split;                 // fp32: see Split
     int dz_planes;                         // grad: planes of dZ that are written
     int a0, b0;                            // added to the row coordinate of A and of B
     int *status;                           // set to 1 when a wait ran out
@@ -106,7 +110,9 @@ struct Params {
     int first, busy, after_busy, after;
 };
 
-// Plane products, smallest first.  All six: fp32 by fp32; the last two: dZ in two planes by a 16-bit operand; the last: 16-bit.
+// Plane products, smallest first.  All six: three bf16 planes by three; the last three: two fp16 planes by two; the last
+// two: dZ in two planes by a 16-bit operand; the last: 16-bit.
+constexpr float kLowScale = 2048.f;  // of the second of two fp16 planes
 __constant__ const int kPairA[6] = {2, 0, 1, 0, 1, 0}, kPairB[6] = {0, 2, 1, 1, 0, 0};
 
 template <typename T> constexpr bool kIsHalf = std::is_same<T, __half>::value;
@@ -114,8 +120,8 @@ template <typename T> constexpr bool kIsFloat = std::is_same<T, float>::value;
 // fp16 dZ is kept times 2^14: |dz| <= 2, and probabilities down to 2^-28 stay normal numbers
 template <typename T> constexpr float kDzScale = kIsHalf<T> ? 16384.f : 1.f;
 
-template <typename T> __device__ constexpr uint32_t ce_instr(int n, bool a_mn, bool b_mn) {
-    const uint32_t fmt = kIsHalf<T> ? 0u : 1u;
+__device__ constexpr uint32_t ce_instr(bool fp16, int n, bool a_mn, bool b_mn) {
+    const uint32_t fmt = fp16 ? 0u : 1u;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) |
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kBM >> 4) << 24);  // M = 256 over the pair
 }
@@ -125,6 +131,33 @@ __device__ __forceinline__ float top_scale(unsigned bits) {
     const unsigned e = bits >> 23;
     if (e >= 255u) return __int_as_float(0x7fffffff);  // a gradient that is not finite: everything is NaN
     return e == 0u ? (bits ? 1.17549435e-38f : 1.f) : __uint_as_float(e << 23);
+}
+
+// How fp32 operands are split, from what the pass over X and W found: bits of the largest finite |x|, complement of the
+// bits of the smallest of the rows' largest (rows of zeros aside), the same of w.
+struct Split {
+    bool half = false;                                 // two fp16 planes
+    float x = 1.f, w = 1.f, x_back = 1.f, w_back = 1.f;  // scales before the split, and their inverses
+};
+constexpr unsigned kSpread = 24;
+__device__ __forceinline__ Split read_split(const unsigned *found) {
+    Split s;
+    const unsigned x_top = found[0] >> 23, x_low = ~found[1] >> 23, w_top = found[2] >> 23, w_low = ~found[3] >> 23;
+    auto fits = [](unsigned top, unsigned low) { return top == 0u || (top >= 15u && top <= 254u && top - low <= kSpread); };
+    // a matrix of zeros (or of nothing but denormal numbers, which the planes do not hold) has top 0
+    if (found[0] != 0u && x_top == 0u) return s;
+    if (found[2] != 0u && w_top == 0u) return s;
+    if (!fits(x_top, x_low) || !fits(w_top, w_low)) return s;
+    s.half = true;
+    if (x_top) {
+        s.x = __uint_as_float((268u - x_top) << 23);  // the largest comes to [2^14, 2^15)
+        s.x_back = __uint_as_float((x_top - 14u) << 23);
+    }
+    if (w_top) {
+        s.w = __uint_as_float((268u - w_top) << 23);
+        s.w_back = __uint_as_float((w_top - 14u) << 23);
+    }
+    return s;
 }
 
 // The first tile of pair c when t tiles are dealt in order to g pairs; the pair that has tile i.
@@ -161,6 +194,15 @@ __device__ __forceinline__ uint32_t take_plane(float &a, float &b) {
     const uint32_t word = (ha >> 16) | hb;
     a = isfinite(a) ? a - __uint_as_float(ha) : 0.f;
     b = isfinite(b) ? b - __uint_as_float(hb) : 0.f;
+    return word;
+}
+
+// The next fp16 plane of a, b (rounded); a and b become what is left, times kLowScale.
+__device__ __forceinline__ uint32_t take_half(float &a, float &b) {
+    const uint32_t word = pack2<__half>(a, b);
+    const float ha = unpack_low<__half>(word), hb = unpack_high<__half>(word);
+    a = isfinite(ha) ? (a - ha) * kLowScale : 0.f;
+    b = isfinite(hb) ? (b - hb) * kLowScale : 0.f;
     return word;
 }
 
@@ -289,11 +331,16 @@ __device__ __forceinline__ float column_sum(float (&v)[32], int lane) {
     return v[0];
 }
 
-// What the gradients of w and b, and of x, are multiplied by: the one gradient of the loss, or the power of two that
-// the tokens' own ones were divided by.
-template <typename T> __device__ __forceinline__ float result_scale(const Params &p) {
+// What the gradients are multiplied by (0: of x, 1: of w, 2: of b): the one gradient of the loss, or the power of two that
+// the tokens' own ones were divided by; and what dZ and the other operand were scaled by.
+constexpr float kHalfDz = 16384.f;  // fp32 dZ in fp16 planes, as fp16 dZ
+template <typename T> __device__ __forceinline__ float result_scale(const Params &p, int which) {
     float scale = p.reduction == kReduceNone ? top_scale(*p.grad_top) : *p.grad;
     if (p.reduction == kReduceMean) scale = *p.count > 0.f ? scale / *p.count : 0.f;
+    if constexpr (kIsFloat<T>) {
+        const Split split = read_split(p.split);
+        return which == 2 || !split.half ? scale : scale * (1.f / kHalfDz) * (which == 0 ? split.w_back : split.x_back);
+    }
     return scale * (1.f / kDzScale<T>);
 }
 
@@ -342,7 +389,13 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     fence_after_sync();
     const uint32_t tmem = *tmem_word;
     Work<kKind> work(p);
-    const int first_pair = 6 - p.n_pairs;
+    Split split;
+    if constexpr (kPrecise) split = read_split(p.split);
+    const int first_pair = 6 - (kPrecise ? (split.half ? 3 : 6) : p.n_pairs);
+    // sums that share an accumulator: all plane products, but of two fp16 planes the two small ones (both times kLowScale)
+    // and the large one
+    const int groups = kPrecise && split.half ? 2 : 1;
+    auto group_pairs = [&](int group) { return groups == 1 ? 6 - first_pair : group == 0 ? 2 : 1; };
     if (warp >= kFinishWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
     if (warp == kFinishWarps) {
@@ -402,37 +455,40 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             bool ok = true;
             while (ok && work.next()) {
                 const bool a_mn = kKind == kProducts && work.which == 1, b_mn = kKind == kProducts;
-                const uint32_t instr = ce_instr<T>(work.width(), a_mn, b_mn);
+                const uint32_t instr = ce_instr(kPrecise ? split.half : kIsHalf<T>, work.width(), a_mn, b_mn);
                 const int run = kPrecise ? kRunTiles : work.k1;
                 for (int kr = work.k0; ok && kr < work.k1; kr += run) {
-                    const uint32_t d = tmem + buf * kBN;
-                    ok = mbar_wait_or_stop(bar_read + 8 * buf, read_phase ^ 1u, stop);
-                    if (!ok) break;
-                    fence_after_sync();
-                    uint32_t accumulate = 0;
-                    const int steps = (6 - first_pair) * (min(kr + run, work.k1) - kr);
-                    for (int step = 0; step < steps; ++step) {
-                        ok = mbar_wait_or_stop(bar_full + 8 * s, phase, stop);
+                    const int k_tiles = min(kr + run, work.k1) - kr;
+                    for (int group = 0; ok && group < groups; ++group) {
+                        const uint32_t d = tmem + buf * kBN;
+                        ok = mbar_wait_or_stop(bar_read + 8 * buf, read_phase ^ 1u, stop);
                         if (!ok) break;
                         fence_after_sync();
-                        const uint32_t a = base + s * kStageBytes, b = a + kABytes;
+                        uint32_t accumulate = 0;
+                        const int steps = group_pairs(group) * k_tiles;
+                        for (int step = 0; step < steps; ++step) {
+                            ok = mbar_wait_or_stop(bar_full + 8 * s, phase, stop);
+                            if (!ok) break;
+                            fence_after_sync();
+                            const uint32_t a = base + s * kStageBytes, b = a + kABytes;
 #pragma unroll
-                        for (int ks = 0; ks < kBK / 16; ++ks) {
-                            mma_pair(d, a_mn ? desc_mnmajor(a, ks) : desc_kmajor(a, ks), b_mn ? desc_mnmajor(b, ks) : desc_kmajor(b, ks), instr,
-                                     accumulate);
-                            accumulate = 1;
+                            for (int ks = 0; ks < kBK / 16; ++ks) {
+                                mma_pair(d, a_mn ? desc_mnmajor(a, ks) : desc_kmajor(a, ks), b_mn ? desc_mnmajor(b, ks) : desc_kmajor(b, ks),
+                                         instr, accumulate);
+                                accumulate = 1;
+                            }
+                            mma_commit_pair(bar_empty + 8 * s);
+                            if (++s == kStages) {
+                                s = 0;
+                                phase ^= 1u;
+                            }
                         }
-                        mma_commit_pair(bar_empty + 8 * s);
-                        if (++s == kStages) {
-                            s = 0;
-                            phase ^= 1u;
+                        if (!ok) break;
+                        mma_commit_pair(bar_ready + 8 * buf);
+                        if (++buf == 2) {
+                            buf = 0;
+                            read_phase ^= 1u;
                         }
-                    }
-                    if (!ok) break;
-                    mma_commit_pair(bar_ready + 8 * buf);
-                    if (++buf == 2) {
-                        buf = 0;
-                        read_phase ^= 1u;
                     }
                 }
             }
@@ -454,8 +510,11 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         int tgt = -1;
         float row_lse = 0.f, row_l2 = 0.f, row_g = 0.f, uniform = 0.f;
         bool row_plain = true, row_skips = false;  // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0
-        float scale = 1.f;
-        if constexpr (kKind == kProducts) scale = result_scale<T>(p);
+        float scales[2] = {1.f, 1.f};
+        if constexpr (kKind == kProducts) {
+            scales[0] = result_scale<T>(p, 0);
+            scales[1] = result_scale<T>(p, 1);
+        }
         // grad, 16-bit: column sums over the pair's token blocks of one vocabulary block
         constexpr bool kKeepSums = kKind == kGrad && !kPrecise;
         const uint32_t out_tile = base + kStages * kStageBytes + warp * 2 * kOutBytes;
@@ -540,10 +599,10 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + i);
-                            v[i] += b.x;
-                            v[i + 1] += b.y;
-                            v[i + 2] += b.z;
-                            v[i + 3] += b.w;
+                            v[i] = fmaf(v[i] * split.x_back, split.w_back, b.x);
+                            v[i + 1] = fmaf(v[i + 1] * split.x_back, split.w_back, b.y);
+                            v[i + 2] = fmaf(v[i + 2] * split.x_back, split.w_back, b.z);
+                            v[i + 3] = fmaf(v[i + 3] * split.x_back, split.w_back, b.w);
                         }
                     } else {  // logits times log2(e)
 #pragma unroll
@@ -659,15 +718,16 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         if constexpr (kPrecise) {
                             float left[32];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) left[i] = v[i];
-#pragma unroll
-                            for (int plane = 0; plane < 3; ++plane) {
+                            for (int i = 0; i < 32; ++i) left[i] = split.half ? v[i] * kHalfDz : v[i];
+                            for (int plane = 0; plane < (split.half ? 2 : 3); ++plane) {
                                 const uint32_t tile = next_tile();
 #pragma unroll
                                 for (int u = 0; u < 4; ++u) {
                                     uint32_t w[4];
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i) w[i] = take_plane(left[8 * u + 2 * i], left[8 * u + 2 * i + 1]);
+                                    for (int i = 0; i < 4; ++i)
+                                        w[i] = split.half ? take_half(left[8 * u + 2 * i], left[8 * u + 2 * i + 1])
+                                                          : take_plane(left[8 * u + 2 * i], left[8 * u + 2 * i + 1]);
                                     st_shared_v4(tile + narrow + ((u ^ turn) << 4), w[0], w[1], w[2], w[3]);
                                 }
                                 send(n * kBN + c0, plane, tile);
@@ -715,7 +775,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             if (q.last) {
                                 const bool ignored = work.which == 0 && p.target[row] == p.ignore_index;
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] = ignored ? 0.f : v[i] * scale;
+                                for (int i = 0; i < 32; ++i) v[i] = ignored ? 0.f : v[i] * (work.which == 0 ? scales[0] : scales[1]);
                                 store_row(static_cast<T *>(q.out) + row * q.n_ext, q.n_ext * static_cast<int64_t>(sizeof(T)), col, left, v);
                             } else {
                                 store_row(q.acc + row * q.acc_ld, q.acc_ld * 4, col, left, v);
@@ -734,20 +794,23 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
                 ok = true;
                 for (int kr = work.k0; ok && kr < work.k1; kr += kRunTiles) {
-                    ok = __all_sync(0xffffffffu, mbar_wait_or_stop(bar_ready + 8 * buf, ready_phase, stop));
-                    if (!ok) break;
-                    fence_after_sync();
+                    for (int group = 0; ok && group < groups; ++group) {
+                        ok = __all_sync(0xffffffffu, mbar_wait_or_stop(bar_ready + 8 * buf, ready_phase, stop));
+                        if (!ok) break;
+                        fence_after_sync();
+                        const float weight = group < groups - 1 ? 1.f / kLowScale : 1.f;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (first + 32 * j < cols) {
-                            uint32_t r[32];
-                            tmem_ld32(tmem + lanes + buf * kBN + first + 32 * j, r);
-                            tmem_ld_wait();
+                        for (int j = 0; j < 4; ++j) {
+                            if (first + 32 * j < cols) {
+                                uint32_t r[32];
+                                tmem_ld32(tmem + lanes + buf * kBN + first + 32 * j, r);
+                                tmem_ld_wait_for(r);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sum[j][i] += __uint_as_float(r[i]);
+                                for (int i = 0; i < 32; ++i) sum[j][i] = fmaf(__uint_as_float(r[i]), weight, sum[j][i]);
+                            }
                         }
+                        release();
                     }
-                    release();
                 }
                 if constexpr (kKind != kProducts) ok = !finish_barrier_or(!ok);  // s_bias is whole, and all these warps go on or none does
                 if (!ok) break;
@@ -1079,12 +1142,51 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
 }
 
 // ---- operands that TMA cannot read where they lie (fp32, rows or bases off 16 bytes): copied into rows of a multiple
-// of 8 elements, fp32 as three bf16 planes.  Rows whose target is ignored (target given) are zeroed: their features
-// may hold anything, and 0 * NaN would reach every gradient of W.
+// of 8 elements, fp32 as planes.  Rows whose target is ignored (target given) are zeroed: their features may hold
+// anything, and 0 * NaN would reach every gradient of W.
+__global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *__restrict__ x, int64_t ldx, int64_t x_rows, const float *__restrict__ w,
+                                                               int64_t ldw, int64_t w_rows, int dim, const int64_t *__restrict__ target,
+                                                               int64_t ignore_index, unsigned *__restrict__ found) {
+    __shared__ unsigned s_found[4];
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x < 4) s_found[threadIdx.x] = 0u;
+    __syncthreads();
+    unsigned best[4] = {0u, 0u, 0u, 0u};
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * 8;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < x_rows + w_rows; i += stride) {
+        const bool of_x = i < x_rows;
+        if (of_x && target[i] == ignore_index) continue;
+        const float *row = of_x ? x + i * ldx : w + (i - x_rows) * ldw;
+        unsigned top = 0u;
+        for (int c = lane; c < dim; c += 32) {
+            const unsigned bits = __float_as_uint(row[c]) & 0x7FFFFFFFu;
+            if (bits < 0x7F800000u) top = max(top, bits);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (top == 0u) continue;
+        if (of_x) {
+            best[0] = max(best[0], top);
+            best[1] = max(best[1], ~top);
+        } else {
+            best[2] = max(best[2], top);
+            best[3] = max(best[3], ~top);
+        }
+    }
+    if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) atomicMax(&s_found[k], best[k]);
+    }
+    __syncthreads();
+    if (threadIdx.x < 4) atomicMax(&found[threadIdx.x], s_found[threadIdx.x]);
+}
+
 template <typename T>
 __global__ void linear_ce_pack_kernel(const T *__restrict__ src, int64_t ld, int64_t rows, int dim, uint16_t *__restrict__ dst,
-                                      int64_t dst_ld, int64_t plane, const int64_t *__restrict__ target, int64_t ignore_index) {
+                                      int64_t dst_ld, int64_t plane, const int64_t *__restrict__ target, int64_t ignore_index,
+                                      const unsigned *__restrict__ found, int is_w) {
     const int64_t pieces = dst_ld / 8, total = rows * pieces;
+    Split split;
+    if constexpr (kIsFloat<T>) split = read_split(found);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t row = i / pieces;
         const int c = static_cast<int>(i % pieces) * 8;
@@ -1092,22 +1194,22 @@ __global__ void linear_ce_pack_kernel(const T *__restrict__ src, int64_t ld, int
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = !skip && c + j < dim ? to_acc<T>(src[row * ld + c + j]) : 0.f;
-        constexpr int kPlanes = std::is_same<T, float>::value ? 3 : 1;
+        if constexpr (kIsFloat<T>) {
+            if (split.half) {
 #pragma unroll
-        for (int q = 0; q < kPlanes; ++q) {
-            uint4 w;
-            if constexpr (kPlanes == 3) {
-                w.x = take_plane(v[0], v[1]);
-                w.y = take_plane(v[2], v[3]);
-                w.z = take_plane(v[4], v[5]);
-                w.w = take_plane(v[6], v[7]);
-            } else {
-                w.x = pack2<T>(v[0], v[1]);
-                w.y = pack2<T>(v[2], v[3]);
-                w.z = pack2<T>(v[4], v[5]);
-                w.w = pack2<T>(v[6], v[7]);
+                for (int j = 0; j < 8; ++j) v[j] *= is_w ? split.w : split.x;
             }
-            *reinterpret_cast<uint4 *>(dst + q * plane + row * dst_ld + c) = w;
+            for (int q = 0; q < (split.half ? 2 : 3); ++q) {
+                uint4 word;
+                word.x = split.half ? take_half(v[0], v[1]) : take_plane(v[0], v[1]);
+                word.y = split.half ? take_half(v[2], v[3]) : take_plane(v[2], v[3]);
+                word.z = split.half ? take_half(v[4], v[5]) : take_plane(v[4], v[5]);
+                word.w = split.half ? take_half(v[6], v[7]) : take_plane(v[6], v[7]);
+                *reinterpret_cast<uint4 *>(dst + q * plane + row * dst_ld + c) = word;
+            }
+        } else {
+            *reinterpret_cast<uint4 *>(dst + row * dst_ld + c) =
+                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
         }
     }
 }
@@ -1157,7 +1259,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_constant__ Params p, int which) {
     const Product &q = p.product[which];
     const int64_t pieces = q.acc_ld / 4, rows = q.row_end - q.row_offset, total = rows * pieces, plane = static_cast<int64_t>(q.m_tiles) * kBM * q.acc_ld;
-    const float scale = *p.status ? __int_as_float(0x7fffffff) : result_scale<T>(p);
+    const float scale = *p.status ? __int_as_float(0x7fffffff) : result_scale<T>(p, which);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t in_piece = i / pieces, row = q.row_offset + in_piece;
         const int col = static_cast<int>(i % pieces) * 4, left = min(4, q.n_ext - col);
@@ -1206,7 +1308,7 @@ __global__ void __launch_bounds__(256) linear_ce_bias_kernel(const __grid_consta
     for (int i = 0; i < 8; ++i) s += s_part[i][threadIdx.x];
     if (add) s += acc[c];
     if (!last) acc[c] = s;
-    else out[c] = *p.status ? from_acc<T>(__int_as_float(0x7fffffff)) : from_acc<T>(s * result_scale<T>(p));
+    else out[c] = *p.status ? from_acc<T>(__int_as_float(0x7fffffff)) : from_acc<T>(s * result_scale<T>(p, 2));
 }
 
 // ---- host side
@@ -1263,12 +1365,13 @@ struct Shape {
 struct ForwardSpace {
     float *partial, *z_target;
     double *block_sums;
-    unsigned *ticket;
+    unsigned *ticket, *found;
     int *status;
     uint16_t *x, *w;
     ForwardSpace(Workspace &ws, const Shape &s) {
         status = ws.take<int>(1);
         ticket = ws.take<unsigned>(1);
+        found = ws.take<unsigned>(4);
         block_sums = ws.take<double>(2 * ce_div(s.n * 32, kLossThreads));
         z_target = ws.take<float>(s.n);
         partial = ws.take<float>(s.few ? static_cast<int64_t>(kFewBlocks) * 3 * s.n : s.pieces() * 2 * 3 * s.m_tiles() * kBM);
@@ -1347,7 +1450,7 @@ struct BackwardSpace {
     int64_t rows, cols;  // tokens x vocabulary of a piece
     int64_t dz_ld, dz_plane, acc_ld;
     int *status;
-    unsigned *ticket, *grad_top;
+    unsigned *ticket, *grad_top, *found;
     uint16_t *dz, *x, *w, *x_clean;
     unsigned char *clean;
     float *dx_acc, *dw_acc, *col_sums, *db_acc, *partial;
@@ -1360,6 +1463,7 @@ struct BackwardSpace {
         status = ws.take<int>(1);
         ticket = ws.take<unsigned>(1);
         grad_top = ws.take<unsigned>(1);
+        found = ws.take<unsigned>(4);
         dz = ws.take<uint16_t>(dz_plane * s.dz_planes);
         x = s.pack_x ? ws.take<uint16_t>(s.packed(s.n)) : nullptr;
         w = s.pack_w ? ws.take<uint16_t>(s.packed(s.vocab)) : nullptr;
@@ -1370,8 +1474,10 @@ struct BackwardSpace {
         db_acc = want_db && rows < s.n ? ws.take<float>(s.vocab) : nullptr;
         // the rows of column sums and the parts that any of the pieces may need (the last ones are smaller)
         int64_t sum_rows = 0, parts = 0;
-        for (int64_t r : {rows, s.n - (ce_div(s.n, rows) - 1) * rows}) {
-            for (int64_t c : {cols, s.vocab - (ce_div(s.vocab, cols) - 1) * cols}) {
+        const int64_t last_r = s.n - (ce_div(s.n, rows) - 1) * rows, last_c = s.vocab - (ce_div(s.vocab, cols) - 1) * cols;
+        for (int64_t r : {rows, last_r}) {
+            for (int64_t c : {cols, last_c}) {
+                if ((r == rows && rows > s.n) || (c == cols && cols > s.vocab)) continue;  // there is the last one only
                 const int64_t m = ce_div(r, kBM), n = ce_div(c, kBN);
                 sum_rows = std::max(sum_rows, 8 * (s.planes == 3 ? m : shared_pieces(m, m * n)));
                 Product px, pw;
@@ -1457,19 +1563,6 @@ template <typename T, int kKind> int launch_ce(const Maps &m, const Params &p, i
     return BPT_OK;
 }
 
-template <typename T>
-int pack_operand(const void *src, int64_t ld, int64_t rows, const Shape &s, uint16_t *dst, const int64_t *target, int64_t ignore_index,
-                 cudaStream_t stream, Operand *out) {
-    out->at = dst;
-    out->ld = s.packed_ld;
-    out->plane = align_up(rows * s.packed_ld, 64);
-    const int64_t blocks = std::min<int64_t>(ce_div(rows * (s.packed_ld / 8), 256), 148 * 16);
-    linear_ce_pack_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T *>(src), ld, rows, s.dim, dst,
-                                                                               s.packed_ld, out->plane, target, ignore_index);
-    BPT_LAUNCH_CHECK();
-    return BPT_OK;
-}
-
 #define BPT_TRY(call)                  \
     do {                               \
         const int rc__ = (call);       \
@@ -1484,6 +1577,36 @@ struct Call {
     float smoothing;
     int reduction;
 };
+
+template <typename T>
+int pack_operand(const void *src, int64_t ld, int64_t rows, const Shape &s, uint16_t *dst, const Call &c, bool is_w, const unsigned *found,
+                 cudaStream_t stream, Operand *out) {
+    out->at = dst;
+    out->ld = s.packed_ld;
+    out->plane = align_up(rows * s.packed_ld, 64);
+    const int64_t blocks = std::min<int64_t>(ce_div(rows * (s.packed_ld / 8), 256), 148 * 16);
+    linear_ce_pack_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T *>(src), ld, rows, s.dim, dst, s.packed_ld,
+                                                                               out->plane, is_w ? nullptr : c.target, c.ignore_index, found, is_w);
+    BPT_LAUNCH_CHECK();
+    return BPT_OK;
+}
+// X and W as the tiles read them: where they lie, or packed.
+template <typename T>
+int pack_operands(const Shape &s, const Call &c, uint16_t *x_to, uint16_t *w_to, unsigned *found, cudaStream_t stream, Operand *x, Operand *w) {
+    *x = Operand{c.x, c.ldx, 0};
+    *w = Operand{c.w, c.ldw, 0};
+    if constexpr (kIsFloat<T>) {
+        BPT_CUDA(cudaMemsetAsync(found, 0, 4 * sizeof(unsigned), stream));
+        const int64_t blocks = std::min<int64_t>(ce_div(s.n + s.vocab, 8), 148 * 8);
+        linear_ce_spread_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const float *>(c.x), c.ldx, s.n,
+                                                                                  static_cast<const float *>(c.w), c.ldw, s.vocab, s.dim,
+                                                                                  c.target, c.ignore_index, found);
+        BPT_LAUNCH_CHECK();
+    }
+    if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, x_to, c, false, found, stream, x));
+    if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, w_to, c, true, found, stream, w));
+    return BPT_OK;
+}
 
 template <typename T> int launch_few(const Shape &s, const Call &c, ForwardSpace &f, cudaStream_t stream) {
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(kFewBlocks, ce_div(s.vocab, 64)));
@@ -1504,7 +1627,6 @@ template <typename T> int launch_few(const Shape &s, const Call &c, ForwardSpace
 
 template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace &f, float *loss, float *lse, float *count, cudaStream_t stream) {
     constexpr bool kHalf = kIsHalf<T>;
-    Operand x{c.x, c.ldx, 0}, w{c.w, c.ldw, 0};
     LossParams l{};
     const int pairs = pairs_for(s.m_tiles() * s.v_tiles());
     if (s.few) {
@@ -1513,8 +1635,8 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
         l.rows_padded = s.n;
         l.unit = 1.f;
     } else {
-        if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, f.x, nullptr, 0, stream, &x));
-        if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, f.w, nullptr, 0, stream, &w));
+        Operand x, w;
+        BPT_TRY(pack_operands<T>(s, c, f.x, f.w, f.found, stream, &x, &w));
         Maps maps;
         BPT_TRY(make_map(&maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
         BPT_TRY(make_map(&maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));
@@ -1527,6 +1649,7 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
         p.n_pairs = s.logit_pairs();
         p.dz_planes = s.dz_planes;
         p.status = f.status;
+        p.split = f.found;
         p.n_rows = s.n;
         p.ignore_index = c.ignore_index;
         p.vocab = s.vocab;
@@ -1570,9 +1693,8 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
                 void *dw, void *db, cudaStream_t stream) {
     constexpr bool kHalf = kIsHalf<T>;
     constexpr bool kFloat = std::is_same<T, float>::value;
-    Operand x{c.x, c.ldx, 0}, w{c.w, c.ldw, 0};
-    if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, f.x, c.target, c.ignore_index, stream, &x));
-    if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, f.w, nullptr, 0, stream, &w));
+    Operand x, w;
+    BPT_TRY(pack_operands<T>(s, c, f.x, f.w, f.found, stream, &x, &w));
     const int64_t clean_ld = ce_div(s.dim, 8) * 8;
     if (f.clean) {
         linear_ce_clean_kernel<<<static_cast<unsigned>(ce_div(s.n, 64)), 256, 0, stream>>>(
@@ -1597,6 +1719,7 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     p.n_pairs = s.logit_pairs();
     p.dz_planes = s.dz_planes;
     p.status = f.status;
+    p.split = f.found;
     p.ticket = f.ticket;
     p.spoilt = db;
     p.n_rows = s.n;

@@ -388,3 +388,52 @@ def test_models_train_on_it():
         logp = mt(*args)
         want = -(0.9 * logp.gather(1, words.unsqueeze(1)).squeeze(1) + 0.1 * logp.mean(1)).mean()
     assert abs(float(smooth) - float(want)) < 1e-5 * float(want)
+
+
+@pytest.mark.parametrize("spread", [0, 12, 24, 25, 40, 100])
+@pytest.mark.parametrize("of", ["x", "w", "all"])
+def test_fp32_rows_of_very_different_size(spread, of):
+    """fp32 operands are split by what their rows' sizes allow: two scaled planes, or three with the whole range.  Each token's
+    loss has to be as good as its own numbers allow (Ez with the row's own A), whatever the other rows are; and the
+    gradients of a token of ordinary size have to be as good as in a batch of such tokens alone."""
+    from bpt_b200.loss import linear_cross_entropy
+    n, vocab, dim = 300, 500, 72
+    x, w, b, t = inputs(n, vocab, dim, torch.float32)
+    down = torch.ones(n, device="cuda", dtype=torch.float64)
+    if of in ("x", "all"):
+        down = 2.0 ** -(torch.arange(n, device="cuda", dtype=torch.float64) % (spread + 1))
+        x = (x.double() * down.unsqueeze(1)).float()
+    if of in ("w", "all"):
+        w = (w.double() * 2.0 ** -(torch.arange(vocab, device="cuda", dtype=torch.float64) % (spread + 1)).unsqueeze(1)).float()
+    if of == "all":  # and far from 1 altogether
+        x, w = x * 2.0 ** -20, w * 2.0 ** 20
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    rows = linear_cross_entropy(xl, wl, t, bias=b, reduction="none")
+    rows.sum().backward()
+    xd, wd = x.double().requires_grad_(True), w.double().requires_grad_(True)
+    exact = torch.nn.functional.cross_entropy(xd @ wd.t() + b.double(), t, reduction="none")
+    exact.sum().backward()
+    A = (x.double().abs() @ w.double().abs().t()).amax(1) + b.double().abs().max()
+    Ez = (dim / 16 + 16) * 2 * U * A
+    assert bool(((rows.detach().double() - exact.detach()).abs() <= 2 * Ez + 2.0 ** -20 * exact.detach().clamp(min=1)).all())
+    # gradients: errors of probabilities (relative, by the row's Ez), of the planes, and of the sums
+    p = torch.softmax(x.double() @ w.double().t() + b.double(), 1)
+    dz = p.clone()
+    dz[torch.arange(n, device="cuda"), t] -= 1
+    Edz = (2 * Ez.unsqueeze(1) + 2.0 ** -19) * p + (vocab / 16 + 16) * 2 * U * dz.abs()
+    near(xl.grad, xd.grad, Edz @ w.double().abs(), "dx")
+    near(wl.grad, wd.grad, (Edz + (n / 16 + 16) * 2 * U * dz.abs()).t() @ x.double().abs(), "dw")
+
+
+def test_fp32_nonfinite_rows_stay_to_themselves():
+    from bpt_b200.loss import linear_cross_entropy
+    x, w, b, t = inputs(300, 500, 72, torch.float32)
+    want = linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    for bad in (float("nan"), float("inf"), 3e38):
+        y = x.clone()
+        y[7, 3] = bad
+        got = linear_cross_entropy(y, w, t, bias=b, reduction="none")
+        keep = torch.arange(300, device="cuda") != 7
+        assert torch.allclose(got[keep], want[keep], rtol=4e-6, atol=4e-6)  # 2 Ez of the module's note
+        if bad != 3e38:
+            assert bool(torch.isnan(got[7]))
