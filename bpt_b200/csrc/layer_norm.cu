@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(kBlock, kBlock == 256 ? 2 : 1)
 layer_norm_backward_kernel(const T *__restrict__ gy, const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma,
                            const float *__restrict__ mean_in, const float *__restrict__ rstd_in, T *__restrict__ da,
                            float *__restrict__ partial, int64_t n_rows, int dim, int tpr) {
+    tc5::let_next_start();  // the reduction, which waits for this kernel's end
     __shared__ float slots[2][2][16];
     extern __shared__ __align__(16) unsigned char smem[];  // rows ahead; at the end the sums, [rows of the block][dim]
     const int t = threadIdx.x & (tpr - 1), rows_here = kBlock / tpr, mine = threadIdx.x / tpr, step = tpr * kVec;
@@ -454,6 +455,7 @@ template <typename T>
 __global__ void __launch_bounds__(32 * kReduceRows)
 layer_norm_reduce_kernel(const float *__restrict__ partial, int n_partial, int dim, T *__restrict__ dgamma,
                          T *__restrict__ dbeta) {
+    tc5::wait_for_previous();
     __shared__ float part[kReduceRows][32];
     const int c = blockIdx.x * 32 + threadIdx.x;
     float s = 0.f;
@@ -566,9 +568,8 @@ int launch_layer_norm_backward(const void *gy, const void *x, const void *r, con
     });
     if (rc != BPT_OK) return rc;
     if (partial) {
-        layer_norm_reduce_kernel<T><<<(2 * dim + 31) / 32, dim3(32, kReduceRows), 0, stream>>>(
-            partial, static_cast<int>(grid), dim, static_cast<T *>(dgamma), static_cast<T *>(dbeta));
-        BPT_LAUNCH_CHECK();
+        BPT_CUDA(tc5::launch_after(layer_norm_reduce_kernel<T>, (2 * dim + 31) / 32, dim3(32, kReduceRows), 0, stream, partial,
+                                   static_cast<int>(grid), dim, static_cast<T *>(dgamma), static_cast<T *>(dbeta)));
     }
     return BPT_OK;
 }

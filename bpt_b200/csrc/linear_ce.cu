@@ -377,16 +377,18 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         mbar_init(bar_drain, 1);
         fence_mbar_init();
-        if (kKind != kProducts && blockIdx.x == 0) {
-            *p.ticket = 0u;
-            if (p.starts) *p.status = 0;
-        }
     }
     if (warp == kFinishWarps + 1) tmem_alloc_pair(tmem_slot, 512);
     fence_before_sync();
     __syncthreads();
     cluster_sync();  // both blocks' barriers are set up
     fence_after_sync();
+    let_next_start();
+    wait_for_previous();
+    if (kKind != kProducts && blockIdx.x == 0 && tid == 0) {
+        *p.ticket = 0u;
+        if (p.starts) *p.status = 0;
+    }
     const uint32_t tmem = *tmem_word;
     Work<kKind> work(p);
     Split split;
@@ -910,6 +912,7 @@ __global__ void __launch_bounds__(256, 2) linear_ce_few_kernel(const T *__restri
                                                             const T *__restrict__ bias, const int64_t *__restrict__ target, int n, int vocab,
                                                             int dim, float *__restrict__ partial, float *__restrict__ z_target,
                                                             unsigned *ticket, int *status) {
+    let_next_start();
     constexpr int kVec = 16 / sizeof(T), kFew = 8;
     extern __shared__ float xs[];  // [kTokens][dim]
     __shared__ float s_max[8][kTokens], s_sum[8][kTokens], s_z[8][kTokens];
@@ -1058,6 +1061,8 @@ struct LossParams {
 };
 
 template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_loss_kernel(const LossParams p) {
+    let_next_start();
+    wait_for_previous();
     const int64_t row = (static_cast<int64_t>(blockIdx.x) * kLossThreads + threadIdx.x) / kLanes;
     const int lane = threadIdx.x % kLanes;
     float loss = 0.f;
@@ -1257,6 +1262,8 @@ __global__ void linear_ce_top_kernel(const float *__restrict__ grad, const int64
 // Sums of a product's K parts (and of earlier pieces), in their order: a thread has 4 neighbouring columns.
 template <typename T>
 __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_constant__ Params p, int which) {
+    let_next_start();
+    wait_for_previous();
     const Product &q = p.product[which];
     const int64_t pieces = q.acc_ld / 4, rows = q.row_end - q.row_offset, total = rows * pieces, plane = static_cast<int64_t>(q.m_tiles) * kBM * q.acc_ld;
     const float scale = *p.status ? __int_as_float(0x7fffffff) : result_scale<T>(p, which);
@@ -1293,6 +1300,8 @@ __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_const
 template <typename T>
 __global__ void __launch_bounds__(256) linear_ce_bias_kernel(const __grid_constant__ Params p, int pairs, int each_m, float *acc, int add,
                                                              int last, T *__restrict__ out) {
+    let_next_start();
+    wait_for_previous();
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
     __shared__ float s_part[8][32];
     const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles, n = blockIdx.x * 32 / kBN;
@@ -1558,8 +1567,7 @@ template <typename T, int kKind> int launch_ce(const Maps &m, const Params &p, i
         BPT_CUDA(cudaFuncSetAttribute(linear_ce_kernel<T, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kKind)));
         if (device < 64) done.fetch_or(uint64_t(1) << device);
     }
-    linear_ce_kernel<T, kKind><<<2 * pairs, kThreads, smem_bytes(kKind), stream>>>(m.a, m.b, m.c, m.d, m.e, p);
-    BPT_LAUNCH_CHECK();
+    BPT_CUDA(launch_after(linear_ce_kernel<T, kKind>, 2 * pairs, kThreads, smem_bytes(kKind), stream, m.a, m.b, m.c, m.d, m.e, p));
     return BPT_OK;
 }
 
@@ -1682,9 +1690,9 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     l.ticket = f.ticket;
     l.status = f.status;
     // a row of many pieces (few rows, so many blocks shared each) is merged by a warp
-    if (l.pieces > 8 || s.pieces() > 8) linear_ce_loss_kernel<32><<<static_cast<unsigned>(ce_div(s.n * 32, kLossThreads)), kLossThreads, 0, stream>>>(l);
-    else linear_ce_loss_kernel<1><<<static_cast<unsigned>(ce_div(s.n, kLossThreads)), kLossThreads, 0, stream>>>(l);
-    BPT_LAUNCH_CHECK();
+    const bool many = l.pieces > 8 || s.pieces() > 8;
+    BPT_CUDA(launch_after(many ? linear_ce_loss_kernel<32> : linear_ce_loss_kernel<1>,
+                          static_cast<unsigned>(ce_div(many ? s.n * 32 : s.n, kLossThreads)), kLossThreads, 0, stream, l));
     return BPT_OK;
 }
 
@@ -1756,9 +1764,8 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             const int pairs = pairs_for(static_cast<int64_t>(g.m_tiles) * g.n_tiles);
             BPT_TRY((launch_ce<T, kGrad>(grad_maps, g, pairs, stream)));
             if (db) {
-                linear_ce_bias_kernel<T><<<static_cast<unsigned>(ce_div(cols, 32)), 256, 0, stream>>>(
-                    g, pairs, kFloat, f.db_acc ? f.db_acc + v0 : nullptr, n0 > 0, last_rows, static_cast<T *>(db) + v0);
-                BPT_LAUNCH_CHECK();
+                BPT_CUDA(launch_after(linear_ce_bias_kernel<T>, static_cast<unsigned>(ce_div(cols, 32)), 256, 0, stream, g, pairs, kFloat,
+                                      f.db_acc ? f.db_acc + v0 : nullptr, n0 > 0, last_rows, static_cast<T *>(db) + v0));
             }
             if (!dx && !dw) continue;
             BPT_TRY(make_map(&maps.a, kHalf, f.dz, rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, kRows));
@@ -1793,8 +1800,7 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
                 const Product &r = q.product[which];
                 if (r.parts <= 1) continue;
                 const int64_t blocks = std::min<int64_t>(ce_div((r.row_end - r.row_offset) * (r.acc_ld / 4), 256), 148 * 8);
-                linear_ce_parts_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(q, which);
-                BPT_LAUNCH_CHECK();
+                BPT_CUDA(launch_after(linear_ce_parts_kernel<T>, static_cast<unsigned>(blocks), 256, 0, stream, q, which));
             }
         }
     }

@@ -137,6 +137,25 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// Programmatic dependent launch: a kernel launched by launch_after may start when the one before it in the stream says so
+// (let_next_start) or ends; before it touches memory it waits for that one's end (wait_for_previous).
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+template <typename... Args, typename... Given>
+inline cudaError_t launch_after(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Given... given) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, static_cast<Args>(given)...);
+}
+
 // Waits for this warp's tcgen05.ld into r; r is named so that nothing that reads it moves before the wait.
 __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n"
