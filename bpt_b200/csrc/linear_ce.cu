@@ -6,7 +6,8 @@
 //     loss_i = lse_i - (1 - e) z_it - (e / V) sum_v z_iv
 //     d z_iv = g_i (exp(z_iv - lse_i) - e / V - (1 - e) [v = t])       (g_i: gradient that reaches loss_i)
 //     d x = dZ W,   d W = dZ^T X,   d b = column sums of dZ
-// Tokens whose target is `ignore_index` have loss 0 and g = 0.
+// Tokens whose target is `ignore_index` have loss 0 and g = 0.  The others are counted and listed first; where some are
+// ignored, the features of the others are brought together and only they are worked on (whatever the ignored ones hold).
 //
 // All four products run in one kernel shape on the 5th-generation tensor cores: a persistent pair of blocks (a cluster
 // of two on one pair of SMs) walks 256 x 256 tiles, 128 rows of the result in each block.  In each block one warp brings
@@ -68,11 +69,10 @@ enum { kReduceNone = 0, kReduceMean = 1, kReduceSum = 2 };
 struct Product {
     int m_tiles, n_tiles, k_tiles, n_ext;
     int parts, part_tiles;                 // K parts of a tile (each of part_tiles K blocks; sums go to `partial` if parts > 1)
-    int b0;                                // added to B's row coordinate
-    int64_t row_offset, row_end;           // rows of the output: row_offset + tile row, below row_end
+    int64_t row_offset, row_end;           // d w: rows of the output are row_offset + tile row, below row_end
     float *acc;                            // fp32 sums of earlier pieces (leading dimension acc_ld), or null
-    float *partial;                        // [part][m_tiles * 256][acc_ld]
-    int64_t acc_ld;
+    float *partial;                        // [part][row of the piece][acc_ld], partial_plane from part to part
+    int64_t acc_ld, partial_plane;
     int add, last;                         // acc holds earlier pieces; write `out`
     void *out;
     __host__ __device__ int64_t tiles() const { return static_cast<int64_t>(m_tiles) * n_tiles; }
@@ -81,13 +81,16 @@ struct Product {
 
 struct Params {
     int m_tiles, n_tiles, k_tiles, n_ext;  // stats, grad: tiles; columns in all (the last tile may be narrower)
-    int m_ext;                             // grad: rows of the piece
+    int m_ext, piece, pieces;              // tokens of the piece, if all count (the first is a0); which of how many it is
     int n_pairs;                           // plane products: 1 or 2; fp32: 3 or 6, as `split` says
     const unsigned *split;                 // fp32: see Split
     int dz_planes;                         // grad: planes of dZ that are written
     int a0, b0;                            // added to the row coordinate of A and of B
     int *status;                           // set to 1 when a wait ran out
     int64_t n_rows, ignore_index;          // tokens in all
+    const int *n_counted;                  // tokens that count, and which they are; rows of X, Z, dZ count these alone
+    const int32_t *index;
+    int gathered;                          // where some are ignored, X is read from a copy of the others' rows
     int vocab;
     const void *bias;
     const int64_t *target;
@@ -103,7 +106,6 @@ struct Params {
     int64_t col_ld;
     const float *count;
     const unsigned *grad_top;              // none: bits of max |g|
-    const unsigned char *clean;            // d w: per 64 tokens, 1 = read the copy with ignored rows zeroed
     // products: 0 = d x, 1 = d w.  The one with the longer units goes first, dealt in turn; pairs below `busy` have one
     // more of them.  The shorter units follow in runs of `after_busy` and `after` per pair.
     Product product[2];
@@ -165,6 +167,9 @@ __host__ __device__ __forceinline__ int first_tile(int64_t t, int g, int c) { re
 __host__ __device__ __forceinline__ int pair_of_tile(int64_t t, int g, int64_t i) {
     return static_cast<int>(((i + 1) * g + t - 1) / t) - 1;
 }
+
+// Of the pairs launched, those that have tiles.
+__device__ __forceinline__ int pairs_used(int pairs, int64_t tiles) { return static_cast<int>(min(static_cast<int64_t>(pairs), tiles)); }
 
 __device__ __forceinline__ void st_global_v8(void *p, const uint32_t (&v)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
@@ -246,57 +251,119 @@ template <typename T> __device__ __forceinline__ void store_row(T *row, int64_t 
     }
 }
 
+// How the two products of a piece are dealt to the pairs of blocks.
+struct Deal {
+    int pairs, first, busy, after_busy, after;
+    int steps;  // of the pair with the most work
+};
+// Unit lengths l0, l1 (in K blocks, with what a unit costs besides) and numbers u0, u1: the longer units in turn, then
+// runs of the shorter ones so that the pair with the most work has as little as possible.
+__host__ __device__ inline Deal deal(int pairs, int l0, int u0, int l1, int u1) {
+    Deal d;
+    d.pairs = pairs;
+    d.first = u0 > 0 && (l0 >= l1 || u1 == 0) ? 0 : 1;
+    const int long_l = d.first == 0 ? l0 : l1, long_u = d.first == 0 ? u0 : u1, short_l = d.first == 0 ? l1 : l0, short_u = d.first == 0 ? u1 : u0;
+    const int each = long_u / pairs;
+    d.busy = long_u % pairs;
+    auto room = [&](int t, int units) { return t < units * long_l ? 0 : (t - units * long_l) / short_l; };
+    int low = d.busy ? (each + 1) * long_l : each * long_l, high = low + (short_u / pairs + 1) * short_l + long_l;
+    while (short_u > 0 && low < high) {
+        const int t = (low + high) / 2;
+        if (d.busy * room(t, each + 1) + (pairs - d.busy) * room(t, each) >= short_u) high = t;
+        else low = t + 1;
+    }
+    d.steps = low;
+    d.after_busy = short_u > 0 ? room(low, each + 1) : 0;
+    d.after = short_u > 0 ? room(low, each) : 0;
+    return d;
+}
+// A unit's fixed cost, and that of its sums through memory where a tile has several parts, in K blocks of one product
+// (0.3 us): measured.
+constexpr int64_t kUnitSteps = 4, kPartSteps = 20;
+__host__ __device__ inline int unit_steps(int k_tiles, int parts, int n_pairs) {
+    return (k_tiles + parts - 1) / parts * n_pairs + kUnitSteps + (parts > 1 ? kPartSteps : 0);
+}
 // The work of a pair, in the order in which all its warps take it: a tile, the K blocks of it, and for the products
 // which product and part.
 template <int kKind> struct Work {
     const Params &p;
     int64_t at, end;              // stats, grad: consecutive tiles
     int pair, pairs, stage;       // products
-    int64_t stop_first;
+    int m_tiles;                  // stats, grad: with the tokens that count
+    int x_units, w_units, x_k, w_k, first, busy, after_busy, after;
+    int cur_tiles, cur_n, cur_k, cur_part;  // of the product that is being worked on
     int m, n, k0, k1, which, part;
-    __device__ explicit Work(const Params &p_) : p(p_) {
+    // rows: tokens of the piece that count
+    __device__ Work(const Params &p_, int rows) : p(p_) {
         pair = blockIdx.x >> 1;
         pairs = gridDim.x >> 1;
         which = part = 0;
+        m_tiles = (rows + kBM - 1) / kBM;
         if constexpr (kKind != kProducts) {
-            const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-            at = first_tile(total, pairs, pair);
-            end = first_tile(total, pairs, pair + 1);
+            const int64_t total = static_cast<int64_t>(m_tiles) * p.n_tiles;
+            pairs = pairs_used(pairs, total);
+            at = pair < pairs ? first_tile(total, pairs, pair) : 0;
+            end = pair < pairs ? first_tile(total, pairs, pair + 1) : 0;
             k0 = 0;
             k1 = p.k_tiles;
         } else {
+            const Product &x = p.product[0], &w = p.product[1];
+            x_units = x.m_tiles ? m_tiles * x.n_tiles * x.parts : 0;
+            w_units = static_cast<int>(w.units());
+            x_k = x.k_tiles;
+            w_k = (rows + kBK - 1) / kBK;
+            first = p.first;
+            busy = p.busy;
+            after_busy = p.after_busy;
+            after = p.after;
+        }
+    }
+    // products: where fewer tokens count, they are dealt again (by one thread for its block)
+    __device__ Deal deal_again(int n_pairs) const {
+        return deal(pairs, unit_steps(x_k, p.product[0].parts, n_pairs), x_units, unit_steps(w_k, p.product[1].parts, n_pairs), w_units);
+    }
+    __device__ void start() {
+        if constexpr (kKind == kProducts) {
             stage = 0;
             at = pair;
-            end = p.product[p.first].units();
+            take(first);
+            end = first == 0 ? x_units : w_units;
         }
+    }
+    __device__ void take(int product) {
+        which = product;
+        const Product &q = p.product[product];
+        cur_n = q.n_tiles;
+        cur_k = product == 0 ? x_k : w_k;
+        cur_tiles = (product == 0 ? x_units : w_units) / q.parts;
+        cur_part = (cur_k + q.parts - 1) / q.parts;
     }
     __device__ bool next() {
         if constexpr (kKind != kProducts) {
             if (at >= end) return false;
             // stats: the vocabulary blocks of a token block in a row; grad: the token blocks of a vocabulary block
-            m = static_cast<int>(kKind == kStats ? at / p.n_tiles : at % p.m_tiles);
-            n = static_cast<int>(kKind == kStats ? at % p.n_tiles : at / p.m_tiles);
+            m = static_cast<int>(kKind == kStats ? at / p.n_tiles : at % m_tiles);
+            n = static_cast<int>(kKind == kStats ? at % p.n_tiles : at / m_tiles);
             ++at;
             return true;
         } else {
             if (stage == 0 && at >= end) {
                 stage = 1;
-                const int64_t units = p.product[1 - p.first].units();
-                const int64_t before = pair < p.busy ? static_cast<int64_t>(pair) * p.after_busy
-                                                     : static_cast<int64_t>(p.busy) * p.after_busy + static_cast<int64_t>(pair - p.busy) * p.after;
+                const int64_t before = pair < busy ? static_cast<int64_t>(pair) * after_busy
+                                                   : static_cast<int64_t>(busy) * after_busy + static_cast<int64_t>(pair - busy) * after;
                 at = before;
-                end = before + (pair < p.busy ? p.after_busy : p.after);
+                end = before + (pair < busy ? after_busy : after);
+                take(1 - first);
+                const int units = first == 0 ? w_units : x_units;
                 if (end > units) end = units;
             }
             if (at >= end) return false;
-            which = stage == 0 ? p.first : 1 - p.first;
-            const Product &q = p.product[which];
-            part = static_cast<int>(at / q.tiles());
-            const int tile = static_cast<int>(at % q.tiles());
-            m = tile / q.n_tiles;
-            n = tile % q.n_tiles;
-            k0 = part * q.part_tiles;
-            k1 = min(k0 + q.part_tiles, q.k_tiles);
+            part = static_cast<int>(at) / cur_tiles;
+            const int tile = static_cast<int>(at) - part * cur_tiles;
+            m = tile / cur_n;
+            n = tile - m * cur_n;
+            k0 = part * cur_part;
+            k1 = min(k0 + cur_part, cur_k);
             at += stage == 0 ? pairs : 1;
             return true;
         }
@@ -344,8 +411,23 @@ template <typename T> __device__ __forceinline__ float result_scale(const Params
     return scale * (1.f / kDzScale<T>);
 }
 
-// map_a, map_b: stats, grad: X and W rows; products: dZ rows and W columns.  map_c, map_d, map_e: dZ columns, X columns,
-// the copy of X with ignored rows zeroed.
+// A piece's part of the tokens that count, evenly cut where some are ignored.
+struct PieceRows {
+    int first, rows;
+};
+__device__ __forceinline__ PieceRows piece_rows(const Params &p) {
+    const int counted = *p.n_counted;
+    PieceRows r{p.a0, p.m_ext};
+    if (counted < p.n_rows) {
+        const int each = ((counted + p.pieces - 1) / p.pieces + kBM - 1) / kBM * kBM;
+        r.first = min(p.piece * each, counted);
+        r.rows = min(each, counted - r.first);
+    }
+    return r;
+}
+
+// map_a, map_b: stats, grad: X and W rows; products: dZ rows and W columns.  map_c: dZ, as it is stored (grad), its columns
+// (products).  map_d, map_e: stats, grad: the copy of X, rows; products: X columns, those of its copy.
 template <typename T, int kKind>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
@@ -390,7 +472,11 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (p.starts) *p.status = 0;
     }
     const uint32_t tmem = *tmem_word;
-    Work<kKind> work(p);
+    const bool some_ignored = *p.n_counted < p.n_rows, copied = some_ignored && p.gathered;
+    const int32_t *const index = some_ignored ? p.index : nullptr;
+    const PieceRows part_of = piece_rows(p);
+    const int rows_here = part_of.rows, a0 = part_of.first;
+    Work<kKind> work(p, rows_here);
     Split split;
     if constexpr (kPrecise) split = read_split(p.split);
     const int first_pair = 6 - (kPrecise ? (split.half ? 3 : 6) : p.n_pairs);
@@ -398,6 +484,24 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     // and the large one
     const int groups = kPrecise && split.half ? 2 : 1;
     auto group_pairs = [&](int group) { return groups == 1 ? 6 - first_pair : group == 0 ? 2 : 1; };
+    if constexpr (kKind == kProducts) {
+        if (some_ignored) {
+            int *const s_deal = reinterpret_cast<int *>(smem_raw);  // the bias' place, which products have no use for
+            if (tid == 0) {
+                const Deal d = work.deal_again(6 - first_pair);
+                s_deal[0] = d.first;
+                s_deal[1] = d.busy;
+                s_deal[2] = d.after_busy;
+                s_deal[3] = d.after;
+            }
+            __syncthreads();
+            work.first = s_deal[0];
+            work.busy = s_deal[1];
+            work.after_busy = s_deal[2];
+            work.after = s_deal[3];
+        }
+    }
+    work.start();
     if (warp >= kFinishWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
     if (warp == kFinishWarps) {
@@ -419,18 +523,18 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             const int b_bytes = kKind == kProducts ? chunks * kChunkBytes : kBBytes;
                             if (rank == 0) mbar_expect(bar_full + 8 * s, 2 * (kABytes + b_bytes));
                             if constexpr (kKind == kProducts) {
-                                const int b_row = p.product[work.which].b0 + k * kBK;
+                                const int b_row = (work.which == 0 ? p.b0 : a0) + k * kBK;
                                 if (work.which == 0) {
                                     tma_load_pair(a, &map_a, k * kBK, m0, pa, full);
                                     for (int c = 0; c < chunks; ++c) tma_load_pair(b + c * kChunkBytes, &map_b, n0 + 64 * c, b_row, pb, full);
                                 } else {
                                     tma_load_pair(a, &map_c, m0, k * kBK, pa, full);
                                     tma_load_pair(a + kChunkBytes, &map_c, m0 + 64, k * kBK, pa, full);
-                                    const CUtensorMap *map = p.clean && p.clean[b_row / kBK] ? &map_e : &map_d;
-                                    for (int c = 0; c < chunks; ++c) tma_load_pair(b + c * kChunkBytes, map, n0 + 64 * c, b_row, pb, full);
+                                    for (int c = 0; c < chunks; ++c)
+                                        tma_load_pair(b + c * kChunkBytes, copied ? &map_e : &map_d, n0 + 64 * c, b_row, pb, full);
                                 }
                             } else {
-                                tma_load_pair(a, &map_a, k * kBK, p.a0 + m0, pa, full);
+                                tma_load_pair(a, copied ? &map_d : &map_a, k * kBK, a0 + m0, pa, full);
                                 tma_load_pair(b, &map_b, k * kBK, p.b0 + n0, pb, full);
                             }
                             ++issued;
@@ -511,11 +615,11 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         float run_max = -INFINITY, run_sum = 0.f, run_z = 0.f;
         int tgt = -1;
         float row_lse = 0.f, row_l2 = 0.f, row_g = 0.f, uniform = 0.f;
-        bool row_plain = true, row_skips = false;  // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0
-        float scales[2] = {1.f, 1.f};
+        bool row_plain = true, row_skips = false;  // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0 (none there)
+        float x_scale = 1.f, w_scale = 1.f;
         if constexpr (kKind == kProducts) {
-            scales[0] = result_scale<T>(p, 0);
-            scales[1] = result_scale<T>(p, 1);
+            x_scale = result_scale<T>(p, 0);
+            w_scale = result_scale<T>(p, 1);
         }
         // grad, 16-bit: column sums over the pair's token blocks of one vocabulary block
         constexpr bool kKeepSums = kKind == kGrad && !kPrecise;
@@ -556,18 +660,17 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 parity ^= 1;
                 if (m != row_m) {
                     row_m = m;
-                    const int64_t row = p.a0 + static_cast<int64_t>(m) * kBM + trow;
-                    const bool live = row < p.n_rows;
-                    const int64_t target = live ? p.target[row] : p.ignore_index;
-                    const bool counted = live && target != p.ignore_index;
-                    tgt = counted && target >= 0 && target < p.vocab ? static_cast<int>(target) : -1;
+                    const bool live = m * kBM + trow < rows_here;
+                    const int64_t at = a0 + static_cast<int64_t>(m) * kBM + trow, row = live && index ? index[at] : at;
+                    const int64_t target = live ? p.target[row] : -1;
+                    tgt = target >= 0 && target < p.vocab ? static_cast<int>(target) : -1;
                     if constexpr (kKind == kStats) {
                         run_max = -INFINITY;
                         run_sum = run_z = 0.f;
                     } else {
                         row_lse = live ? p.lse[row] : 0.f;
                         row_g = 0.f;
-                        if (counted) {
+                        if (live) {
                             row_g = 1.f;
                             if (p.reduction == kReduceNone) row_g = p.grad[row] * (1.f / top_scale(*p.grad_top));
                             if (tgt < 0) row_g = __int_as_float(0x7fffffff);  // no such class: the gradients say so
@@ -581,7 +684,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 }
                 if constexpr (kKeepSums) {
                     if (n != col_n && col_n >= 0 && p.col_sums) {
-                        const int piece = work.pair - pair_of_tile(static_cast<int64_t>(p.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(col_n) * p.m_tiles);
+                        const int piece = work.pair - pair_of_tile(static_cast<int64_t>(work.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(col_n) * work.m_tiles);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             store_col_sums(col_sum[j], j, col_n, piece);
@@ -637,7 +740,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             float zt = 0.f;
 #pragma unroll
                             for (int i = 0; i < 32; ++i) zt = i == local ? v[i] : zt;
-                            p.z_target[p.a0 + static_cast<int64_t>(m) * kBM + trow] = zt * kUnit;
+                            p.z_target[a0 + static_cast<int64_t>(m) * kBM + trow] = zt * kUnit;
                         }
                         // Sums of exp(v - run_max), where run_max is a number near the largest so far: it moves only when
                         // a sum gets large (or is not a number), which saves looking for the maximum of every 32.
@@ -690,7 +793,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                 }
                             }
                         }
-                        if (row_skips) {  // some row of the warp is ignored: zeros there, whatever its logits are
+                        if (row_skips) {  // some of the warp's rows are not there or have no gradient: zeros, whatever the logits are
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = row_g == 0.f ? 0.f : v[i];
                         }
@@ -705,8 +808,8 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         auto send = [&](int x, int plane, uint32_t tile) {
                             fence_async_smem();
                             __syncwarp();
-                            if (lane == 0) {
-                                if (y < p.m_ext) tma_store(&map_c, x, y, plane, tile);
+                            if (lane == 0) {  // rows that are not there go out as zeros: the next product reads whole K blocks
+                                tma_store(&map_c, x, y, plane, tile);
                                 store_commit();
                             }
                             out_at ^= 1;
@@ -763,21 +866,21 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     }
                 } else {
                     const Product &q = p.product[work.which];
-                    const int64_t in_piece = static_cast<int64_t>(m) * kBM + trow, row = q.row_offset + in_piece;
+                    const int64_t in_piece = static_cast<int64_t>(m) * kBM + trow;
                     const int col = n * kBN + c0, left = q.n_ext - col;
-                    if (row < q.row_end) {
+                    if (work.which == 0 ? in_piece < rows_here : q.row_offset + in_piece < q.row_end) {
                         if (q.parts > 1) {
-                            store_row(q.partial + (static_cast<int64_t>(work.part) * q.m_tiles * kBM + in_piece) * q.acc_ld, q.acc_ld * 4, col, left, v);
+                            store_row(q.partial + work.part * q.partial_plane + in_piece * q.acc_ld, q.acc_ld * 4, col, left, v);
                         } else {
+                            const int64_t at = (work.which == 0 ? a0 : q.row_offset) + in_piece, row = work.which == 0 && index ? index[at] : at;
                             if (q.add) {
                                 const float *sums = q.acc + row * q.acc_ld + col;
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) v[i] += i < left ? sums[i] : 0.f;
                             }
                             if (q.last) {
-                                const bool ignored = work.which == 0 && p.target[row] == p.ignore_index;
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] = ignored ? 0.f : v[i] * (work.which == 0 ? scales[0] : scales[1]);
+                                for (int i = 0; i < 32; ++i) v[i] *= work.which == 0 ? x_scale : w_scale;
                                 store_row(static_cast<T *>(q.out) + row * q.n_ext, q.n_ext * static_cast<int64_t>(sizeof(T)), col, left, v);
                             } else {
                                 store_row(q.acc + row * q.acc_ld, q.acc_ld * 4, col, left, v);
@@ -827,7 +930,8 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     }
                 }
             } else {
-                ok = mbar_wait_or_stop(bar_ready + 8 * buf, ready_phase, stop);
+                const bool empty = kKind == kProducts && work.k1 <= work.k0;  // no token counts: there are no products
+                ok = empty || mbar_wait_or_stop(bar_ready + 8 * buf, ready_phase, stop);
                 if constexpr (kKind != kProducts) ok = !finish_barrier_or(!ok);
                 else ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -838,8 +942,13 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     if (first + 32 * j < cols) {
                         uint32_t r[32];
                         float v[32];
-                        tmem_ld32(tmem + lanes + buf * kBN + first + 32 * j, r);
-                        tmem_ld_wait_for(r);
+                        if (!empty) {
+                            tmem_ld32(tmem + lanes + buf * kBN + first + 32 * j, r);
+                            tmem_ld_wait_for(r);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) r[i] = 0u;
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
                         finish(v, first + 32 * j);
@@ -854,12 +963,12 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         __syncwarp();
                     }
                 }
-                release();
+                if (!empty) release();
             }
             if constexpr (kKind == kStats) {
                 if (n == p.n_tiles - 1 || work.at == work.end) {  // the last tile of these rows in this pair
-                    const int64_t rows_padded = static_cast<int64_t>(p.m_tiles) * kBM;
-                    const int piece = work.pair - pair_of_tile(static_cast<int64_t>(p.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(m) * p.n_tiles);
+                    const int64_t rows_padded = static_cast<int64_t>(work.m_tiles) * kBM;
+                    const int piece = work.pair - pair_of_tile(static_cast<int64_t>(work.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(m) * p.n_tiles);
                     float *at = p.partial + (static_cast<int64_t>(piece) * 2 + half) * 3 * rows_padded + static_cast<int64_t>(m) * kBM + trow;
                     at[0] = run_max;
                     at[rows_padded] = run_sum;
@@ -869,7 +978,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         if constexpr (kKeepSums) {
             if (col_n >= 0 && p.col_sums) {
-                const int piece = work.pair - pair_of_tile(static_cast<int64_t>(p.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(col_n) * p.m_tiles);
+                const int piece = work.pair - pair_of_tile(static_cast<int64_t>(work.m_tiles) * p.n_tiles, work.pairs, static_cast<int64_t>(col_n) * work.m_tiles);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) store_col_sums(col_sum[j], j, col_n, piece);
             }
@@ -894,7 +1003,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 __threadfence();
                 if (*static_cast<volatile int *>(p.status)) {
                     const T nan = from_acc<T>(__int_as_float(0x7fffffff));
-                    if (p.product[0].tiles() && p.product[0].last) static_cast<T *>(p.product[0].out)[p.product[0].row_offset * p.product[0].n_ext] = nan;
+                    if (p.product[0].tiles() && p.product[0].last) static_cast<T *>(p.product[0].out)[static_cast<int64_t>(p.a0) * p.product[0].n_ext] = nan;
                     if (p.product[1].tiles() && p.product[1].last) static_cast<T *>(p.product[1].out)[p.product[1].row_offset * p.product[1].n_ext] = nan;
                     if (p.spoilt) *static_cast<T *>(p.spoilt) = nan;
                 }
@@ -1050,9 +1159,11 @@ struct LossParams {
     const float *partial, *z_target;
     const int64_t *target;
     int64_t n_rows, ignore_index;
-    int m_tiles, n_tiles, pairs, vocab, reduction;
+    const int *n_counted;  // null: rows are all the tokens, ignored ones among them
+    const int32_t *index;
+    int n_tiles, pairs, vocab, reduction;
     int pieces;            // of every row, or 0: what the tiles' dealing gives
-    int64_t rows_padded;   // between a piece's numbers
+    int64_t rows_padded;   // between a piece's numbers, or 0: whole tiles of the rows
     float smoothing, unit;  // unit: of a piece's maximum, in logits
     float *loss, *lse, *count;
     double *block_sums;  // [blocks][sum, count]
@@ -1067,10 +1178,13 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
     const int lane = threadIdx.x % kLanes;
     float loss = 0.f;
     bool counted = false;
-    if (row < p.n_rows) {
-        const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles, m = row / kBM, rows_padded = p.rows_padded;
+    const int64_t n_rows = p.n_counted ? *p.n_counted : p.n_rows;
+    if (row < n_rows) {
+        const int64_t m_tiles = (n_rows + kBM - 1) / kBM, total = m_tiles * p.n_tiles, m = row / kBM;
+        const int64_t rows_padded = p.rows_padded ? p.rows_padded : m_tiles * kBM;
+        const int pairs = pairs_used(p.pairs, total);
         const int pieces = p.pieces ? p.pieces
-                                    : 2 * (pair_of_tile(total, p.pairs, (m + 1) * p.n_tiles - 1) - pair_of_tile(total, p.pairs, m * p.n_tiles) + 1);
+                                    : 2 * (pair_of_tile(total, pairs, (m + 1) * p.n_tiles - 1) - pair_of_tile(total, pairs, m * p.n_tiles) + 1);
         float top = -INFINITY, sum = 0.f, z = 0.f;
         for (int i = lane; i < pieces; i += kLanes) top = fmaxf(top, p.partial[static_cast<int64_t>(i) * 3 * rows_padded + row]);
 #pragma unroll
@@ -1088,7 +1202,7 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
         }
         if (lane == 0) {
             const float lse = top * p.unit + logf(sum);
-            const int64_t target = p.target[row];
+            const int64_t token = n_rows < p.n_rows ? p.index[row] : row, target = p.target[token];
             counted = target != p.ignore_index;
             if (counted) {
                 const bool known = target >= 0 && target < p.vocab;
@@ -1097,8 +1211,8 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
                 if (p.smoothing != 0.f) loss += p.smoothing * (zt - z / static_cast<float>(p.vocab));
             }
             if (*p.status) loss = __int_as_float(0x7fffffff);
-            if (p.lse) p.lse[row] = lse;
-            if (p.reduction == kReduceNone) p.loss[row] = loss;
+            if (p.lse) p.lse[token] = lse;
+            if (p.reduction == kReduceNone) p.loss[token] = loss;
         }
     }
     if (p.reduction == kReduceNone) return;
@@ -1147,8 +1261,7 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
 }
 
 // ---- operands that TMA cannot read where they lie (fp32, rows or bases off 16 bytes): copied into rows of a multiple
-// of 8 elements, fp32 as planes.  Rows whose target is ignored (target given) are zeroed: their features may hold
-// anything, and 0 * NaN would reach every gradient of W.
+// of 8 elements, fp32 as planes.
 __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *__restrict__ x, int64_t ldx, int64_t x_rows, const float *__restrict__ w,
                                                                int64_t ldw, int64_t w_rows, int dim, const int64_t *__restrict__ target,
                                                                int64_t ignore_index, unsigned *__restrict__ found) {
@@ -1187,18 +1300,21 @@ __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *__re
 
 template <typename T>
 __global__ void linear_ce_pack_kernel(const T *__restrict__ src, int64_t ld, int64_t rows, int dim, uint16_t *__restrict__ dst,
-                                      int64_t dst_ld, int64_t plane, const int64_t *__restrict__ target, int64_t ignore_index,
+                                      int64_t dst_ld, int64_t plane, const int32_t *__restrict__ index, const int *__restrict__ n_counted,
                                       const unsigned *__restrict__ found, int is_w) {
-    const int64_t pieces = dst_ld / 8, total = rows * pieces;
+    // X: the rows that count, and rows of zeros up to a whole K block
+    const int64_t counted = n_counted ? *n_counted : rows;
+    const int64_t pieces = dst_ld / 8, total = min((counted + kBK - 1) / kBK * kBK, rows) * pieces;
     Split split;
     if constexpr (kIsFloat<T>) split = read_split(found);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t row = i / pieces;
         const int c = static_cast<int>(i % pieces) * 8;
-        const bool skip = target && target[row] == ignore_index;
+        // the index is there where some tokens are ignored
+        const T *from = src + (counted < rows && row < counted ? index[row] : row) * ld + c;
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = !skip && c + j < dim ? to_acc<T>(src[row * ld + c + j]) : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = row < counted && c + j < dim ? to_acc<T>(from[j]) : 0.f;
         if constexpr (kIsFloat<T>) {
             if (split.half) {
 #pragma unroll
@@ -1219,33 +1335,92 @@ __global__ void linear_ce_pack_kernel(const T *__restrict__ src, int64_t ld, int
     }
 }
 
-// Per 64 tokens: whether any is ignored; their rows are then copied with the ignored ones zeroed, and the dW product
-// reads the copy.  Where nothing is ignored nothing is copied.
-__global__ void __launch_bounds__(256) linear_ce_clean_kernel(const uint16_t *__restrict__ x, int64_t ld, int64_t rows, int dim,
-                                                              const int64_t *__restrict__ target, int64_t ignore_index,
-                                                              uint16_t *__restrict__ copy, int64_t copy_ld,
-                                                              unsigned char *__restrict__ clean) {
-    __shared__ unsigned char skip[64];
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 64;
-    bool ignored = false;
-    if (threadIdx.x < 64) {
-        ignored = row0 + threadIdx.x < rows && target[row0 + threadIdx.x] == ignore_index;
-        skip[threadIdx.x] = ignored;
+// ---- the tokens that count: how many of each 256, then, where some are ignored, which they are, in their order.
+constexpr int kTokenBlock = 256;
+__global__ void __launch_bounds__(kTokenBlock) linear_ce_count_kernel(const int64_t *__restrict__ target, int64_t n, int64_t ignore_index,
+                                                                      int32_t *__restrict__ counts) {
+    let_next_start();
+    wait_for_previous();
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kTokenBlock + threadIdx.x;
+    const int here = __syncthreads_count(i < n && target[i] != ignore_index);
+    if (threadIdx.x == 0) counts[blockIdx.x] = here;
+}
+
+__device__ __forceinline__ int block_sum(int v, int *s_warp) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < kTokenBlock / 32; ++i) v += s_warp[i];
+    return v;
+}
+
+// A column of blocks (four share the rows' copying, a warp a row: latency) writes the index of its 256 tokens, brings the features of those that count to their places in the copy (if
+// given; the last block adds rows of zeros up to a whole K block), and puts zeros where the ignored ones' loss (reduction
+// none) and rows of d x (backward) go.  Where every token counts it does nothing.
+__global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uint16_t *__restrict__ x, int64_t ld, int64_t n, int dim,
+                                                                       const int64_t *__restrict__ target, int64_t ignore_index,
+                                                                       const int32_t *__restrict__ counts, int32_t *__restrict__ index,
+                                                                       int *__restrict__ n_counted, uint16_t *__restrict__ copy,
+                                                                       int64_t copy_ld, unsigned char *__restrict__ dx, int64_t dx_row_bytes,
+                                                                       float *__restrict__ loss) {
+    __shared__ int s_warp[kTokenBlock / 32], s_place[kTokenBlock];
+    let_next_start();
+    wait_for_previous();
+    int all = 0, before = 0;
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += kTokenBlock) {
+        const int v = counts[i];
+        all += v;
+        if (i < blockIdx.x) before += v;
     }
-    const bool any = __syncthreads_or(ignored);
-    if (threadIdx.x == 0) clean[blockIdx.x] = any;
-    if (!any) return;
-    const int pieces = (dim + 7) / 8;
-    for (int i = threadIdx.x; i < 64 * pieces; i += 256) {
-        const int r = i / pieces, c = i % pieces * 8;
-        if (row0 + r >= rows) break;
-        const uint16_t *from = x + (row0 + r) * ld + c;
-        uint16_t *to = copy + (row0 + r) * copy_ld + c;
-        if (c + 8 <= dim) {
-            *reinterpret_cast<uint4 *>(to) = skip[r] ? make_uint4(0u, 0u, 0u, 0u) : *reinterpret_cast<const uint4 *>(from);
-        } else {
-            for (int j = 0; j < dim - c; ++j) to[j] = skip[r] ? uint16_t(0) : from[j];
+    all = block_sum(all, s_warp);
+    const bool last = blockIdx.x == gridDim.x - 1;
+    if (last && blockIdx.y == 0 && threadIdx.x == 0) *n_counted = all;
+    if (all == n) return;
+    before = block_sum(before, s_warp);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t start = static_cast<int64_t>(blockIdx.x) * kTokenBlock, token = start + threadIdx.x;
+    const bool counts_here = token < n && target[token] != ignore_index;
+    const unsigned ballot = __ballot_sync(0xffffffffu, counts_here);
+    __syncthreads();
+    if (lane == 0) s_warp[warp] = __popc(ballot);
+    __syncthreads();
+    int place = before + __popc(ballot & ((1u << lane) - 1u));
+    for (int i = 0; i < warp; ++i) place += s_warp[i];
+    s_place[threadIdx.x] = counts_here ? place : -1;
+    if (blockIdx.y == 0) {
+        if (counts_here) index[place] = static_cast<int32_t>(token);
+        else if (loss && token < n) loss[token] = 0.f;
+    }
+    __syncthreads();
+    const bool dx_wide = ((reinterpret_cast<uintptr_t>(dx) | dx_row_bytes) & 15) == 0;
+    for (int t = blockIdx.y * (kTokenBlock / 32) + warp; t < kTokenBlock && start + t < n; t += gridDim.y * (kTokenBlock / 32)) {  // a warp a row
+        const int to_row = s_place[t];
+        if (to_row >= 0 && copy) {
+            const uint16_t *from = x + (start + t) * ld;
+            uint16_t *to = copy + to_row * copy_ld;
+            for (int c = lane * 8; c < dim; c += 256) {
+                if (c + 8 <= dim) {
+                    *reinterpret_cast<uint4 *>(to + c) = *reinterpret_cast<const uint4 *>(from + c);
+                } else {
+                    for (int j = c; j < dim; ++j) to[j] = from[j];
+                }
+            }
+        } else if (to_row < 0 && dx) {
+            unsigned char *to = dx + (start + t) * dx_row_bytes;
+            if (dx_wide) {
+                for (int64_t c = lane * 16; c < dx_row_bytes; c += 512) *reinterpret_cast<uint4 *>(to + c) = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+                for (int64_t c = lane * 2; c < dx_row_bytes; c += 64) *reinterpret_cast<uint16_t *>(to + c) = uint16_t(0);
+            }
         }
+    }
+    if (last && blockIdx.y == 0 && copy) {
+        const int64_t end = min((static_cast<int64_t>(all) + kBK - 1) / kBK * kBK, n);
+        for (int64_t row = all + warp; row < end; row += kTokenBlock / 32)
+            for (int c = lane; c < dim; c += 32) copy[row * copy_ld + c] = 0;
     }
 }
 
@@ -1265,15 +1440,16 @@ __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_const
     let_next_start();
     wait_for_previous();
     const Product &q = p.product[which];
-    const int64_t pieces = q.acc_ld / 4, rows = q.row_end - q.row_offset, total = rows * pieces, plane = static_cast<int64_t>(q.m_tiles) * kBM * q.acc_ld;
+    const int64_t pieces = q.acc_ld / 4, rows = which == 0 ? piece_rows(p).rows : q.row_end - q.row_offset, total = rows * pieces;
+    const int32_t *const index = which == 0 && *p.n_counted < p.n_rows ? p.index : nullptr;
     const float scale = *p.status ? __int_as_float(0x7fffffff) : result_scale<T>(p, which);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t in_piece = i / pieces, row = q.row_offset + in_piece;
+        const int64_t in_piece = i / pieces, at = (which == 0 ? piece_rows(p).first : q.row_offset) + in_piece, row = index ? index[at] : at;
         const int col = static_cast<int>(i % pieces) * 4, left = min(4, q.n_ext - col);
         const float *from = q.partial + in_piece * q.acc_ld + col;
         float4 s = *reinterpret_cast<const float4 *>(from);
         for (int k = 1; k < q.parts; ++k) {
-            const float4 t = *reinterpret_cast<const float4 *>(from + k * plane);
+            const float4 t = *reinterpret_cast<const float4 *>(from + k * q.partial_plane);
             s.x += t.x;
             s.y += t.y;
             s.z += t.z;
@@ -1288,8 +1464,7 @@ __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_const
             if (!q.last) {
                 sums[j] = v[j];
             } else {
-                const bool ignored = which == 0 && p.target[row] == p.ignore_index;
-                static_cast<T *>(q.out)[row * q.n_ext + col + j] = from_acc<T>(ignored ? 0.f : v[j] * scale);
+                static_cast<T *>(q.out)[row * q.n_ext + col + j] = from_acc<T>(v[j] * scale);
             }
         }
     }
@@ -1304,8 +1479,10 @@ __global__ void __launch_bounds__(256) linear_ce_bias_kernel(const __grid_consta
     wait_for_previous();
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
     __shared__ float s_part[8][32];
-    const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles, n = blockIdx.x * 32 / kBN;
-    const int pieces = each_m ? p.m_tiles : pair_of_tile(total, pairs, (n + 1) * p.m_tiles - 1) - pair_of_tile(total, pairs, n * p.m_tiles) + 1;
+    const int64_t m_tiles = (piece_rows(p).rows + kBM - 1) / kBM, total = m_tiles * p.n_tiles, n = blockIdx.x * 32 / kBN;
+    int pieces = static_cast<int>(m_tiles);
+    pairs = pairs_used(pairs, total);
+    if (!each_m && m_tiles) pieces = pair_of_tile(total, pairs, (n + 1) * m_tiles - 1) - pair_of_tile(total, pairs, n * m_tiles) + 1;
     float s = 0.f;
     if (c < p.n_ext)
         for (int r = part; r < pieces * 8; r += 8) s += p.col_sums[r * p.col_ld + c];
@@ -1376,14 +1553,21 @@ struct ForwardSpace {
     double *block_sums;
     unsigned *ticket, *found;
     int *status;
-    uint16_t *x, *w;
+    uint16_t *x, *w, *gathered;
+    int *n_counted;
+    int32_t *index, *counts;
     ForwardSpace(Workspace &ws, const Shape &s) {
         status = ws.take<int>(1);
         ticket = ws.take<unsigned>(1);
         found = ws.take<unsigned>(4);
         block_sums = ws.take<double>(2 * ce_div(s.n * 32, kLossThreads));
         z_target = ws.take<float>(s.n);
-        partial = ws.take<float>(s.few ? static_cast<int64_t>(kFewBlocks) * 3 * s.n : s.pieces() * 2 * 3 * s.m_tiles() * kBM);
+        // pieces x rows, with whatever part of the tokens counts: at most (pairs + two a block of rows) blocks of rows
+        partial = ws.take<float>(s.few ? static_cast<int64_t>(kFewBlocks) * 3 * s.n : (kPairs + 2 * s.m_tiles()) * 2 * 3 * kBM);
+        n_counted = ws.take<int>(1);
+        index = s.few ? nullptr : ws.take<int32_t>(s.n);
+        counts = s.few ? nullptr : ws.take<int32_t>(ce_div(s.n, kTokenBlock));
+        gathered = s.few || s.pack_x ? nullptr : ws.take<uint16_t>(s.n * s.packed_ld);
         x = s.pack_x && !s.few ? ws.take<uint16_t>(s.packed(s.n)) : nullptr;
         w = s.pack_w && !s.few ? ws.take<uint16_t>(s.packed(s.vocab)) : nullptr;
     }
@@ -1394,50 +1578,23 @@ struct ForwardSpace {
 // 64 MB 1340 / 1987 us, 128 MB 1075 / 1744, 256 MB 892 / 1557, 512 MB 866 / 1533.
 constexpr int64_t kDzBytes = 256 << 20;
 
-// How the two products of a piece are dealt to the pairs of blocks.
-struct Deal {
-    int pairs, first, busy, after_busy, after;
-    int64_t steps;  // of the pair with the most work
-};
-// Unit lengths l0, l1 (in K blocks, with what a unit costs besides) and numbers u0, u1: the longer units in turn, then
-// runs of the shorter ones so that the pair with the most work has as little as possible.
-Deal deal(int64_t l0, int64_t u0, int64_t l1, int64_t u1) {
-    Deal d;
-    d.pairs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kPairs, u0 + u1)));
-    d.first = u0 > 0 && (l0 >= l1 || u1 == 0) ? 0 : 1;
-    const int64_t long_l = d.first == 0 ? l0 : l1, long_u = d.first == 0 ? u0 : u1, short_l = d.first == 0 ? l1 : l0, short_u = d.first == 0 ? u1 : u0;
-    const int64_t each = long_u / d.pairs;
-    d.busy = static_cast<int>(long_u % d.pairs);
-    auto room = [&](int64_t t, int64_t units) { return t < units * long_l ? 0 : (t - units * long_l) / short_l; };
-    int64_t low = d.busy ? (each + 1) * long_l : each * long_l, high = low + (short_u / d.pairs + 1) * short_l + long_l;
-    while (short_u > 0 && low < high) {
-        const int64_t t = (low + high) / 2;
-        if (d.busy * room(t, each + 1) + (d.pairs - d.busy) * room(t, each) >= short_u) high = t;
-        else low = t + 1;
-    }
-    d.steps = low;
-    d.after_busy = short_u > 0 ? static_cast<int>(room(low, each + 1)) : 0;
-    d.after = short_u > 0 ? static_cast<int>(room(low, each)) : 0;
-    return d;
-}
-// A unit's fixed cost, and that of its sums through memory where a tile has several parts, in K blocks of one product
-// (0.3 us): measured.
-constexpr int64_t kUnitSteps = 4, kPartSteps = 20;
 // What a launch costs in K blocks, and the elements of a sum that is read and written once more in the time of one.
 constexpr int64_t kLaunchSteps = 15, kStepElements = 200000;
 // Splits the longer tiles along K where that shortens the work of the pair with the most of it: few tiles, long K.
 Deal split_and_deal(Product &x, Product &w, int n_pairs) {
-    auto steps = [&](const Product &q, int parts) {
-        return ce_div(q.k_tiles, parts) * n_pairs + kUnitSteps + (parts > 1 ? kPartSteps : 0);
-    };
     Product &longer = w.tiles() == 0 || (x.tiles() > 0 && x.k_tiles >= w.k_tiles) ? x : w;
     Product &other = &longer == &x ? w : x;
+    auto dealt = [&](int parts) {
+        const int l = unit_steps(longer.k_tiles, parts, n_pairs), u = static_cast<int>(longer.tiles() * parts);
+        const int lo = unit_steps(other.k_tiles, 1, n_pairs), uo = static_cast<int>(other.tiles());
+        const int pairs = std::max(1, std::min(kPairs, u + uo));
+        return &longer == &x ? deal(pairs, l, u, lo, uo) : deal(pairs, lo, uo, l, u);
+    };
     Deal best{};
     int best_parts = 0;
     for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 36, 72}) {
         if (parts > 1 && (longer.k_tiles < 4 * parts || longer.tiles() * parts > 2 * kPairs)) break;
-        const int64_t l = steps(longer, parts), u = longer.tiles() * parts;
-        const Deal d = &longer == &x ? deal(l, u, steps(other, 1), other.tiles()) : deal(steps(other, 1), other.tiles(), l, u);
+        const Deal d = dealt(parts);
         if (best_parts == 0 || d.steps < best.steps) {
             best = d;
             best_parts = parts;
@@ -1448,11 +1605,7 @@ Deal split_and_deal(Product &x, Product &w, int n_pairs) {
     w.part_tiles = w.k_tiles;
     longer.part_tiles = static_cast<int>(ce_div(longer.k_tiles, best_parts));
     longer.parts = static_cast<int>(ce_div(longer.k_tiles, std::max(1, longer.part_tiles)));
-    if (longer.parts != best_parts) {  // rounding left fewer parts
-        const int64_t l = steps(longer, longer.parts), u = longer.units();
-        best = &longer == &x ? deal(l, u, steps(other, 1), other.tiles()) : deal(steps(other, 1), other.tiles(), l, u);
-    }
-    return best;
+    return longer.parts == best_parts ? best : dealt(longer.parts);  // rounding may have left fewer parts
 }
 
 struct BackwardSpace {
@@ -1460,8 +1613,9 @@ struct BackwardSpace {
     int64_t dz_ld, dz_plane, acc_ld;
     int *status;
     unsigned *ticket, *grad_top, *found;
-    uint16_t *dz, *x, *w, *x_clean;
-    unsigned char *clean;
+    uint16_t *dz, *x, *w, *gathered;
+    int *n_counted;
+    int32_t *index, *counts;
     float *dx_acc, *dw_acc, *col_sums, *db_acc, *partial;
     BackwardSpace(Workspace &ws, const Shape &s, bool want_dx, bool want_dw, bool want_db) {
         choose_pieces(s, want_dx, want_dw);
@@ -1476,8 +1630,10 @@ struct BackwardSpace {
         dz = ws.take<uint16_t>(dz_plane * s.dz_planes);
         x = s.pack_x ? ws.take<uint16_t>(s.packed(s.n)) : nullptr;
         w = s.pack_w ? ws.take<uint16_t>(s.packed(s.vocab)) : nullptr;
-        x_clean = !s.pack_x && want_dw ? ws.take<uint16_t>(s.n * ce_div(s.dim, 8) * 8) : nullptr;
-        clean = !s.pack_x && want_dw ? ws.take<unsigned char>(ce_div(s.n, 64)) : nullptr;
+        gathered = s.pack_x ? nullptr : ws.take<uint16_t>(s.n * s.packed_ld);
+        n_counted = ws.take<int>(1);
+        index = ws.take<int32_t>(s.n);
+        counts = ws.take<int32_t>(ce_div(s.n, kTokenBlock));
         dx_acc = want_dx && !own_acc && cols < s.vocab ? ws.take<float>(s.n * acc_ld) : nullptr;
         dw_acc = want_dw && !own_acc && rows < s.n ? ws.take<float>(s.vocab * acc_ld) : nullptr;
         db_acc = want_db && rows < s.n ? ws.take<float>(s.vocab) : nullptr;
@@ -1492,8 +1648,8 @@ struct BackwardSpace {
                 Product px, pw;
                 products(s, want_dx, want_dw, r, c, &px, &pw);
                 split_and_deal(px, pw, s.product_pairs());
-                for (const Product &q : {px, pw})
-                    if (q.parts > 1) parts = std::max(parts, static_cast<int64_t>(q.parts) * q.m_tiles * kBM * acc_ld);
+                if (px.parts > 1) parts = std::max(parts, px.parts * rows * acc_ld);
+                if (pw.parts > 1) parts = std::max(parts, pw.parts * cols * acc_ld);
             }
         }
         col_sums = want_db ? ws.take<float>(sum_rows * cols) : nullptr;
@@ -1586,33 +1742,47 @@ struct Call {
     int reduction;
 };
 
+struct Tokens {  // the index and its length, on the device
+    int32_t *index, *counts;
+    int *n_counted;
+    uint16_t *gathered;
+};
+
 template <typename T>
-int pack_operand(const void *src, int64_t ld, int64_t rows, const Shape &s, uint16_t *dst, const Call &c, bool is_w, const unsigned *found,
+int pack_operand(const void *src, int64_t ld, int64_t rows, const Shape &s, uint16_t *dst, const Tokens &t, bool is_w, const unsigned *found,
                  cudaStream_t stream, Operand *out) {
     out->at = dst;
     out->ld = s.packed_ld;
     out->plane = align_up(rows * s.packed_ld, 64);
     const int64_t blocks = std::min<int64_t>(ce_div(rows * (s.packed_ld / 8), 256), 148 * 16);
     linear_ce_pack_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T *>(src), ld, rows, s.dim, dst, s.packed_ld,
-                                                                               out->plane, is_w ? nullptr : c.target, c.ignore_index, found, is_w);
+                                                                               out->plane, is_w ? nullptr : t.index, is_w ? nullptr : t.n_counted, found,
+                                                                               is_w);
     BPT_LAUNCH_CHECK();
     return BPT_OK;
 }
-// X and W as the tiles read them: where they lie, or packed.
+// The index of the tokens that count; X and W as the tiles read them: where they lie (X, where tokens are ignored: from
+// the copy), or packed.  loss: where ignored tokens' zeros go, or null; dx: the same for their rows of d x.
 template <typename T>
-int pack_operands(const Shape &s, const Call &c, uint16_t *x_to, uint16_t *w_to, unsigned *found, cudaStream_t stream, Operand *x, Operand *w) {
+int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x_to, uint16_t *w_to, unsigned *found, float *loss, void *dx,
+                     cudaStream_t stream, Operand *x, Operand *w) {
     *x = Operand{c.x, c.ldx, 0};
     *w = Operand{c.w, c.ldw, 0};
+    const unsigned blocks = static_cast<unsigned>(ce_div(s.n, kTokenBlock));
+    BPT_CUDA(launch_after(linear_ce_count_kernel, blocks, kTokenBlock, 0, stream, c.target, s.n, c.ignore_index, t.counts));
+    BPT_CUDA(launch_after(linear_ce_gather_kernel, dim3(blocks, 4), kTokenBlock, 0, stream, static_cast<const uint16_t *>(c.x), c.ldx, s.n, s.dim, c.target,
+                          c.ignore_index, t.counts, t.index, t.n_counted, t.gathered, s.packed_ld, static_cast<unsigned char *>(dx),
+                          static_cast<int64_t>(s.dim) * static_cast<int64_t>(sizeof(T)), loss));
     if constexpr (kIsFloat<T>) {
         BPT_CUDA(cudaMemsetAsync(found, 0, 4 * sizeof(unsigned), stream));
-        const int64_t blocks = std::min<int64_t>(ce_div(s.n + s.vocab, 8), 148 * 8);
-        linear_ce_spread_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const float *>(c.x), c.ldx, s.n,
+        const int64_t found_by = std::min<int64_t>(ce_div(s.n + s.vocab, 8), 148 * 8);
+        linear_ce_spread_kernel<<<static_cast<unsigned>(found_by), 256, 0, stream>>>(static_cast<const float *>(c.x), c.ldx, s.n,
                                                                                   static_cast<const float *>(c.w), c.ldw, s.vocab, s.dim,
                                                                                   c.target, c.ignore_index, found);
         BPT_LAUNCH_CHECK();
     }
-    if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, x_to, c, false, found, stream, x));
-    if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, w_to, c, true, found, stream, w));
+    if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, x_to, t, false, found, stream, x));
+    if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, w_to, t, true, found, stream, w));
     return BPT_OK;
 }
 
@@ -1644,11 +1814,13 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
         l.unit = 1.f;
     } else {
         Operand x, w;
-        BPT_TRY(pack_operands<T>(s, c, f.x, f.w, f.found, stream, &x, &w));
+        BPT_TRY(prepare_operands<T>(s, c, Tokens{f.index, f.counts, f.n_counted, f.gathered}, f.x, f.w, f.found, c.reduction == kReduceNone ? loss : nullptr,
+                                    nullptr, stream, &x, &w));
         Maps maps;
         BPT_TRY(make_map(&maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
         BPT_TRY(make_map(&maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));
         maps.c = maps.d = maps.e = maps.a;
+        if (f.gathered) BPT_TRY(make_map(&maps.d, kHalf, f.gathered, s.n, s.dim, s.packed_ld, 1, 0, kRows));
         Params p{};
         p.m_tiles = static_cast<int>(s.m_tiles());
         p.n_tiles = s.v_tiles();
@@ -1658,6 +1830,11 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
         p.dz_planes = s.dz_planes;
         p.status = f.status;
         p.split = f.found;
+        p.m_ext = static_cast<int>(s.n);
+        p.pieces = 1;
+        p.n_counted = f.n_counted;
+        p.index = f.index;
+        p.gathered = f.gathered != nullptr;
         p.n_rows = s.n;
         p.ignore_index = c.ignore_index;
         p.vocab = s.vocab;
@@ -1669,7 +1846,8 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
         p.starts = 1;
         p.smoothed = c.smoothing != 0.f;
         BPT_TRY((launch_ce<T, kStats>(maps, p, pairs, stream)));
-        l.rows_padded = s.m_tiles() * kBM;
+        l.n_counted = f.n_counted;
+        l.index = f.index;
         l.unit = kIsFloat<T> ? 1.f : kLn2;
     }
     l.partial = f.partial;
@@ -1677,7 +1855,6 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     l.target = c.target;
     l.n_rows = s.n;
     l.ignore_index = c.ignore_index;
-    l.m_tiles = static_cast<int>(s.m_tiles());
     l.n_tiles = s.v_tiles();
     l.pairs = pairs;
     l.vocab = s.vocab;
@@ -1702,13 +1879,7 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     constexpr bool kHalf = kIsHalf<T>;
     constexpr bool kFloat = std::is_same<T, float>::value;
     Operand x, w;
-    BPT_TRY(pack_operands<T>(s, c, f.x, f.w, f.found, stream, &x, &w));
-    const int64_t clean_ld = ce_div(s.dim, 8) * 8;
-    if (f.clean) {
-        linear_ce_clean_kernel<<<static_cast<unsigned>(ce_div(s.n, 64)), 256, 0, stream>>>(
-            static_cast<const uint16_t *>(c.x), c.ldx, s.n, s.dim, c.target, c.ignore_index, f.x_clean, clean_ld, f.clean);
-        BPT_LAUNCH_CHECK();
-    }
+    BPT_TRY(prepare_operands<T>(s, c, Tokens{f.index, f.counts, f.n_counted, f.gathered}, f.x, f.w, f.found, nullptr, dx, stream, &x, &w));
     if (c.reduction == kReduceNone) {
         BPT_CUDA(cudaMemsetAsync(f.grad_top, 0, sizeof(unsigned), stream));
         linear_ce_top_kernel<<<static_cast<unsigned>(std::min<int64_t>(ce_div(s.n, 256), 148)), 256, 0, stream>>>(grad, c.target, s.n,
@@ -1719,10 +1890,11 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     BPT_TRY(make_map(&grad_maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
     BPT_TRY(make_map(&grad_maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));
     grad_maps.d = grad_maps.e = grad_maps.a;
+    if (f.gathered) BPT_TRY(make_map(&grad_maps.d, kHalf, f.gathered, s.n, s.dim, s.packed_ld, 1, 0, kRows));
     BPT_TRY(make_map(&maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, 64));
     BPT_TRY(make_map(&maps.d, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, 64));
     maps.e = maps.d;
-    if (f.clean) BPT_TRY(make_map(&maps.e, kHalf, f.x_clean, s.n, s.dim, clean_ld, 1, 0, 64));
+    if (f.gathered) BPT_TRY(make_map(&maps.e, kHalf, f.gathered, s.n, s.dim, s.packed_ld, 1, 0, 64));
     Params p{};
     p.n_pairs = s.logit_pairs();
     p.dz_planes = s.dz_planes;
@@ -1743,7 +1915,10 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     p.reduction = c.reduction;
     p.col_sums = f.col_sums;
     p.col_ld = f.cols;
-    p.clean = f.clean;
+    p.n_counted = f.n_counted;
+    p.index = f.index;
+    p.gathered = f.gathered != nullptr;
+    p.pieces = static_cast<int>(ce_div(s.n, f.rows));
     const bool own_acc = kFloat && s.dim == f.acc_ld;
     for (int64_t n0 = 0; n0 < s.n; n0 += f.rows) {
         const int64_t rows = std::min(f.rows, s.n - n0);
@@ -1751,6 +1926,7 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
         for (int64_t v0 = 0; v0 < s.vocab; v0 += f.cols) {
             const int64_t cols = std::min<int64_t>(f.cols, s.vocab - v0);
             const bool last_cols = v0 + f.cols >= s.vocab;
+            p.piece = static_cast<int>(n0 / f.rows);
             Params g = p;
             g.m_tiles = static_cast<int>(ce_div(rows, kBM));
             g.n_tiles = static_cast<int>(ce_div(cols, kBN));
@@ -1760,7 +1936,7 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             g.a0 = static_cast<int>(n0);
             g.starts = n0 == 0 && v0 == 0;
             g.b0 = static_cast<int>(v0);
-            BPT_TRY(make_map(&grad_maps.c, kHalf, f.dz, rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, 32, s.dz_planes == 1 ? 64 : 32));
+            BPT_TRY(make_map(&grad_maps.c, kHalf, f.dz, f.rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, 32, s.dz_planes == 1 ? 64 : 32));
             const int pairs = pairs_for(static_cast<int64_t>(g.m_tiles) * g.n_tiles);
             BPT_TRY((launch_ce<T, kGrad>(grad_maps, g, pairs, stream)));
             if (db) {
@@ -1768,9 +1944,11 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
                                       f.db_acc ? f.db_acc + v0 : nullptr, n0 > 0, last_rows, static_cast<T *>(db) + v0));
             }
             if (!dx && !dw) continue;
-            BPT_TRY(make_map(&maps.a, kHalf, f.dz, rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, kRows));
-            BPT_TRY(make_map(&maps.c, kHalf, f.dz, rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, 64));
+            BPT_TRY(make_map(&maps.a, kHalf, f.dz, f.rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, kRows));
+            BPT_TRY(make_map(&maps.c, kHalf, f.dz, f.rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, 64));
             Params q = p;
+            q.a0 = static_cast<int>(n0);
+            q.m_ext = static_cast<int>(rows);
             BackwardSpace::products(s, dx, dw, rows, cols, &q.product[0], &q.product[1]);
             Product &px = q.product[0], &pw = q.product[1];
             const Deal d = split_and_deal(px, pw, s.product_pairs());
@@ -1779,14 +1957,13 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             q.busy = d.busy;
             q.after_busy = d.after_busy;
             q.after = d.after;
-            px.b0 = static_cast<int>(v0);
-            px.row_offset = n0;
-            px.row_end = n0 + rows;
+            q.b0 = static_cast<int>(v0);
+            px.partial_plane = f.rows * f.acc_ld;
+            pw.partial_plane = f.cols * f.acc_ld;
             px.acc = own_acc ? static_cast<float *>(dx) : f.dx_acc;
             px.add = v0 > 0;
             px.last = last_cols;
             px.out = dx;
-            pw.b0 = static_cast<int>(n0);
             pw.row_offset = v0;
             pw.row_end = v0 + cols;
             pw.acc = own_acc ? static_cast<float *>(dw) : f.dw_acc;
@@ -1799,7 +1976,7 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             for (int which = 0; which < 2; ++which) {
                 const Product &r = q.product[which];
                 if (r.parts <= 1) continue;
-                const int64_t blocks = std::min<int64_t>(ce_div((r.row_end - r.row_offset) * (r.acc_ld / 4), 256), 148 * 8);
+                const int64_t blocks = std::min<int64_t>(ce_div((which == 0 ? f.rows : cols) * (r.acc_ld / 4), 256), 148 * 8);
                 BPT_CUDA(launch_after(linear_ce_parts_kernel<T>, static_cast<unsigned>(blocks), 256, 0, stream, q, which));
             }
         }
