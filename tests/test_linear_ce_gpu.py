@@ -122,8 +122,15 @@ def test_values_and_gradients(shape, dtype):
 @pytest.mark.parametrize("shape", [(2100, 20000, 64), (20000, 2100, 64), (34000, 4000, 32), (12000, 12000, 40), (6000, 40000, 32),
                                    (40000, 6000, 32), (20, 300000, 16), (300000, 20, 16)])
 def test_pieces(shape, dtype):
-    """More cells than are kept at a time: the vocabulary is cut, the tokens are, and both."""
+    """More cells than are kept at a time: the vocabulary is cut, the tokens are, and both; few, many and all but a few of
+    the tokens ignored, so that a piece has fewer tokens than it was planned for, or none."""
     check(*inputs(*shape, dtype, padded=0.1), smoothing=0.1)
+    if shape[0] * shape[1] > 1.4e8:
+        x, w, b, t = inputs(*shape, dtype, padded=0.7)
+        check(x, w, b, t)
+        t[3:-2] = IGNORE
+        t[0] = t[-1] = 1
+        check(x, w, b, t, reduction="sum")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
