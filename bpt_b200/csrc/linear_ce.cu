@@ -42,7 +42,7 @@ namespace {
 
 using namespace tc5;
 
-constexpr int kBM = 256, kBN = 256, kBK = 64;  // a pair's tile; each block has 128 of the rows
+constexpr int kBM = 256, kBN = 256, kBK = 64, kStages = 6;  // a pair's tile; each block has 128 of the rows
 constexpr int kRows = kBM / 2, kCols = kBN / 2;               // what a block loads of A and of B
 constexpr int kABytes = kRows * kBK * 2, kBBytes = kCols * kBK * 2, kStageBytes = kABytes + kBBytes;
 constexpr int kChunkBytes = 64 * 128;  // an MN-major tile: 64 rows along K of 64 elements
@@ -55,13 +55,12 @@ constexpr int kPairs = 74;             // pairs of blocks at most: one block per
 constexpr int kRunTiles = 8;           // fp32: K blocks added up by the tensor core before the sum is taken out
 
 enum Kind { kStats, kGrad, kProducts };
-// Shared memory: the bias of two tiles, barriers; from the next 1024-byte boundary on operand stages, and for grad two
-// tiles of 32 rows x 64 columns of dZ per finishing warp, on their way out (one stage less for them).
+// Shared memory: the bias of two tiles, barriers; from the next 1024-byte boundary on operand stages, and for grad a tile
+// of 32 rows x 64 columns of dZ per finishing warp, on its way out.
 constexpr int kOutBytes = 32 * 128;
-constexpr int stages(int kind) { return kind == kGrad ? 5 : 6; }
-constexpr int out_bytes(int kind) { return kind == kGrad ? 2 * kFinishWarps * kOutBytes : 0; }
+constexpr int out_bytes(int kind) { return kind == kGrad ? kFinishWarps * kOutBytes : 0; }
 constexpr int kHeadBytes = 3072;
-constexpr int smem_bytes(int kind) { return kHeadBytes + stages(kind) * kStageBytes + out_bytes(kind); }
+constexpr int smem_bytes(int kind) { return kHeadBytes + kStages * kStageBytes + out_bytes(kind); }
 static_assert(smem_bytes(kGrad) <= 227 * 1024 && smem_bytes(kStats) <= 227 * 1024, "a block's shared memory");
 enum { kReduceNone = 0, kReduceMean = 1, kReduceSum = 2 };
 
@@ -104,6 +103,10 @@ struct Params {
     int reduction;
     float *col_sums;                       // grad: column sums of dZ, 8 rows a piece (a warp's rows each), or null
     int64_t col_ld;
+    int grad_pairs, grad_n_tiles, grad_n_ext;  // products: the grad launch that left them
+    float *db_acc;                         // products: sums of earlier pieces
+    int db_add, db_last;
+    void *db;                              // of this piece, or null
     const float *count;
     const unsigned *grad_top;              // none: bits of max |g|
     // products: 0 = d x, 1 = d w.  The one with the longer units goes first, dealt in turn; pairs below `busy` have one
@@ -426,6 +429,34 @@ __device__ __forceinline__ PieceRows piece_rows(const Params &p) {
     return r;
 }
 
+// d b of a piece, by two warps of each products block that have nothing else to do, 32 columns at a time: the column sums
+// that the pairs of the grad launch (fp32: the token blocks) left, added to those of earlier rows; the last are scaled
+// and stored.
+template <typename T> __device__ __forceinline__ void finish_bias(const Params &p, int rows_here, int warp, int warps, int lane) {
+    const float scale = result_scale<T>(p, 2);
+    const int64_t m_tiles = (rows_here + kBM - 1) / kBM, total = m_tiles * p.grad_n_tiles;
+    const int pairs = pairs_used(p.grad_pairs, total);
+    for (int c0 = warp * 32; c0 < p.grad_n_ext; c0 += warps * 32) {
+        const int c = c0 + lane, n = c0 / kBN;
+        int pieces = static_cast<int>(m_tiles);
+        if (!kIsFloat<T> && m_tiles) pieces = pair_of_tile(total, pairs, (n + 1) * m_tiles - 1) - pair_of_tile(total, pairs, n * m_tiles) + 1;
+        if (c >= p.grad_n_ext) continue;
+        const float *from = p.col_sums + c;
+        float s[8];  // the eight rows of every piece
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = 0.f;
+#pragma unroll 2
+        for (int r = 0; r < pieces; ++r) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += __ldcg(from + (static_cast<int64_t>(r) * 8 + i) * p.col_ld);
+        }
+        float all = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+        if (p.db_add) all += p.db_acc[c];
+        if (!p.db_last) p.db_acc[c] = all;
+        else static_cast<T *>(p.db)[c] = from_acc<T>(all * scale);
+    }
+}
+
 // map_a, map_b: stats, grad: X and W rows; products: dZ rows and W columns.  map_c: dZ, as it is stored (grad), its columns
 // (products).  map_d, map_e: stats, grad: the copy of X, rows; products: X columns, those of its copy.
 template <typename T, int kKind>
@@ -433,7 +464,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
                  const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_e, const __grid_constant__ Params p) {
     constexpr bool kPrecise = std::is_same<T, float>::value;
-    constexpr int kStages = stages(kKind);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     float *s_bias = reinterpret_cast<float *>(smem_raw);  // [2][256]
     // full (block 0's is used) and empty per stage, sums ready and sums read (block 0's) per accumulator
@@ -604,6 +634,8 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 while (!mbar_try(bar_drain, 0u) && clock64() - start < kWaitCycles) {}
             }
         }
+    } else if (kKind == kProducts && p.db) {
+        finish_bias<T>(p, rows_here, static_cast<int>(blockIdx.x) * 2 + warp - (kFinishWarps + 2), static_cast<int>(gridDim.x) * 2, lane);
     }
     } else {  // ---- finishing: warp % 4 names the 32 of this block's rows, warp / 4 the half of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kFinishRegs));
@@ -623,8 +655,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         // grad, 16-bit: column sums over the pair's token blocks of one vocabulary block
         constexpr bool kKeepSums = kKind == kGrad && !kPrecise;
-        const uint32_t out_tile = base + kStages * kStageBytes + warp * 2 * kOutBytes;
-        int out_at = 0;
+        const uint32_t out_tile = base + kStages * kStageBytes + warp * kOutBytes;
         float col_sum[kKeepSums ? 4 : 1][32];
         if constexpr (kKeepSums) {
 #pragma unroll
@@ -812,12 +843,11 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                 tma_store(&map_c, x, y, plane, tile);
                                 store_commit();
                             }
-                            out_at ^= 1;
                         };
-                        auto next_tile = [&] {  // the other one may still be on its way
-                            if (lane == 0) store_wait_read<1>();
+                        auto next_tile = [&] {  // what it held has left
+                            if (lane == 0) store_wait_read<0>();
                             __syncwarp();
-                            return out_tile + out_at * kOutBytes;
+                            return out_tile;
                         };
                         const uint32_t narrow = lane * 64, turn = lane >> 1 & 3;  // a row of a 64-byte-swizzled tile
                         if constexpr (kPrecise) {
@@ -839,7 +869,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             }
                         } else if (p.dz_planes == 1) {
                             const int at = (c0 >> 5) & 1;  // which half of the tile's 64 columns
-                            const uint32_t tile = at == 0 ? next_tile() : out_tile + out_at * kOutBytes;
+                            const uint32_t tile = at == 0 ? next_tile() : out_tile;
 #pragma unroll
                             for (int u = 0; u < 4; ++u)
                                 st_shared_v4(tile + swz(lane, at * 4 + u), pack2<T>(v[8 * u], v[8 * u + 1]), pack2<T>(v[8 * u + 2], v[8 * u + 3]),
@@ -1470,33 +1500,6 @@ __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_const
     }
 }
 
-// d b of a piece: the column sums that the pairs (or, each_m, the token blocks) left, added to those of earlier rows;
-// the last one is scaled and stored.
-template <typename T>
-__global__ void __launch_bounds__(256) linear_ce_bias_kernel(const __grid_constant__ Params p, int pairs, int each_m, float *acc, int add,
-                                                             int last, T *__restrict__ out) {
-    let_next_start();
-    wait_for_previous();
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
-    __shared__ float s_part[8][32];
-    const int64_t m_tiles = (piece_rows(p).rows + kBM - 1) / kBM, total = m_tiles * p.n_tiles, n = blockIdx.x * 32 / kBN;
-    int pieces = static_cast<int>(m_tiles);
-    pairs = pairs_used(pairs, total);
-    if (!each_m && m_tiles) pieces = pair_of_tile(total, pairs, (n + 1) * m_tiles - 1) - pair_of_tile(total, pairs, n * m_tiles) + 1;
-    float s = 0.f;
-    if (c < p.n_ext)
-        for (int r = part; r < pieces * 8; r += 8) s += p.col_sums[r * p.col_ld + c];
-    s_part[part][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (part > 0 || c >= p.n_ext) return;
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += s_part[i][threadIdx.x];
-    if (add) s += acc[c];
-    if (!last) acc[c] = s;
-    else out[c] = *p.status ? from_acc<T>(__int_as_float(0x7fffffff)) : from_acc<T>(s * result_scale<T>(p, 2));
-}
-
 // ---- host side
 struct Operand {  // a matrix as TMA reads it
     const void *at;
@@ -1939,11 +1942,6 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             BPT_TRY(make_map(&grad_maps.c, kHalf, f.dz, f.rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, 32, s.dz_planes == 1 ? 64 : 32));
             const int pairs = pairs_for(static_cast<int64_t>(g.m_tiles) * g.n_tiles);
             BPT_TRY((launch_ce<T, kGrad>(grad_maps, g, pairs, stream)));
-            if (db) {
-                BPT_CUDA(launch_after(linear_ce_bias_kernel<T>, static_cast<unsigned>(ce_div(cols, 32)), 256, 0, stream, g, pairs, kFloat,
-                                      f.db_acc ? f.db_acc + v0 : nullptr, n0 > 0, last_rows, static_cast<T *>(db) + v0));
-            }
-            if (!dx && !dw) continue;
             BPT_TRY(make_map(&maps.a, kHalf, f.dz, f.rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, kRows));
             BPT_TRY(make_map(&maps.c, kHalf, f.dz, f.rows, cols, f.dz_ld, s.dz_planes, f.dz_plane, 64));
             Params q = p;
@@ -1971,8 +1969,16 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             pw.last = last_rows;
             pw.out = dw;
             px.acc_ld = pw.acc_ld = f.acc_ld;
+            q.grad_pairs = pairs;
+            q.grad_n_tiles = g.n_tiles;
+            q.grad_n_ext = g.n_ext;
+            q.db = db ? static_cast<T *>(db) + v0 : nullptr;
+            q.db_acc = f.db_acc ? f.db_acc + v0 : nullptr;
+            q.db_add = n0 > 0;
+            q.db_last = last_rows;
             px.partial = pw.partial = f.partial;  // at most one of them has parts
-            BPT_TRY((launch_ce<T, kProducts>(maps, q, d.pairs, stream)));
+            // d b is shared by the blocks of all pairs, also where there are fewer units than pairs
+            BPT_TRY((launch_ce<T, kProducts>(maps, q, db ? kPairs : d.pairs, stream)));
             for (int which = 0; which < 2; ++which) {
                 const Product &r = q.product[which];
                 if (r.parts <= 1) continue;
