@@ -504,10 +504,9 @@ template <typename F> int ln_dispatch(const LnLayout &l, int dim, F f) {
                   : f(std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
 }
 
-// Blocks of a kernel that run at once; its shared memory is allowed on the way.
+// Blocks of a kernel that run at once.
 template <typename K> int ln_resident(K kernel, int block, size_t smem) {
     int per_sm = 1;
-    if (smem > (40 << 10)) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
     return per_sm * 148;
 }
@@ -529,6 +528,8 @@ int launch_layer_norm(const void *x, const void *r, const void *gamma, const voi
             constexpr int kPiece = vec.value * sizeof(T), kAhead = kPiece >= 16 ? 2 : 0;
             using R = Rows<T, vec.value, vecs.value, has_r.value ? 2 : 1, block.value, kAhead>;
             auto kernel = layer_norm_kernel<T, vec.value, vecs.value, has_r.value, block.value, kAhead>;
+            static tc5::OncePerDevice allowed;
+            BPT_CUDA(tc5::allow_smem(allowed, kernel, R::kSmem));
             static const int resident = ln_resident(kernel, block.value, R::kSmem);  // one wave of persistent blocks
             kernel<<<static_cast<unsigned>(std::min<int64_t>(blocks, resident)), block.value, R::kSmem, stream>>>(
                 static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(gamma), static_cast<const T *>(beta), eps,
@@ -558,7 +559,8 @@ int launch_layer_norm_backward(const void *gy, const void *x, const void *r, con
                                          : layer_norm_backward_kernel<T, vec.value, vecs.value, has_r.value, 512, kAhead>;
             const size_t sums = sizeof(float) * static_cast<size_t>(l.block / l.tpr) * dim;  // at most 512 * 16 floats
             const size_t smem = std::max<size_t>(kAhead * kRow * (l.block / 256), partial ? sums : 0);
-            if (smem > (40 << 10)) BPT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10));
+            static tc5::OncePerDevice allowed[2];
+            BPT_CUDA(tc5::allow_smem(allowed[l.block == 512], kernel, std::max<size_t>(kAhead * kRow * (l.block / 256), 32 << 10)));
             kernel<<<grid, l.block, smem, stream>>>(static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const T *>(r),
                                                     static_cast<const T *>(gamma), mean, rstd, static_cast<T *>(da), partial, n_rows, dim, l.tpr);
             BPT_LAUNCH_CHECK();

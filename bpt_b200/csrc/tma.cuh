@@ -3,6 +3,8 @@
 
 #include <cuda.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "tc5.cuh"
 
@@ -135,6 +137,19 @@ template <int n> __device__ __forceinline__ void store_wait_read() { asm volatil
 __device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Allows a kernel its dynamic shared memory, once per device (two threads that meet here do it twice).
+struct OncePerDevice {
+    std::atomic<uint64_t> done{0};
+};
+template <typename K> inline cudaError_t allow_smem(OncePerDevice &once, K kernel, size_t bytes) {
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess || (device < 64 && (once.done.load(std::memory_order_relaxed) >> device & 1))) return err;
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (err == cudaSuccess && device < 64) once.done.fetch_or(uint64_t(1) << device);
+    return err;
 }
 
 // Programmatic dependent launch: a kernel launched by launch_after may start when the one before it in the stream says so

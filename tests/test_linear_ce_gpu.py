@@ -133,6 +133,16 @@ def test_pieces(shape, dtype):
         check(x, w, b, t, reduction="sum")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_millions_of_tokens(dtype, reduction):
+    """More than the blocks that list the tokens have at 256 each: they go through theirs in turns."""
+    n = 2 * 1048576 + 77
+    x, w, b, t = inputs(n, 5, 8, dtype, padded=0.3, seed=11)
+    grad = torch.linspace(0.5, 1.5, n, device="cuda") if reduction == "none" else None
+    check(x, w, b, t, reduction=reduction, grad=grad)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_bitwise_reproducible(dtype):
     args = inputs(3001, 12345, 128, dtype, padded=0.2)
