@@ -65,7 +65,7 @@ enum { kReduceNone = 0, kReduceMean = 1, kReduceSum = 2 };
 
 // One of the two products of a piece.  A unit of work is a tile and a part of its K.
 struct Product {
-    int m_tiles, n_tiles, k_tiles, n_ext;
+    int m_tiles, n_tiles, k_tiles, n_ext, width;  // width: columns of a tile, the same for all but the last
     int parts;                             // K parts of a tile (their sums go to `partial` if parts > 1)
     int64_t row_offset, row_end;           // d w: rows of the output are row_offset + tile row, below row_end
     float *acc;                            // fp32 sums of earlier pieces (leading dimension acc_ld), or null
@@ -80,7 +80,7 @@ struct Product {
 struct Params {
     int n_tiles, k_tiles, n_ext;           // stats, grad: tiles; columns in all (the last tile may be narrower)
     int m_ext, piece, pieces;              // tokens of the piece, if all count (the first is a0); which of how many it is
-    int n_pairs;                           // plane products: 1 or 2; fp32: 3 or 6, as `split` says
+    int a_planes;                          // 16-bit products: of dZ, as A, 1 or 2
     const unsigned *split;                 // fp32: see Split
     int dz_planes;                         // grad: planes of dZ that are written
     int a0, b0;                            // added to the row coordinate of A and of B
@@ -114,10 +114,7 @@ struct Params {
     int first, busy, after_busy, after;
 };
 
-// Plane products, smallest first.  All six: three bf16 planes by three; the last three: two fp16 planes by two; the last
-// two: dZ in two planes by a 16-bit operand; the last: 16-bit.
 constexpr float kLowScale = 2048.f;  // of the second of two fp16 planes
-__constant__ const int kPairA[6] = {2, 0, 1, 0, 1, 0}, kPairB[6] = {0, 2, 1, 1, 0, 0};
 
 template <typename T> constexpr bool kIsHalf = std::is_same<T, __half>::value;
 template <typename T> constexpr bool kIsFloat = std::is_same<T, float>::value;
@@ -282,8 +279,8 @@ __host__ __device__ inline Deal deal(int pairs, int l0, int u0, int l1, int u1) 
 // A unit's fixed cost, and that of its sums through memory where a tile has several parts, in K blocks of one product
 // (0.3 us): measured.
 constexpr int64_t kUnitSteps = 4, kPartSteps = 20;
-__host__ __device__ inline int unit_steps(int k_tiles, int parts, int n_pairs) {
-    return (k_tiles + parts - 1) / parts * n_pairs + kUnitSteps + (parts > 1 ? kPartSteps : 0);
+__host__ __device__ inline int unit_steps(int k_tiles, int parts, int stages) {
+    return (k_tiles + parts - 1) / parts * stages + kUnitSteps + (parts > 1 ? kPartSteps : 0);
 }
 // The work of a pair, in the order in which all its warps take it: a tile, the K blocks of it, and for the products
 // which product and part.
@@ -293,7 +290,7 @@ template <int kKind> struct Work {
     int pair, pairs, stage;       // products
     int m_tiles;                  // stats, grad: with the tokens that count
     int x_units, w_units, x_k, w_k, first, busy, after_busy, after;
-    int cur_tiles, cur_n, cur_k, cur_part;  // of the product that is being worked on
+    int cur_tiles, cur_n, cur_width, cur_k, cur_part;  // of the product that is being worked on
     int m, n, k0, k1, which, part;
     // rows: tokens of the piece that count
     __device__ Work(const Params &p_, int rows) : p(p_) {
@@ -321,8 +318,8 @@ template <int kKind> struct Work {
         }
     }
     // products: where fewer tokens count, they are dealt again (by one thread for its block)
-    __device__ Deal deal_again(int n_pairs) const {
-        return deal(pairs, unit_steps(x_k, p.product[0].parts, n_pairs), x_units, unit_steps(w_k, p.product[1].parts, n_pairs), w_units);
+    __device__ Deal deal_again(int stages) const {
+        return deal(pairs, unit_steps(x_k, p.product[0].parts, stages), x_units, unit_steps(w_k, p.product[1].parts, stages), w_units);
     }
     __device__ void start() {
         if constexpr (kKind == kProducts) {
@@ -336,6 +333,7 @@ template <int kKind> struct Work {
         which = product;
         const Product &q = p.product[product];
         cur_n = q.n_tiles;
+        cur_width = q.width;
         cur_k = product == 0 ? x_k : w_k;
         cur_tiles = (product == 0 ? x_units : w_units) / q.parts;
         cur_part = (cur_k + q.parts - 1) / q.parts;
@@ -372,8 +370,10 @@ template <int kKind> struct Work {
     }
     __device__ int64_t tiles() const { return static_cast<int64_t>(m_tiles) * p.n_tiles; }  // stats, grad
     __device__ int n_ext() const { return kKind == kProducts ? p.product[which].n_ext : p.n_ext; }
+    __device__ int n0() const { return n * (kKind == kProducts ? cur_width : kBN); }  // the tile's first column
+    __device__ int cols() const { return min(kKind == kProducts ? cur_width : kBN, n_ext() - n0()); }
     // columns of the product instruction: whole 32s, half of them from each block's B
-    __device__ int width() const { return (min(kBN, n_ext() - n * kBN) + 31) / 32 * 32; }
+    __device__ int width() const { return (cols() + 31) / 32 * 32; }
 };
 
 // Barrier of the finishing warps that also says whether any of their threads gave up.
@@ -509,16 +509,14 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     Work<kKind> work(p, rows_here);
     Split split;
     if constexpr (kPrecise) split = read_split(p.split);
-    const int first_pair = 6 - (kPrecise ? (split.half ? 3 : 6) : p.n_pairs);
-    // sums that share an accumulator: all plane products, but of two fp16 planes the two small ones (both times kLowScale)
-    // and the large one
-    const int groups = kPrecise && split.half ? 2 : 1;
-    auto group_pairs = [&](int group) { return groups == 1 ? 6 - first_pair : group == 0 ? 2 : 1; };
+    // Stages of a K block.  fp32: one for each plane of A and of B, which all products of planes share.  16-bit: one, or one
+    // for each plane of dZ with its own copy of B (first the second planes' product, whose terms are the smaller ones).
+    const int planes = kPrecise ? (split.half ? 2 : 3) : kKind == kProducts ? p.a_planes : 1;
     if constexpr (kKind == kProducts) {
         if (some_ignored) {
             int *const s_deal = reinterpret_cast<int *>(smem_raw);  // the bias' place, which products have no use for
             if (tid == 0) {
-                const Deal d = work.deal_again(6 - first_pair);
+                const Deal d = work.deal_again(planes);
                 s_deal[0] = d.first;
                 s_deal[1] = d.busy;
                 s_deal[2] = d.after_busy;
@@ -541,42 +539,50 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 bool ok = true;
                 while (ok && work.next()) {
                     const int m0 = work.m * kBM + static_cast<int>(rank) * kRows, half = work.width() / 2;
-                    const int n0 = work.n * kBN + static_cast<int>(rank) * half, chunks = (half + 63) / 64;
+                    const int n0 = work.n0() + static_cast<int>(rank) * half, chunks = (half + 63) / 64;
                     const int run = kPrecise ? kRunTiles : work.k1;
                     for (int kr = work.k0; ok && kr < work.k1; kr += run) {
-                        for (int pair = first_pair; ok && pair < 6; ++pair) {
-                            const int pa = kPairA[pair], pb = kPairB[pair];
-                            for (int k = kr; k < min(kr + run, work.k1); ++k) {
-                                ok = mbar_wait_or_stop(bar_empty + 8 * s, phase ^ 1u, stop);
-                                if (!ok) break;
-                                const uint32_t a = base + s * kStageBytes, b = a + kABytes, full = map_to(bar_full + 8 * s, 0);
-                                const int b_bytes = kKind == kProducts ? chunks * kChunkBytes : kBBytes;
-                                if (rank == 0) mbar_expect(bar_full + 8 * s, 2 * (kABytes + b_bytes));
-                                if constexpr (kKind == kProducts) {
-                                    const int b_row = (work.which == 0 ? p.b0 : a0) + k * kBK;
-                                    if (work.which == 0) {
-                                        tma_load_pair(a, &map_a, k * kBK, m0, pa, full);
-                                        for (int c = 0; c < chunks; ++c) tma_load_pair(b + c * kChunkBytes, &map_b, n0 + 64 * c, b_row, pb, full);
-                                    } else {
-                                        tma_load_pair(a, &map_c, m0, k * kBK, pa, full);
-                                        tma_load_pair(a + kChunkBytes, &map_c, m0 + 64, k * kBK, pa, full);
-                                        for (int c = 0; c < chunks; ++c)
-                                            tma_load_pair(b + c * kChunkBytes, copied ? &map_e : &map_d, n0 + 64 * c, b_row, pb, full);
-                                    }
+                        const int k_end = min(kr + run, work.k1);
+                        int k = kr, plane = kPrecise ? 0 : planes - 1;
+                        while (true) {
+                            ok = mbar_wait_or_stop(bar_empty + 8 * s, phase ^ 1u, stop);
+                            if (!ok) break;
+                            const uint32_t a = base + s * kStageBytes, b = a + kABytes, full = map_to(bar_full + 8 * s, 0);
+                            const int b_bytes = kKind == kProducts ? chunks * kChunkBytes : kBBytes, b_plane = kPrecise ? plane : 0;
+                            if (rank == 0) mbar_expect(bar_full + 8 * s, 2 * (kABytes + b_bytes));
+                            if constexpr (kKind == kProducts) {
+                                const int b_row = (work.which == 0 ? p.b0 : a0) + k * kBK;
+                                if (work.which == 0) {
+                                    tma_load_pair(a, &map_a, k * kBK, m0, plane, full);
+                                    for (int c = 0; c < chunks; ++c) tma_load_pair(b + c * kChunkBytes, &map_b, n0 + 64 * c, b_row, b_plane, full);
                                 } else {
-                                    tma_load_pair(a, copied ? &map_d : &map_a, k * kBK, a0 + m0, pa, full);
-                                    tma_load_pair(b, &map_b, k * kBK, p.b0 + n0, pb, full);
+                                    tma_load_pair(a, &map_c, m0, k * kBK, plane, full);
+                                    tma_load_pair(a + kChunkBytes, &map_c, m0 + 64, k * kBK, plane, full);
+                                    for (int c = 0; c < chunks; ++c)
+                                        tma_load_pair(b + c * kChunkBytes, copied ? &map_e : &map_d, n0 + 64 * c, b_row, b_plane, full);
                                 }
-                                ++issued;
-                                if (++s == kStages) {
-                                    s = 0;
-                                    phase ^= 1u;
+                            } else {
+                                tma_load_pair(a, copied ? &map_d : &map_a, k * kBK, a0 + m0, plane, full);
+                                tma_load_pair(b, &map_b, k * kBK, p.b0 + n0, b_plane, full);
+                            }
+                            ++issued;
+                            if (++s == kStages) {
+                                s = 0;
+                                phase ^= 1u;
+                            }
+                            if constexpr (kPrecise) {
+                                if (++plane == planes) {
+                                    plane = 0;
+                                    if (++k == k_end) break;
                                 }
+                            } else if (++k == k_end) {
+                                k = kr;
+                                if (plane-- == 0) break;
                             }
                         }
                     }
                 }
-                if (!ok) {  // the last loads of every stage land before the block ends (block 0's barriers know)
+            if (!ok) {  // the last loads of every stage land before the block ends (block 0's barriers know)
                     for (uint32_t i = 0; i < kStages && i < issued; ++i) {
                         const uint32_t load = issued - 1 - i, bar = bar_full + 8 * (load % kStages);
                         const long long start = clock64();
@@ -592,27 +598,53 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 while (ok && work.next()) {
                     const bool a_mn = kKind == kProducts && work.which == 1, b_mn = kKind == kProducts;
                     const uint32_t instr = ce_instr(kPrecise ? split.half : kIsHalf<T>, work.width(), a_mn, b_mn);
+                    // descriptors (addresses in them count 16 bytes) of the first stage, made once a tile: one thread issues all
+                    const uint64_t a_desc = a_mn ? desc_mnmajor(base, 0) : desc_kmajor(base, 0);
+                    const uint64_t b_desc = b_mn ? desc_mnmajor(base + kABytes, 0) : desc_kmajor(base + kABytes, 0);
+                    const uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+                    constexpr uint32_t kStageStep = kStageBytes / 16;
                     const int run = kPrecise ? kRunTiles : work.k1;
                     for (int kr = work.k0; ok && kr < work.k1; kr += run) {
                         const int k_tiles = min(kr + run, work.k1) - kr;
-                        for (int group = 0; ok && group < groups; ++group) {
-                            const uint32_t d = tmem + buf * kBN;
-                            ok = mbar_wait_or_stop(bar_read + 8 * buf, read_phase ^ 1u, stop);
+                        auto multiply = [&](uint32_t d, int a, int b, uint32_t accumulate) {  // of A in stage a, B in stage b
+#pragma unroll
+                            for (int ks = 0; ks < kBK / 16; ++ks)
+                                mma_pair(d, a_desc + a * kStageStep + ks * a_step, b_desc + b * kStageStep + ks * b_step, instr, ks > 0 ? 1u : accumulate);
+                        };
+                        ok = mbar_wait_or_stop(bar_read + 8 * buf, read_phase ^ 1u, stop);
+                        if (!ok) break;
+                        fence_after_sync();
+                        if constexpr (kPrecise) {
+                            for (int k = 0; ok && k < k_tiles; ++k) {  // a K block's stages are neighbours: planes divides kStages
+                                for (int q = 0; q < planes; ++q) {     // with plane q come the products of it and those before
+                                    ok = mbar_wait_or_stop(bar_full + 8 * (s + q), phase, stop);
+                                    if (!ok) break;
+                                    fence_after_sync();
+                                    for (int i = 0; i <= q; ++i) {
+                                        for (int j = i < q ? q : 0; j <= q && i + j < planes; ++j) {
+                                            const bool low = i + j > 0;
+                                            multiply(tmem + (low ? 0 : kBN), s + i, s + j,
+                                                     k > 0 || (low && !(q == 1 && i == 0)) ? 1u : 0u);
+                                        }
+                                    }
+                                }
+                                if (!ok) break;
+                                for (int q = 0; q < planes; ++q) mma_commit_pair(bar_empty + 8 * (s + q));
+                                s += planes;
+                                if (s == kStages) {
+                                    s = 0;
+                                    phase ^= 1u;
+                                }
+                            }
                             if (!ok) break;
-                            fence_after_sync();
-                            uint32_t accumulate = 0;
-                            const int steps = group_pairs(group) * k_tiles;
-                            for (int step = 0; step < steps; ++step) {
+                            mma_commit_pair(bar_ready);
+                            read_phase ^= 1u;
+                        } else {
+                            for (int step = 0; step < planes * k_tiles; ++step) {
                                 ok = mbar_wait_or_stop(bar_full + 8 * s, phase, stop);
                                 if (!ok) break;
                                 fence_after_sync();
-                                const uint32_t a = base + s * kStageBytes, b = a + kABytes;
-#pragma unroll
-                                for (int ks = 0; ks < kBK / 16; ++ks) {
-                                    mma_pair(d, a_mn ? desc_mnmajor(a, ks) : desc_kmajor(a, ks), b_mn ? desc_mnmajor(b, ks) : desc_kmajor(b, ks),
-                                             instr, accumulate);
-                                    accumulate = 1;
-                                }
+                                multiply(tmem + buf * kBN, s, s, step > 0);
                                 mma_commit_pair(bar_empty + 8 * s);
                                 if (++s == kStages) {
                                     s = 0;
@@ -671,13 +703,15 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_at(bar_read_0 + 8 * buf);
-            if (++buf == 2) {
+            if constexpr (kPrecise) {  // one sum is under way at a time, in both accumulators
+                ready_phase ^= 1u;
+            } else if (++buf == 2) {
                 buf = 0;
                 ready_phase ^= 1u;
             }
         };
         while (work.next()) {
-            const int m = work.m, n = work.n, cols = min(kBN, work.n_ext() - n * kBN);
+            const int m = work.m, n = work.n, cols = work.cols();
             const float *bias = s_bias + parity * kBN;
             if constexpr (kKind != kProducts) {
                 const int col = n * kBN + tid;  // 256 finishing threads, 256 columns
@@ -732,13 +766,16 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     const int local = tgt - (p.b0 + n * kBN + c0);  // the target's place in these 32, if it is there
                     const bool here = tgt >= 0 && local >= 0 && local < 32;
                     if constexpr (kPrecise) {  // logits; probabilities from differences of logits
+                        const float2 x_back = make_float2(split.x_back, split.x_back), w_back = make_float2(split.w_back, split.w_back);
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + i);
-                            v[i] = fmaf(v[i] * split.x_back, split.w_back, b.x);
-                            v[i + 1] = fmaf(v[i + 1] * split.x_back, split.w_back, b.y);
-                            v[i + 2] = fmaf(v[i + 2] * split.x_back, split.w_back, b.z);
-                            v[i + 3] = fmaf(v[i + 3] * split.x_back, split.w_back, b.w);
+                            const float2 lo = fma2(mul2(make_float2(v[i], v[i + 1]), x_back), w_back, make_float2(b.x, b.y));
+                            const float2 hi = fma2(mul2(make_float2(v[i + 2], v[i + 3]), x_back), w_back, make_float2(b.z, b.w));
+                            v[i] = lo.x;
+                            v[i + 1] = lo.y;
+                            v[i + 2] = hi.x;
+                            v[i + 3] = hi.y;
                         }
                     } else {  // logits times log2(e)
 #pragma unroll
@@ -786,26 +823,38 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         }
                         float more = sum.x + sum.y;
                         if (kPrecise || !(more < 1e18f) || run_max == -INFINITY) {
-                            float top = v[0];
+                            float tops[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                            for (int i = 1; i < 32; ++i) top = fmaxf(top, v[i]);
+                            for (int i = 4; i < 32; ++i) tops[i & 3] = fmaxf(tops[i & 3], v[i]);
+                            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                             if (top > run_max) {
                                 run_sum *= ex2((run_max - top) * (kPrecise ? kLog2e : 1.f));
                                 run_max = top;
                             }
                             const float m0 = run_max == -INFINITY ? 0.f : run_max;
-                            float part[4] = {0.f, 0.f, 0.f, 0.f};
+                            const float2 from = make_float2(-m0, -m0);
+                            sum = make_float2(0.f, 0.f);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) part[i & 3] += ex2((v[i] - m0) * (kPrecise ? kLog2e : 1.f));
-                            more = (part[0] + part[1]) + (part[2] + part[3]);
+                            for (int i = 0; i < 32; i += 2) {
+                                float2 d = add2(make_float2(v[i], v[i + 1]), from);
+                                if constexpr (kPrecise) d = mul2(d, make_float2(kLog2e, kLog2e));
+                                sum = add2(sum, make_float2(ex2(d.x), ex2(d.y)));
+                            }
+                            more = sum.x + sum.y;
                         }
                         run_sum += more;
                     } else {
                         // p g - e / V g, with p = exp(z - lse); where every g of the warp is 1 and nothing is smoothed,
                         // the type's scale rides in the exponent
                         if constexpr (kPrecise) {
+                            const float2 from = make_float2(-row_lse, -row_lse), g2 = make_float2(row_g, row_g), u2 = make_float2(-uniform, -uniform);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = fmaf(ex2((v[i] - row_lse) * kLog2e), row_g, -uniform);
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), from), make_float2(kLog2e, kLog2e));
+                                const float2 dz = fma2(make_float2(ex2(d.x), ex2(d.y)), g2, u2);
+                                v[i] = dz.x;
+                                v[i + 1] = dz.y;
+                            }
                         } else {
                             const float2 from = make_float2(-row_l2, -row_l2);
 #pragma unroll
@@ -852,20 +901,26 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         const uint32_t narrow = lane * 64, turn = lane >> 1 & 3;  // a row of a 64-byte-swizzled tile
                         if constexpr (kPrecise) {
                             float left[32];
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) left[i] = split.half ? v[i] * kHalfDz : v[i];
-                            for (int plane = 0; plane < (split.half ? 2 : 3); ++plane) {
+                            auto store_plane = [&](int plane, auto next_word) {
                                 const uint32_t tile = next_tile();
 #pragma unroll
                                 for (int u = 0; u < 4; ++u) {
                                     uint32_t w[4];
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        w[i] = split.half ? take_half(left[8 * u + 2 * i], left[8 * u + 2 * i + 1])
-                                                          : take_plane(left[8 * u + 2 * i], left[8 * u + 2 * i + 1]);
+                                    for (int i = 0; i < 4; ++i) w[i] = next_word(left[8 * u + 2 * i], left[8 * u + 2 * i + 1]);
                                     st_shared_v4(tile + narrow + ((u ^ turn) << 4), w[0], w[1], w[2], w[3]);
                                 }
                                 send(n * kBN + c0, plane, tile);
+                            };
+                            if (split.half) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) left[i] = v[i] * kHalfDz;
+                                store_plane(0, [](float &a, float &b) { return take_half(a, b); });
+                                store_plane(1, [](float &a, float &b) { return pack2<__half>(a, b); });
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) left[i] = v[i];
+                                for (int plane = 0; plane < 3; ++plane) store_plane(plane, [](float &a, float &b) { return take_plane(a, b); });
                             }
                         } else if (p.dz_planes == 1) {
                             const int at = (c0 >> 5) & 1;  // which half of the tile's 64 columns
@@ -897,7 +952,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 } else {
                     const Product &q = p.product[work.which];
                     const int64_t in_piece = static_cast<int64_t>(m) * kBM + trow;
-                    const int col = n * kBN + c0, left = q.n_ext - col;
+                    const int col = work.n0() + c0, left = q.n_ext - col;
                     if (work.which == 0 ? in_piece < rows_here : q.row_offset + in_piece < q.row_end) {
                         if (q.parts > 1) {
                             store_row(q.partial + work.part * q.partial_plane + in_piece * q.acc_ld, q.acc_ld * 4, col, left, v);
@@ -919,9 +974,12 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     }
                 }
             };
-            const int first = half * (kBN / 2);
+            // of the products' narrower tiles each half has half of the 32s, too
+            const int middle = kKind == kProducts ? (cols + 63) / 64 * 32 : kBN / 2, first = half * middle;
+            const int until = kKind == kProducts && half == 0 ? min(cols, middle) : cols;
             bool ok;
             if constexpr (kPrecise) {  // add the runs up in registers, then finish
+                const float low_weight = split.half ? 1.f / kLowScale : 1.f;
                 float sum[4][32];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -929,29 +987,35 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
                 ok = true;
                 for (int kr = work.k0; ok && kr < work.k1; kr += kRunTiles) {
-                    for (int group = 0; ok && group < groups; ++group) {
-                        ok = __all_sync(0xffffffffu, mbar_wait_or_stop(bar_ready + 8 * buf, ready_phase, stop));
-                        if (!ok) break;
-                        fence_after_sync();
-                        const float weight = group < groups - 1 ? 1.f / kLowScale : 1.f;
+                    ok = __all_sync(0xffffffffu, mbar_wait_or_stop(bar_ready, ready_phase, stop));
+                    if (!ok) break;
+                    fence_after_sync();
+                    const float2 weight = make_float2(low_weight, low_weight);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (first + 32 * j < cols) {
-                                uint32_t r[32];
-                                tmem_ld32(tmem + lanes + buf * kBN + first + 32 * j, r);
-                                tmem_ld_wait_for(r);
+                    for (int j = 0; j < 4; ++j) {
+                        if (first + 32 * j < until) {
+                            uint32_t low[32], high[32];
+                            tmem_ld32(tmem + lanes + first + 32 * j, low);
+                            tmem_ld32(tmem + lanes + kBN + first + 32 * j, high);
+                            tmem_ld_wait_for(low);
+                            tmem_ld_wait_for(high);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) sum[j][i] = fmaf(__uint_as_float(r[i]), weight, sum[j][i]);
+                            for (int i = 0; i < 32; i += 2) {
+                                float2 v = make_float2(sum[j][i], sum[j][i + 1]);
+                                v = fma2(make_float2(__uint_as_float(low[i]), __uint_as_float(low[i + 1])), weight, v);
+                                v = add2(v, make_float2(__uint_as_float(high[i]), __uint_as_float(high[i + 1])));
+                                sum[j][i] = v.x;
+                                sum[j][i + 1] = v.y;
                             }
                         }
-                        release();
                     }
+                    release();
                 }
                 if constexpr (kKind != kProducts) ok = !finish_barrier_or(!ok);  // s_bias is whole, and all these warps go on or none does
                 if (!ok) break;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (first + 32 * j < cols) {
+                    if (first + 32 * j < until) {
                         finish(sum[j], first + 32 * j);
                         __syncwarp();
                         if constexpr (kKind == kGrad) {
@@ -969,7 +1033,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 // (loading the next 32 columns ahead was slower: 1.4 times for grad, whose sums then spill, 1.03 for stats)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (first + 32 * j < cols) {
+                    if (first + 32 * j < until) {
                         uint32_t r[32];
                         float v[32];
                         if (!empty) {
@@ -1544,6 +1608,10 @@ constexpr int64_t kFewTokens = 256;
 constexpr int64_t few_tokens(int dtype) { return dtype == BPT_F32 ? 8 : 2; }
 constexpr int kFewBlocks = 148 * 2;
 
+// Elements from row to row of a copied operand: whole 128-byte lines, which a row of a TMA box is one of, unless that would
+// be much longer.
+int64_t packed_row(int dim) { return dim > 128 ? ce_div(dim, kBK) * kBK : ce_div(dim, 8) * 8; }
+
 struct Shape {
     int64_t n;
     int vocab, dim, dtype, planes, dz_planes;
@@ -1551,15 +1619,15 @@ struct Shape {
     bool pack_x, pack_w, few;
     Shape(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t n_, int vocab_, int dim_, int dtype_)
         : n(n_), vocab(vocab_), dim(dim_), dtype(dtype_), planes(dtype_ == BPT_F32 ? 3 : 1),
-          dz_planes(dtype_ == BPT_F32 ? 3 : n_ <= kFewTokens ? 2 : 1), packed_ld(ce_div(dim_, 8) * 8),
+          dz_planes(dtype_ == BPT_F32 ? 3 : n_ <= kFewTokens ? 2 : 1), packed_ld(packed_row(dim_)),
           pack_x(!tma_ready(x, ldx, dtype_)), pack_w(!tma_ready(w, ldw, dtype_)) {
         const int vec = dtype_ == BPT_F32 ? 4 : 8;
         const int tokens = n_ <= 1 ? 1 : n_ <= 2 ? 2 : n_ <= 4 ? 4 : 8;  // whose features fit in 40 KB
         few = n_ <= few_tokens(dtype_) && int64_t(tokens) * dim_ <= 10000 && dim_ % vec == 0 && ldw % vec == 0 &&
               reinterpret_cast<uintptr_t>(w) % 16 == 0;
     }
-    int logit_pairs() const { return planes == 3 ? 6 : 1; }                          // plane products of the logits
-    int product_pairs() const { return planes == 3 ? 6 : dz_planes == 2 ? 2 : 1; }  // and of the gradients
+    // stages of a K block: `planes` for the logits, for the gradients
+    int product_stages() const { return planes == 3 ? 3 : dz_planes; }
     int64_t m_tiles() const { return ce_div(n, kBM); }
     int v_tiles() const { return static_cast<int>(ce_div(vocab, kBN)); }
     int64_t packed(int64_t rows) const { return align_up(rows * packed_ld, 64) * planes; }
@@ -1600,12 +1668,12 @@ constexpr int64_t kDzBytes = 256 << 20;
 // What a launch costs in K blocks, and the elements of a sum that is read and written once more in the time of one.
 constexpr int64_t kLaunchSteps = 15, kStepElements = 200000;
 // Splits the longer tiles along K where that shortens the work of the pair with the most of it: few tiles, long K.
-Deal split_and_deal(Product &x, Product &w, int n_pairs) {
+Deal split_and_deal(Product &x, Product &w, int stages) {
     Product &longer = w.tiles() == 0 || (x.tiles() > 0 && x.k_tiles >= w.k_tiles) ? x : w;
     Product &other = &longer == &x ? w : x;
     auto dealt = [&](int parts) {
-        const int l = unit_steps(longer.k_tiles, parts, n_pairs), u = static_cast<int>(longer.tiles() * parts);
-        const int lo = unit_steps(other.k_tiles, 1, n_pairs), uo = static_cast<int>(other.tiles());
+        const int l = unit_steps(longer.k_tiles, parts, stages), u = static_cast<int>(longer.tiles() * parts);
+        const int lo = unit_steps(other.k_tiles, 1, stages), uo = static_cast<int>(other.tiles());
         const int pairs = std::max(1, std::min(kPairs, u + uo));
         return &longer == &x ? deal(pairs, l, u, lo, uo) : deal(pairs, lo, uo, l, u);
     };
@@ -1663,7 +1731,7 @@ struct BackwardSpace {
                 sum_rows = std::max(sum_rows, 8 * (s.planes == 3 ? m : shared_pieces(m, m * n)));
                 Product px, pw;
                 products(s, want_dx, want_dw, r, c, &px, &pw);
-                split_and_deal(px, pw, s.product_pairs());
+                split_and_deal(px, pw, s.product_stages());
                 if (px.parts > 1) parts = std::max(parts, px.parts * rows * acc_ld);
                 if (pw.parts > 1) parts = std::max(parts, pw.parts * cols * acc_ld);
             }
@@ -1688,8 +1756,8 @@ struct BackwardSpace {
             col_cuts = ce_div(n, pn);
             Product x, w;
             products(s, want_dx, want_dw, pm * kBM, pn * kBN, &x, &w);
-            const int64_t steps = split_and_deal(x, w, s.product_pairs()).steps +
-                                  ce_div(pm * pn, kPairs) * (ce_div(s.dim, kBK) * s.logit_pairs() + 1) + 2 * kLaunchSteps;
+            const int64_t steps = split_and_deal(x, w, s.product_stages()).steps +
+                                  ce_div(pm * pn, kPairs) * (ce_div(s.dim, kBK) * s.planes + 1) + 2 * kLaunchSteps;
             const int64_t again = ((col_cuts - 1) * s.n + (row_cuts - 1) * s.vocab) * s.dim / kStepElements;
             const int64_t cost = row_cuts * col_cuts * steps + again;
             if (best < 0 || cost < best) {
@@ -1717,7 +1785,10 @@ struct BackwardSpace {
         *x = Product{};
         *w = Product{};
         x->n_ext = w->n_ext = s.dim;
-        x->n_tiles = w->n_tiles = static_cast<int>(ce_div(s.dim, kBN));
+        // tiles of about the same width, so that the pairs' shares are alike: 4099 x 8003 x 300 in fp32 WWW us with tiles of
+        // 160 and 140 columns, XXX with 256 and 44
+        x->width = w->width = static_cast<int>(ce_div(ce_div(s.dim, ce_div(s.dim, kBN)), 32) * 32);
+        x->n_tiles = w->n_tiles = static_cast<int>(ce_div(s.dim, x->width));
         x->m_tiles = want_dx ? static_cast<int>(ce_div(r, kBM)) : 0;
         w->m_tiles = want_dw ? static_cast<int>(ce_div(c, kBM)) : 0;
         x->k_tiles = static_cast<int>(ce_div(c, kBK));
@@ -1835,7 +1906,6 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
         p.n_tiles = s.v_tiles();
         p.k_tiles = static_cast<int>(ce_div(s.dim, kBK));
         p.n_ext = s.vocab;
-        p.n_pairs = s.logit_pairs();
         p.dz_planes = s.dz_planes;
         p.status = f.status;
         p.split = f.found;
@@ -1905,7 +1975,6 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     maps.e = maps.d;
     if (f.gathered) BPT_TRY(make_map(&maps.e, kHalf, f.gathered, s.n, s.dim, s.packed_ld, 1, 0, 64));
     Params p{};
-    p.n_pairs = s.logit_pairs();
     p.dz_planes = s.dz_planes;
     p.status = f.status;
     p.split = f.found;
@@ -1954,8 +2023,8 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
             q.m_ext = static_cast<int>(rows);
             BackwardSpace::products(s, dx, dw, rows, cols, &q.product[0], &q.product[1]);
             Product &px = q.product[0], &pw = q.product[1];
-            const Deal d = split_and_deal(px, pw, s.product_pairs());
-            q.n_pairs = s.product_pairs();
+            const Deal d = split_and_deal(px, pw, s.product_stages());
+            q.a_planes = s.dz_planes;
             q.first = d.first;
             q.busy = d.busy;
             q.after_busy = d.after_busy;
