@@ -533,7 +533,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     if (warp >= kFinishWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
         if (warp == kFinishWarps) {
-            if (lane == 0) {  // ---- loads of this block's rows of A and half of B
+            if (elect_one()) {  // ---- loads of this block's rows of A and half of B
                 int s = 0;
                 uint32_t phase = 0, issued = 0;
                 bool ok = true;
@@ -591,7 +591,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 }
             }
         } else if (warp == kFinishWarps + 1) {
-            if (lane == 0 && rank == 0) {  // ---- products
+            if (rank == 0 && elect_one()) {  // ---- products
                 int s = 0, buf = 0;
                 uint32_t phase = 0, read_phase = 0;
                 bool ok = true;

@@ -79,6 +79,14 @@ __device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a, uint64_t b
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// One lane of a whole warp.  Where a branch on this guards mma_pair, the compiler knows that one thread runs it and keeps the
+// descriptors in uniform registers; guarded by `lane == 0` an instruction cost 170 cycles to issue, more than the 128 that
+// 256 x 256 x 16 takes (65536 x 8000 x 512, forward: 447 against 411 us).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+    return one;
+}
 // One arrival on each block's barrier at this offset once the products issued so far are done.
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
