@@ -48,7 +48,7 @@ constexpr int kChunkBytes = 64 * 128;  // an MN-major tile: 64 rows along K of 6
 // Eight warps finish tiles, one loads, one issues products (two more make its warpgroup whole).  The finishing warps take
 // registers that the others leave: 256 * 216 + 128 * 72 = 384 * 168, what the block is launched with.
 constexpr int kFinishWarps = 8, kThreads = (kFinishWarps + 4) * 32;
-constexpr int kFinishRegs = 216, kOtherRegs = 72;
+constexpr int kFinishRegs = 208, kOtherRegs = 88;
 static_assert(kFinishWarps * 32 * kFinishRegs + 128 * kOtherRegs <= kThreads * 168, "the block's registers");
 constexpr int kPairs = 74;             // pairs of blocks at most: one block per SM
 constexpr int kRunTiles = 8;           // fp32: K blocks added up by the tensor core before the sum is taken out
@@ -57,10 +57,18 @@ enum Kind { kStats, kGrad, kProducts };
 // Shared memory: the bias of two tiles, barriers; from the next 1024-byte boundary on operand stages, and for grad a tile
 // of 32 rows x 64 columns of dZ per finishing warp, on its way out.
 constexpr int kOutBytes = 32 * 128;
-constexpr int out_bytes(int kind) { return kind == kGrad ? kFinishWarps * kOutBytes : 0; }
 constexpr int kHeadBytes = 3 << 10;
-constexpr int smem_bytes(int kind) { return kHeadBytes + kStages * kStageBytes + out_bytes(kind); }
-static_assert(smem_bytes(kGrad) <= 227 * 1024 && smem_bytes(kStats) <= 227 * 1024, "a block's shared memory");
+constexpr int smem_bytes(int kind) { return kHeadBytes + kStages * kStageBytes + (kind == kProducts ? 0 : kFinishWarps * kOutBytes); }
+static_assert(smem_bytes(kGrad) <= 227 * 1024, "a block's shared memory");
+// stats and grad, 16-bit, rows of at most kKeepTiles K blocks: the operand that stays the same from tile to tile along a
+// pair's walk is kept, one K block in each 16 KB, and the rest of the shared memory has stages of the other operand alone:
+// half the loads.  Where a pair has at least kKeepRun tiles.  65536 x 8000 x 512 forward (109 tiles a pair) kept 392 us,
+// else 411; 8192 x 50000 x 512 forward + backward (85, 17 a piece) 1572 against 1634; 65536 x 256 x 512 (3.5) 133
+// against 130, whose walks end before the fewer stages have paid.
+constexpr int kKeepTiles = 8, kKeepRun = 8;
+constexpr int flow_stages(int kind, int k_tiles) { return (kStages * kStageBytes + (kind == kStats ? kFinishWarps * kOutBytes : 0)) / kABytes - k_tiles; }
+constexpr int kMostStages = flow_stages(kStats, 1);
+static_assert(kABytes == kBBytes && flow_stages(kGrad, kKeepTiles) >= 4 && kMostStages >= kStages, "stages of one operand");
 enum { kReduceNone = 0, kReduceMean = 1, kReduceSum = 2 };
 
 // One of the two products of a piece.  A unit of work is a tile and a part of its K.
@@ -459,36 +467,33 @@ template <typename T> __device__ __forceinline__ void finish_bias(const Params &
 
 // map_a, map_b: stats, grad: X and W rows; products: dZ rows and W columns.  map_c: dZ, as it is stored (grad), its columns
 // (products).  map_d, map_e: stats, grad: the copy of X, rows; products: X columns, those of its copy.
-template <typename T, int kKind>
+template <typename T, int kKind, bool kKeep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
                  const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_e, const __grid_constant__ Params p) {
     constexpr bool kPrecise = std::is_same<T, float>::value;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     float *s_bias = reinterpret_cast<float *>(smem_raw);  // [2][256]
-    // full (block 0's is used) and empty per stage, sums ready and sums read (block 0's) per accumulator
+    // full (block 0's is used) and empty per stage and per K block that is kept, sums ready and sums read (block 0's) per
+    // accumulator
     const uint32_t bars = smem_u32(smem_raw) + 2 * kBN * 4;
-    const uint32_t bar_full = bars, bar_empty = bars + 8 * kStages, bar_ready = bars + 16 * kStages, bar_read = bar_ready + 16,
-                   bar_drain = bar_read + 16, tmem_slot = bar_drain + 8;
-    constexpr int kWordsAt = 2 * kBN * 4 + 16 * kStages + 40;
+    constexpr int kLoadBars = 8 * 2 * (kMostStages + kKeepTiles);
+    const uint32_t bar_full = bars, bar_empty = bar_full + 8 * kMostStages, keep_full = bar_empty + 8 * kMostStages,
+                   keep_empty = keep_full + 8 * kKeepTiles, bar_ready = bars + kLoadBars, bar_read = bar_ready + 16, bar_drain = bar_read + 16,
+                   tmem_slot = bar_drain + 8;
+    constexpr int kWordsAt = 2 * kBN * 4 + kLoadBars + 40;
     volatile uint32_t *tmem_word = reinterpret_cast<volatile uint32_t *>(smem_raw + kWordsAt);
     volatile int *stop = reinterpret_cast<volatile int *>(smem_raw + kWordsAt + 4);
-    const uint32_t base = (bars + 16 * kStages + 48 + 1023u) & ~1023u;  // the same offset in both blocks
+    const uint32_t base = (bars + kLoadBars + 48 + 1023u) & ~1023u;  // the same offset in both blocks
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_rank();
 
-    if (tid == 0) {
-        *stop = 0;
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(bar_full + 8 * s, 1);
-            mbar_init(bar_empty + 8 * s, 1);
-        }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(bar_ready + 8 * b, 1);
-            mbar_init(bar_read + 8 * b, 2 * kFinishWarps);
-        }
-        mbar_init(bar_drain, 1);
+    static_assert(kLoadBars / 8 + 5 <= kThreads, "a thread sets up a barrier");
+    if (tid < kLoadBars / 8 + 5) {  // ready and read, two each, and drain come last
+        const int last = tid - kLoadBars / 8;
+        mbar_init(bars + 8 * tid, last == 2 || last == 3 ? 2 * kFinishWarps : 1);
         fence_mbar_init();
+        if (tid == 0) *stop = 0;
     }
     if (warp == kFinishWarps + 1) tmem_alloc_pair(tmem_slot, 512);
     fence_before_sync();
@@ -532,12 +537,40 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     work.start();
     if (warp >= kFinishWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
+        const bool keep_b = kKind == kGrad || p.n_tiles == 1;  // W's rows, else X's
+        const int stages = kKeep ? flow_stages(kKind, p.k_tiles) : kStages;
+        const uint32_t flow = base + p.k_tiles * kABytes;      // kKeep: the stages
         if (warp == kFinishWarps) {
             if (elect_one()) {  // ---- loads of this block's rows of A and half of B
                 int s = 0;
-                uint32_t phase = 0, issued = 0;
+                uint32_t phase = 0, issued = 0, keep_issued = 0;
                 bool ok = true;
-                while (ok && work.next()) {
+                for (int kept = -1; kKeep && ok && work.next();) {
+                    const int m0 = a0 + work.m * kBM + static_cast<int>(rank) * kRows, n0 = p.b0 + work.n0() + static_cast<int>(rank) * (work.width() / 2);
+                    const bool fresh = kept != (keep_b ? work.n : work.m);
+                    kept = keep_b ? work.n : work.m;
+                    auto load = [&](uint32_t to, bool of_b, int k, uint32_t full) {
+                        if (rank == 0) mbar_expect(full, 2 * kABytes);
+                        tma_load_pair(to, of_b ? &map_b : copied ? &map_d : &map_a, k * kBK, of_b ? n0 : m0, 0, map_to(full, 0));
+                    };
+                    for (int k = 0; k < p.k_tiles; ++k) {
+                        if (fresh) {
+                            ok = mbar_wait_or_stop(keep_empty + 8 * k, (keep_issued / p.k_tiles & 1u) ^ 1u, stop);
+                            if (!ok) break;
+                            load(base + k * kABytes, keep_b, k, keep_full + 8 * k);
+                            ++keep_issued;
+                        }
+                        ok = mbar_wait_or_stop(bar_empty + 8 * s, phase ^ 1u, stop);
+                        if (!ok) break;
+                        load(flow + s * kABytes, !keep_b, k, bar_full + 8 * s);
+                        ++issued;
+                        if (++s == stages) {
+                            s = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+                while (!kKeep && ok && work.next()) {
                     const int m0 = work.m * kBM + static_cast<int>(rank) * kRows, half = work.width() / 2;
                     const int n0 = work.n0() + static_cast<int>(rank) * half, chunks = (half + 63) / 64;
                     const int run = kPrecise ? kRunTiles : work.k1;
@@ -583,11 +616,15 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     }
                 }
             if (!ok) {  // the last loads of every stage land before the block ends (block 0's barriers know)
-                    for (uint32_t i = 0; i < kStages && i < issued; ++i) {
-                        const uint32_t load = issued - 1 - i, bar = bar_full + 8 * (load % kStages);
-                        const long long start = clock64();
-                        while (clock64() - start < kWaitCycles / 8 && !(rank == 0 && mbar_try(bar, (load / kStages) & 1u))) {}
-                    }
+                    auto landed = [&](uint32_t bars, uint32_t n, uint32_t count) {
+                        for (uint32_t i = 0; i < n && i < count; ++i) {
+                            const uint32_t load = count - 1 - i;
+                            const long long start = clock64();
+                            while (clock64() - start < kWaitCycles / 8 && !(rank == 0 && mbar_try(bars + 8 * (load % n), (load / n) & 1u))) {}
+                        }
+                    };
+                    landed(bar_full, stages, issued);
+                    if constexpr (kKeep) landed(keep_full, p.k_tiles, keep_issued);
                 }
             }
         } else if (warp == kFinishWarps + 1) {
@@ -595,7 +632,41 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 int s = 0, buf = 0;
                 uint32_t phase = 0, read_phase = 0;
                 bool ok = true;
-                while (ok && work.next()) {
+                uint32_t keep_phase = 1;
+                for (int kept = -1; kKeep && ok && work.next();) {
+                    const bool fresh = kept != (keep_b ? work.n : work.m);
+                    if (fresh) {
+                        keep_phase ^= 1u;
+                        if (kept >= 0)
+                            for (int k = 0; k < p.k_tiles; ++k) mma_commit_pair(keep_empty + 8 * k);  // once the products so far are done
+                        kept = keep_b ? work.n : work.m;
+                    }
+                    ok = mbar_wait_or_stop(bar_read + 8 * buf, read_phase ^ 1u, stop);
+                    if (!ok) break;
+                    const uint32_t instr = ce_instr(kIsHalf<T>, work.width(), false, false);
+                    const uint64_t kept_desc = desc_kmajor(base, 0), flow_desc = desc_kmajor(flow, 0);
+                    for (int k = 0; k < p.k_tiles; ++k) {
+                        ok = (!fresh || mbar_wait_or_stop(keep_full + 8 * k, keep_phase, stop)) && mbar_wait_or_stop(bar_full + 8 * s, phase, stop);
+                        if (!ok) break;
+                        fence_after_sync();
+                        const uint64_t of_kept = kept_desc + k * (kABytes / 16), of_flow = flow_desc + s * (kABytes / 16);
+#pragma unroll
+                        for (int ks = 0; ks < kBK / 16; ++ks)
+                            mma_pair(tmem + buf * kBN, (keep_b ? of_flow : of_kept) + 2 * ks, (keep_b ? of_kept : of_flow) + 2 * ks, instr, k + ks > 0);
+                        mma_commit_pair(bar_empty + 8 * s);
+                        if (++s == stages) {
+                            s = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit_pair(bar_ready + 8 * buf);
+                    if (++buf == 2) {
+                        buf = 0;
+                        read_phase ^= 1u;
+                    }
+                }
+                while (!kKeep && ok && work.next()) {
                     const bool a_mn = kKind == kProducts && work.which == 1, b_mn = kKind == kProducts;
                     const uint32_t instr = ce_instr(kPrecise ? split.half : kIsHalf<T>, work.width(), a_mn, b_mn);
                     // descriptors (addresses in them count 16 bytes) of the first stage, made once a tile: one thread issues all
@@ -1802,10 +1873,17 @@ struct Maps {
 };
 
 template <typename T, int kKind> int launch_ce(const Maps &m, const Params &p, int pairs, cudaStream_t stream) {
-    static OncePerDevice allowed;
-    BPT_CUDA(allow_smem(allowed, linear_ce_kernel<T, kKind>, smem_bytes(kKind)));
-    BPT_CUDA(launch_after(linear_ce_kernel<T, kKind>, 2 * pairs, kThreads, smem_bytes(kKind), stream, m.a, m.b, m.c, m.d, m.e, p));
-    return BPT_OK;
+    auto launch = [&](auto keep) -> int {
+        static OncePerDevice allowed;
+        auto kernel = linear_ce_kernel<T, kKind, keep.value>;
+        BPT_CUDA(allow_smem(allowed, kernel, smem_bytes(kKind)));
+        BPT_CUDA(launch_after(kernel, 2 * pairs, kThreads, smem_bytes(kKind), stream, m.a, m.b, m.c, m.d, m.e, p));
+        return BPT_OK;
+    };
+    if constexpr (!kIsFloat<T> && kKind != kProducts) {
+        if (p.k_tiles <= kKeepTiles && ce_div(p.m_ext, kBM) * p.n_tiles >= kKeepRun * pairs) return launch(std::true_type());
+    }
+    return launch(std::false_type());
 }
 
 #define BPT_TRY(call)                  \
