@@ -1503,7 +1503,9 @@ __global__ void linear_ce_pack_kernel(const T *__restrict__ src, int64_t ld, int
 
 // ---- the tokens that count: how many a block has, then, where some are ignored, which they are, in their order.  A block
 // has 256 tokens, or as many times 256 as keep the blocks' number (each block reads all their counts) below kTokenBlocks.
-constexpr int kTokenBlock = 256, kTokenBlocks = 4096;
+// Up to kTokensAlone tokens each block counts them all itself, which spares a launch: 777 x 10001 x 512 forward + backward,
+// bound by host time, 86 us against 90; with 4099 x 8003 x 300 in fp32 it is slower, 316 against 313.
+constexpr int kTokenBlock = 256, kTokenBlocks = 4096, kTokensAlone = 2048;
 __host__ __device__ __forceinline__ int64_t block_tokens(int64_t n) {
     return (n + int64_t(kTokenBlocks) * kTokenBlock - 1) / (int64_t(kTokenBlocks) * kTokenBlock) * kTokenBlock;
 }
@@ -1543,11 +1545,21 @@ __global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uin
     __shared__ int s_warp[kTokenBlock / 32], s_place[kTokenBlock];
     let_next_start();
     wait_for_previous();
+    const int64_t first = blockIdx.x * block_tokens(n), end = min(first + block_tokens(n), n);
     int all = 0, before = 0;
-    for (unsigned i = threadIdx.x; i < gridDim.x; i += kTokenBlock) {
-        const int v = counts[i];
-        all += v;
-        if (i < blockIdx.x) before += v;
+    if (n > kTokensAlone) {
+        for (unsigned i = threadIdx.x; i < gridDim.x; i += kTokenBlock) {
+            const int v = counts[i];
+            all += v;
+            if (i < blockIdx.x) before += v;
+        }
+    } else {
+#pragma unroll 8
+        for (int i = threadIdx.x; i < static_cast<int>(n); i += kTokenBlock) {
+            const int v = target[i] != ignore_index;
+            all += v;
+            if (i < first) before += v;
+        }
     }
     all = block_sum(all, s_warp);
     const bool last = blockIdx.x == gridDim.x - 1;
@@ -1556,7 +1568,6 @@ __global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uin
     before = block_sum(before, s_warp);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool dx_wide = ((reinterpret_cast<uintptr_t>(dx) | dx_row_bytes) & 15) == 0;
-    const int64_t first = blockIdx.x * block_tokens(n), end = min(first + block_tokens(n), n);
     for (int64_t start = first; start < end; start += kTokenBlock) {
         const int64_t token = start + threadIdx.x;
         const bool counts_here = token < end && target[token] != ignore_index;
@@ -1856,8 +1867,8 @@ struct BackwardSpace {
         *x = Product{};
         *w = Product{};
         x->n_ext = w->n_ext = s.dim;
-        // tiles of about the same width, so that the pairs' shares are alike: 4099 x 8003 x 300 in fp32 WWW us with tiles of
-        // 160 and 140 columns, XXX with 256 and 44
+        // tiles of about the same width, so that the pairs' shares are alike: 4099 x 8003 x 300 in fp32 361 us with tiles of
+        // 160 and 140 columns, 366 with 256 and 44
         x->width = w->width = static_cast<int>(ce_div(ce_div(s.dim, ce_div(s.dim, kBN)), 32) * 32);
         x->n_tiles = w->n_tiles = static_cast<int>(ce_div(s.dim, x->width));
         x->m_tiles = want_dx ? static_cast<int>(ce_div(r, kBM)) : 0;
@@ -1928,7 +1939,8 @@ int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x
     *x = Operand{c.x, c.ldx, 0};
     *w = Operand{c.w, c.ldw, 0};
     const unsigned blocks = static_cast<unsigned>(ce_div(s.n, block_tokens(s.n)));
-    BPT_CUDA(launch_after(linear_ce_count_kernel, blocks, kTokenBlock, 0, stream, c.target, s.n, c.ignore_index, t.counts));
+    if (s.n > kTokensAlone)
+        BPT_CUDA(launch_after(linear_ce_count_kernel, blocks, kTokenBlock, 0, stream, c.target, s.n, c.ignore_index, t.counts));
     BPT_CUDA(launch_after(linear_ce_gather_kernel, dim3(blocks, 4), kTokenBlock, 0, stream, static_cast<const uint16_t *>(c.x), c.ldx, s.n, s.dim,
                           c.target, c.ignore_index, t.counts, t.index, t.n_counted, t.gathered, s.packed_ld, static_cast<unsigned char *>(dx),
                           static_cast<int64_t>(s.dim) * static_cast<int64_t>(sizeof(T)), loss));
