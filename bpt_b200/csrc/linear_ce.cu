@@ -148,6 +148,7 @@ struct Split {
     bool half = false;                                 // two fp16 planes
     float x = 1.f, w = 1.f, x_back = 1.f, w_back = 1.f;  // scales before the split, and their inverses
 };
+constexpr int kFound = 5;  // those four, and the bits of the largest |g|
 constexpr unsigned kSpread = 24;
 __device__ __forceinline__ Split read_split(const unsigned *found) {
     Split s;
@@ -1434,6 +1435,8 @@ __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *__re
     __shared__ unsigned s_found[4];
     const int lane = threadIdx.x & 31;
     if (threadIdx.x < 4) s_found[threadIdx.x] = 0u;
+    let_next_start();
+    wait_for_previous();
     __syncthreads();
     unsigned best[4] = {0u, 0u, 0u, 0u};
     const int64_t stride = static_cast<int64_t>(gridDim.x) * 8;
@@ -1464,23 +1467,35 @@ __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *__re
     if (threadIdx.x < 4) atomicMax(&found[threadIdx.x], s_found[threadIdx.x]);
 }
 
+template <typename T> struct Unpacked {
+    const T *at;
+    int64_t ld, rows;
+    uint16_t *to;  // null: this operand is read where it lies
+    int64_t plane;
+};
 template <typename T>
-__global__ void linear_ce_pack_kernel(const T *__restrict__ src, int64_t ld, int64_t rows, int dim, uint16_t *__restrict__ dst,
-                                      int64_t dst_ld, int64_t plane, const int32_t *__restrict__ index, const int *__restrict__ n_counted,
-                                      const unsigned *__restrict__ found, int is_w) {
-    // X: the rows that count, and rows of zeros up to a whole K block
-    const int64_t counted = n_counted ? *n_counted : rows;
-    const int64_t pieces = dst_ld / 8, total = min((counted + kBK - 1) / kBK * kBK, rows) * pieces;
+__global__ void __launch_bounds__(256) linear_ce_pack_kernel(const Unpacked<T> x, const Unpacked<T> w, int dim, int64_t to_ld,
+                                                             const int32_t *__restrict__ index, const int *__restrict__ n_counted,
+                                                             const unsigned *__restrict__ found) {
+    let_next_start();
+    wait_for_previous();
+    // of X the rows that count, and rows of zeros up to a whole K block
+    const int64_t counted = *n_counted, pieces = to_ld / 8;
+    const int64_t of_x = x.to ? min((counted + kBK - 1) / kBK * kBK, x.rows) * pieces : 0, total = of_x + (w.to ? w.rows * pieces : 0);
     Split split;
     if constexpr (kIsFloat<T>) split = read_split(found);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t row = i / pieces;
-        const int c = static_cast<int>(i % pieces) * 8;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const bool is_w = i >= of_x;
+        const Unpacked<T> &o = is_w ? w : x;
+        const int64_t in = is_w ? i - of_x : i, row = in / pieces;
+        const int c = static_cast<int>(in - row * pieces) * 8;
+        const bool there = is_w || row < counted;
         // the index is there where some tokens are ignored
-        const T *from = src + (counted < rows && row < counted ? index[row] : row) * ld + c;
+        const T *from = o.at + (!is_w && counted < x.rows && there ? index[row] : row) * o.ld + c;
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = row < counted && c + j < dim ? to_acc<T>(from[j]) : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = there && c + j < dim ? to_acc<T>(from[j]) : 0.f;
+        uint16_t *to = o.to + row * to_ld + c;
         if constexpr (kIsFloat<T>) {
             if (split.half) {
 #pragma unroll
@@ -1492,11 +1507,10 @@ __global__ void linear_ce_pack_kernel(const T *__restrict__ src, int64_t ld, int
                 word.y = split.half ? take_half(v[2], v[3]) : take_plane(v[2], v[3]);
                 word.z = split.half ? take_half(v[4], v[5]) : take_plane(v[4], v[5]);
                 word.w = split.half ? take_half(v[6], v[7]) : take_plane(v[6], v[7]);
-                *reinterpret_cast<uint4 *>(dst + q * plane + row * dst_ld + c) = word;
+                *reinterpret_cast<uint4 *>(to + q * o.plane) = word;
             }
         } else {
-            *reinterpret_cast<uint4 *>(dst + row * dst_ld + c) =
-                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+            *reinterpret_cast<uint4 *>(to) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
         }
     }
 }
@@ -1541,7 +1555,7 @@ __global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uin
                                                                        const int32_t *__restrict__ counts, int32_t *__restrict__ index,
                                                                        int *__restrict__ n_counted, uint16_t *__restrict__ copy,
                                                                        int64_t copy_ld, unsigned char *__restrict__ dx, int64_t dx_row_bytes,
-                                                                       float *__restrict__ loss) {
+                                                                       float *__restrict__ loss, unsigned *__restrict__ found) {
     __shared__ int s_warp[kTokenBlock / 32], s_place[kTokenBlock];
     let_next_start();
     wait_for_previous();
@@ -1564,6 +1578,7 @@ __global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uin
     all = block_sum(all, s_warp);
     const bool last = blockIdx.x == gridDim.x - 1;
     if (last && blockIdx.y == 0 && threadIdx.x == 0) *n_counted = all;
+    if (last && blockIdx.y == 0 && threadIdx.x < kFound) found[threadIdx.x] = 0u;  // for the next kernels
     if (all == n) return;
     before = block_sum(before, s_warp);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1618,6 +1633,8 @@ __global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uin
 // max |g| over the tokens that count, as bits (ordered like the numbers; a NaN is above all).
 __global__ void linear_ce_top_kernel(const float *__restrict__ grad, const int64_t *__restrict__ target, int64_t rows,
                                      int64_t ignore_index, unsigned *__restrict__ top) {
+    let_next_start();
+    wait_for_previous();
     unsigned best = 0u;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows; i += static_cast<int64_t>(gridDim.x) * blockDim.x)
         if (target[i] != ignore_index) best = max(best, __float_as_uint(grad[i]) & 0x7FFFFFFFu);
@@ -1728,7 +1745,7 @@ struct ForwardSpace {
     ForwardSpace(Workspace &ws, const Shape &s) {
         status = ws.take<int>(1);
         ticket = ws.take<unsigned>(1);
-        found = ws.take<unsigned>(4);
+        found = ws.take<unsigned>(kFound);
         block_sums = ws.take<double>(2 * ce_div(s.n * 32, kLossThreads));
         z_target = ws.take<float>(s.n);
         // pieces x rows, with whatever part of the tokens counts: at most (pairs + two a block of rows) blocks of rows
@@ -1791,8 +1808,8 @@ struct BackwardSpace {
         const bool own_acc = s.dtype == BPT_F32 && s.dim == acc_ld;  // fp32 sums can live in the output itself
         status = ws.take<int>(1);
         ticket = ws.take<unsigned>(1);
-        grad_top = ws.take<unsigned>(1);
-        found = ws.take<unsigned>(4);
+        found = ws.take<unsigned>(kFound);
+        grad_top = found + kFound - 1;
         dz = ws.take<uint16_t>(dz_plane * s.dz_planes);
         x = s.pack_x ? ws.take<uint16_t>(s.packed(s.n)) : nullptr;
         w = s.pack_w ? ws.take<uint16_t>(s.packed(s.vocab)) : nullptr;
@@ -1918,19 +1935,6 @@ struct Tokens {  // the index and its length, on the device
     uint16_t *gathered;
 };
 
-template <typename T>
-int pack_operand(const void *src, int64_t ld, int64_t rows, const Shape &s, uint16_t *dst, const Tokens &t, bool is_w, const unsigned *found,
-                 cudaStream_t stream, Operand *out) {
-    out->at = dst;
-    out->ld = s.packed_ld;
-    out->plane = align_up(rows * s.packed_ld, 64);
-    const int64_t blocks = std::min<int64_t>(ce_div(rows * (s.packed_ld / 8), 256), 148 * 16);
-    linear_ce_pack_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<const T *>(src), ld, rows, s.dim, dst, s.packed_ld,
-                                                                               out->plane, is_w ? nullptr : t.index, is_w ? nullptr : t.n_counted, found,
-                                                                               is_w);
-    BPT_LAUNCH_CHECK();
-    return BPT_OK;
-}
 // The index of the tokens that count; X and W as the tiles read them: where they lie (X, where tokens are ignored: from
 // the copy), or packed.  loss: where ignored tokens' zeros go, or null; dx: the same for their rows of d x.
 template <typename T>
@@ -1943,17 +1947,21 @@ int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x
         BPT_CUDA(launch_after(linear_ce_count_kernel, blocks, kTokenBlock, 0, stream, c.target, s.n, c.ignore_index, t.counts));
     BPT_CUDA(launch_after(linear_ce_gather_kernel, dim3(blocks, 4), kTokenBlock, 0, stream, static_cast<const uint16_t *>(c.x), c.ldx, s.n, s.dim,
                           c.target, c.ignore_index, t.counts, t.index, t.n_counted, t.gathered, s.packed_ld, static_cast<unsigned char *>(dx),
-                          static_cast<int64_t>(s.dim) * static_cast<int64_t>(sizeof(T)), loss));
+                          static_cast<int64_t>(s.dim) * static_cast<int64_t>(sizeof(T)), loss, found));
     if constexpr (kIsFloat<T>) {
-        BPT_CUDA(cudaMemsetAsync(found, 0, 4 * sizeof(unsigned), stream));
         const int64_t found_by = std::min<int64_t>(ce_div(s.n + s.vocab, 8), 148 * 8);
-        linear_ce_spread_kernel<<<static_cast<unsigned>(found_by), 256, 0, stream>>>(static_cast<const float *>(c.x), c.ldx, s.n,
-                                                                                  static_cast<const float *>(c.w), c.ldw, s.vocab, s.dim,
-                                                                                  c.target, c.ignore_index, found);
-        BPT_LAUNCH_CHECK();
+        BPT_CUDA(launch_after(linear_ce_spread_kernel, static_cast<unsigned>(found_by), 256, 0, stream, static_cast<const float *>(c.x), c.ldx, s.n,
+                              static_cast<const float *>(c.w), c.ldw, int64_t(s.vocab), s.dim, c.target, c.ignore_index, found));
     }
-    if (s.pack_x) BPT_TRY(pack_operand<T>(c.x, c.ldx, s.n, s, x_to, t, false, found, stream, x));
-    if (s.pack_w) BPT_TRY(pack_operand<T>(c.w, c.ldw, s.vocab, s, w_to, t, true, found, stream, w));
+    if (!s.pack_x && !s.pack_w) return BPT_OK;
+    const Unpacked<T> from_x{static_cast<const T *>(c.x), c.ldx, s.n, x_to, align_up(s.n * s.packed_ld, 64)};
+    const Unpacked<T> from_w{static_cast<const T *>(c.w), c.ldw, s.vocab, w_to, align_up(s.vocab * s.packed_ld, 64)};
+    if (s.pack_x) *x = Operand{x_to, s.packed_ld, from_x.plane};
+    if (s.pack_w) *w = Operand{w_to, s.packed_ld, from_w.plane};
+    const int64_t rows = (s.pack_x ? s.n : 0) + (s.pack_w ? s.vocab : 0);
+    BPT_CUDA(launch_after(linear_ce_pack_kernel<T>, static_cast<unsigned>(std::min<int64_t>(ce_div(rows * (s.packed_ld / 8), 256), 148 * 16)), 256, 0,
+                          stream, from_x, from_w, s.dim, s.packed_ld, static_cast<const int32_t *>(t.index), static_cast<const int *>(t.n_counted),
+                          static_cast<const unsigned *>(found)));
     return BPT_OK;
 }
 
@@ -2050,10 +2058,8 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     Operand x, w;
     BPT_TRY(prepare_operands<T>(s, c, Tokens{f.index, f.counts, f.n_counted, f.gathered}, f.x, f.w, f.found, nullptr, dx, stream, &x, &w));
     if (c.reduction == kReduceNone) {
-        BPT_CUDA(cudaMemsetAsync(f.grad_top, 0, sizeof(unsigned), stream));
-        linear_ce_top_kernel<<<static_cast<unsigned>(std::min<int64_t>(ce_div(s.n, 256), 148)), 256, 0, stream>>>(grad, c.target, s.n,
-                                                                                                               c.ignore_index, f.grad_top);
-        BPT_LAUNCH_CHECK();
+        BPT_CUDA(launch_after(linear_ce_top_kernel, static_cast<unsigned>(std::min<int64_t>(ce_div(s.n, 256), 148)), 256, 0, stream, grad,
+                              c.target, s.n, c.ignore_index, f.grad_top));
     }
     Maps grad_maps, maps;
     BPT_TRY(make_map(&grad_maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
