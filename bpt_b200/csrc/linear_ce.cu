@@ -219,6 +219,16 @@ __device__ __forceinline__ uint32_t take_half(float &a, float &b) {
     return word;
 }
 
+// The same of gradients of logits, which are finite (or NaN, and then all planes may be).
+__device__ __forceinline__ uint32_t take_half_finite(float &a, float &b) {
+    const uint32_t word = pack2<__half>(a, b);
+    const float2 left = fma2(make_float2(unpack_low<__half>(word), unpack_high<__half>(word)), make_float2(-1.f, -1.f), make_float2(a, b));
+    const float2 next = mul2(left, make_float2(kLowScale, kLowScale));
+    a = next.x;
+    b = next.y;
+    return word;
+}
+
 // 32 neighbouring results of one row to the output: 32-byte stores where the row's address allows, else 4 elements, else one.
 template <typename T> __device__ __forceinline__ void store_row(T *row, int64_t row_bytes, int col, int n, const float (&v)[32]) {
     T *p = row + col;
@@ -418,7 +428,7 @@ template <typename T> __device__ __forceinline__ float result_scale(const Params
     if (p.reduction == kReduceMean) scale = *p.count > 0.f ? scale / *p.count : 0.f;
     if constexpr (kIsFloat<T>) {
         const Split split = read_split(p.split);
-        return which == 2 || !split.half ? scale : scale * (1.f / kHalfDz) * (which == 0 ? split.w_back : split.x_back);
+        return !split.half ? scale : scale * (1.f / kHalfDz) * (which == 0 ? split.w_back : which == 1 ? split.x_back : 1.f);
     }
     return scale * (1.f / kDzScale<T>);
 }
@@ -811,7 +821,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             row_g = 1.f;
                             if (p.reduction == kReduceNone) row_g = p.grad[row] * (1.f / top_scale(*p.grad_top));
                             if (tgt < 0) row_g = __int_as_float(0x7fffffff);  // no such class: the gradients say so
-                            row_g *= kDzScale<T>;
+                            row_g *= kPrecise ? (split.half ? kHalfDz : 1.f) : kDzScale<T>;
                         }
                         uniform = p.smoothing / static_cast<float>(p.vocab) * row_g;
                         row_skips = __any_sync(0xffffffffu, row_g == 0.f);
@@ -973,6 +983,8 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         const uint32_t narrow = lane * 64, turn = lane >> 1 & 3;  // a row of a 64-byte-swizzled tile
                         if constexpr (kPrecise) {
                             float left[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) left[i] = v[i];
                             auto store_plane = [&](int plane, auto next_word) {
                                 const uint32_t tile = next_tile();
 #pragma unroll
@@ -985,13 +997,9 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                 send(n * kBN + c0, plane, tile);
                             };
                             if (split.half) {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) left[i] = v[i] * kHalfDz;
-                                store_plane(0, [](float &a, float &b) { return take_half(a, b); });
+                                store_plane(0, [](float &a, float &b) { return take_half_finite(a, b); });
                                 store_plane(1, [](float &a, float &b) { return pack2<__half>(a, b); });
                             } else {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) left[i] = v[i];
                                 for (int plane = 0; plane < 3; ++plane) store_plane(plane, [](float &a, float &b) { return take_plane(a, b); });
                             }
                         } else if (p.dz_planes == 1) {
