@@ -1962,8 +1962,8 @@ int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x
                               static_cast<const float *>(c.w), c.ldw, int64_t(s.vocab), s.dim, c.target, c.ignore_index, found));
     }
     if (!s.pack_x && !s.pack_w) return BPT_OK;
-    const Unpacked<T> from_x{static_cast<const T *>(c.x), c.ldx, s.n, x_to, align_up(s.n * s.packed_ld, 64)};
-    const Unpacked<T> from_w{static_cast<const T *>(c.w), c.ldw, s.vocab, w_to, align_up(s.vocab * s.packed_ld, 64)};
+    const Unpacked<T> from_x{static_cast<const T *>(c.x), c.ldx, s.n, x_to, static_cast<int64_t>(align_up(s.n * s.packed_ld, 64))};
+    const Unpacked<T> from_w{static_cast<const T *>(c.w), c.ldw, s.vocab, w_to, static_cast<int64_t>(align_up(s.vocab * s.packed_ld, 64))};
     if (s.pack_x) *x = Operand{x_to, s.packed_ld, from_x.plane};
     if (s.pack_w) *w = Operand{w_to, s.packed_ld, from_w.plane};
     const int64_t rows = (s.pack_x ? s.n : 0) + (s.pack_w ? s.vocab : 0);
