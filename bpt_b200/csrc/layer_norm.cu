@@ -2,15 +2,20 @@
 //
 // The block of modules/attention.py ends each of its two halves with `norm(h + sublayer(h))`
 // (attention.py:79-81, 141, 168-171).  As two torch operators that is a read of two tensors and a
-// write for the sum, then a read and a write for the normalisation; here a warp owns a row, keeps
-// the sum in registers (fp32), reduces mean and variance with shuffles and writes the result
-// once: 3 passes of N x dim instead of 5.  HBM-bound: (2 reads + 1 write) x N x dim x bytes.
+// write for the sum, then a read and a write for the normalisation; here a row belongs to one warp (up to
+// 512 elements; to more warps beyond), which keeps the sum in registers (fp32), reduces mean and variance with
+// shuffles and writes the result once: 3 passes of N x dim instead of 5.
 //
 // With a = x + r, mean and rstd of a row of a, n = (a - mean) rstd and q = gy gamma the derivative is
 //     d a     = rstd (q - mean(q) - n mean(q n))         (the gradient of x and of r)
 //     d gamma = sum over rows of gy n,   d beta = sum over rows of gy
 // so one pass that reads x, r and gy and writes d a has everything; the sums over rows stay in the registers of
 // the threads that own a column, then go through one partial row per block (no atomics: the order is fixed).
+//
+// HBM-bound: (2 reads + 1 write) x N x dim x bytes forward, (3 reads + 1 write) backward.  131064 x 512 in bf16:
+// forward 68 us, backward 92 us, 5.9 and 5.8 TB/s or 90 and 89% of what a copy reaches; the sums of the partial rows
+// 8 us by themselves, half of it behind the backward's end.  What is left: the reads and writes of a memory that turns
+// round between them, and 23% (backward) and 41% (forward) of the warps an SM could hold, which the rows ahead make up for.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -453,8 +458,7 @@ layer_norm_backward_kernel(const T *__restrict__ gy, const T *__restrict__ x, co
 constexpr int kReduceRows = 16;
 template <typename T>
 __global__ void __launch_bounds__(32 * kReduceRows)
-layer_norm_reduce_kernel(const float *__restrict__ partial, int n_partial, int dim, T *__restrict__ dgamma,
-                         T *__restrict__ dbeta) {
+layer_norm_reduce_kernel(const float *partial, int n_partial, int dim, T *dgamma, T *dbeta) {
     tc5::wait_for_previous();
     __shared__ float part[kReduceRows][32];
     const int c = blockIdx.x * 32 + threadIdx.x;

@@ -13,7 +13,7 @@
 // of two on one pair of SMs) walks 256 x 256 tiles, 128 rows of the result in each block.  In each block one warp brings
 // operand tiles in by TMA (128-byte swizzle, six stages of 32 KB; B's rows are shared, half in each block), one thread
 // of the pair issues tcgen05.mma.cta_group::2 into one of two accumulators in tensor memory, and eight warps read the
-// other accumulator and finish the tile.
+// other accumulator and finish the tile.  (Sixteen warps spilled grad's sums and made stats no faster.)
 //   stats     Z tiles of consecutive vocabulary blocks of one block of tokens: a running maximum and sum per row stay in
 //             registers, a row's pieces (one per pair that worked on it) are merged by the loss kernel;
 //   grad      Z tiles once more (cheaper than keeping them: at D = 512 a logit costs 0.7 ps of tensor time, its fp32
@@ -21,15 +21,23 @@
 //             A pair walks the token blocks of one vocabulary block, so d b stays in registers, summed over the rows
 //             of a thread, before the rounding of dZ;
 //   products  dZ W and dZ^T X of the piece in one launch.  dZ is read K-major by the one and MN-major by the other.
+// What bounds them, at 8192 x 10000 x 512 in bf16, each by itself: stats 66 us (1270 TFLOP/s) and grad 95 us (880; it also
+// writes 164 MB) by the finishing of a tile, whose exponentials, sums and stores two warps a scheduler do; products 114 us
+// (1470, 90% of what a library product of 8192 x 8192 x 8192 reaches) by the 11.7 TB/s at which operands come from the L2.
+// Long walks hide the finishing: stats of 65536 x 8000 x 512 take 332 us (1620 TFLOP/s) alone, 400 in a long run, where the
+// power limit slows everything (library products: 1640 and 1400 TFLOP/s).
 // dZ is rounded to the operands' 16-bit type, without g where all g_i are one number (the scale goes onto the fp32
 // results): a half-step error of each probability, the size of the rounding of the gradients themselves.
 // fp32 operands are split into 16-bit planes, and each product of matrices is run as the products of planes whose weight
 // is above 2^-24.  Scaled by a power of two to the top of fp16's range, an operand is two fp16 planes, the second kept
 // times 2^11: 22 significant bits by rounding, down to 2^-29 of the largest number, and good to 2^-51 of that number
-// below; three products.  That is taken where no row's largest is below 2^-24 of the matrix's largest.  Otherwise three
+// below; three products (of second planes none is needed).  That is taken where no row's largest is below 2^-24 of the matrix's largest.  Otherwise three
 // bf16 planes (24 bits by truncation, exact, any range), six products.  A first pass over X and W finds which, on the
 // device.  The tensor core rounds its running sum towards zero, a bias that grows with K, so the fp32 kernels take the
-// accumulator out every 512 of K, and between products of different scales, and add these runs up in registers.
+// accumulators out every 512 of K and add these runs up in registers; the products of the first planes have an accumulator
+// of their own, so that the small ones do not lose their low bits to it.  4099 x 8003 x 300, 12% ignored, forward +
+// backward: 290 us, 1.0e-6 from the values in 64 bits (an fp32 library product: 2.1e-6); stats 50, grad 71, products 125,
+// copies 30 us.  Runs of 1024 of K would save 10 us and nearly double the error.
 #include <algorithm>
 #include <type_traits>
 
@@ -295,8 +303,8 @@ __host__ __device__ inline Deal deal(int pairs, int l0, int u0, int l1, int u1) 
     d.after = short_u > 0 ? room(low, each) : 0;
     return d;
 }
-// A unit's fixed cost, and that of its sums through memory where a tile has several parts, in K blocks of one product
-// (0.3 us): measured.
+// A unit's fixed cost, and that of its sums through memory where a tile has several parts, in stages (0.3 us): fitted to
+// 65536 x 256 x 512, 777 x 10001 x 512 and 28701 x 8000 x 512, where halving or doubling either cost 1 to 4%.
 constexpr int64_t kUnitSteps = 4, kPartSteps = 20;
 __host__ __device__ inline int unit_steps(int k_tiles, int parts, int stages) {
     return (k_tiles + parts - 1) / parts * stages + kUnitSteps + (parts > 1 ? kPartSteps : 0);
@@ -467,7 +475,7 @@ template <typename T> __device__ __forceinline__ void finish_bias(const Params &
 #pragma unroll 2
         for (int r = 0; r < pieces; ++r) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] += __ldcg(from + (static_cast<int64_t>(r) * 8 + i) * p.col_ld);
+            for (int i = 0; i < 8; ++i) s[i] += from[(static_cast<int64_t>(r) * 8 + i) * p.col_ld];
         }
         float all = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
         if (p.db_add) all += p.db_acc[c];
@@ -1424,9 +1432,10 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
     if (!last) return;
     __threadfence();
     double a = 0.0, b = 0.0;
+    const volatile double *const sums_of = p.block_sums;  // other blocks'
     for (unsigned i = threadIdx.x; i < gridDim.x; i += kLossThreads) {
-        a += __ldcg(p.block_sums + 2 * i);
-        b += __ldcg(p.block_sums + 2 * i + 1);
+        a += sums_of[2 * i];
+        b += sums_of[2 * i + 1];
     }
     const double2 all = block_sum(a, b);
     if (threadIdx.x == 0) {
@@ -1437,9 +1446,9 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
 
 // ---- operands that TMA cannot read where they lie (fp32, rows or bases off 16 bytes): copied into rows of a multiple
 // of 8 elements, fp32 as planes.
-__global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *__restrict__ x, int64_t ldx, int64_t x_rows, const float *__restrict__ w,
-                                                               int64_t ldw, int64_t w_rows, int dim, const int64_t *__restrict__ target,
-                                                               int64_t ignore_index, unsigned *__restrict__ found) {
+__global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *x, int64_t ldx, int64_t x_rows, const float *w,
+                                                               int64_t ldw, int64_t w_rows, int dim, const int64_t *target,
+                                                               int64_t ignore_index, unsigned *found) {
     __shared__ unsigned s_found[4];
     const int lane = threadIdx.x & 31;
     if (threadIdx.x < 4) s_found[threadIdx.x] = 0u;
@@ -1483,8 +1492,8 @@ template <typename T> struct Unpacked {
 };
 template <typename T>
 __global__ void __launch_bounds__(256) linear_ce_pack_kernel(const Unpacked<T> x, const Unpacked<T> w, int dim, int64_t to_ld,
-                                                             const int32_t *__restrict__ index, const int *__restrict__ n_counted,
-                                                             const unsigned *__restrict__ found) {
+                                                             const int32_t *index, const int *n_counted,
+                                                             const unsigned *found) {
     let_next_start();
     wait_for_previous();
     // of X the rows that count, and rows of zeros up to a whole K block
@@ -1531,8 +1540,8 @@ constexpr int kTokenBlock = 256, kTokenBlocks = 4096, kTokensAlone = 2048;
 __host__ __device__ __forceinline__ int64_t block_tokens(int64_t n) {
     return (n + int64_t(kTokenBlocks) * kTokenBlock - 1) / (int64_t(kTokenBlocks) * kTokenBlock) * kTokenBlock;
 }
-__global__ void __launch_bounds__(kTokenBlock) linear_ce_count_kernel(const int64_t *__restrict__ target, int64_t n, int64_t ignore_index,
-                                                                      int32_t *__restrict__ counts) {
+__global__ void __launch_bounds__(kTokenBlock) linear_ce_count_kernel(const int64_t *target, int64_t n, int64_t ignore_index,
+                                                                      int32_t *counts) {
     let_next_start();
     wait_for_previous();
     const int64_t start = blockIdx.x * block_tokens(n), end = min(start + block_tokens(n), n);
@@ -1558,12 +1567,12 @@ __device__ __forceinline__ int block_sum(int v, int *s_warp) {
 // K block), and puts zeros where the ignored ones' loss (reduction none) and rows of d x (backward) go.  Where every token
 // counts it does nothing.  28701 tokens of 512 in bf16, 12% ignored: 20 us in all, against the 120 us by which the products
 // of the ignored ones would be longer.
-__global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uint16_t *__restrict__ x, int64_t ld, int64_t n, int dim,
-                                                                       const int64_t *__restrict__ target, int64_t ignore_index,
-                                                                       const int32_t *__restrict__ counts, int32_t *__restrict__ index,
-                                                                       int *__restrict__ n_counted, uint16_t *__restrict__ copy,
-                                                                       int64_t copy_ld, unsigned char *__restrict__ dx, int64_t dx_row_bytes,
-                                                                       float *__restrict__ loss, unsigned *__restrict__ found) {
+__global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uint16_t *x, int64_t ld, int64_t n, int dim,
+                                                                       const int64_t *target, int64_t ignore_index,
+                                                                       const int32_t *counts, int32_t *index,
+                                                                       int *n_counted, uint16_t *copy,
+                                                                       int64_t copy_ld, unsigned char *dx, int64_t dx_row_bytes,
+                                                                       float *loss, unsigned *found) {
     __shared__ int s_warp[kTokenBlock / 32], s_place[kTokenBlock];
     let_next_start();
     wait_for_previous();
@@ -1639,8 +1648,8 @@ __global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uin
 }
 
 // max |g| over the tokens that count, as bits (ordered like the numbers; a NaN is above all).
-__global__ void linear_ce_top_kernel(const float *__restrict__ grad, const int64_t *__restrict__ target, int64_t rows,
-                                     int64_t ignore_index, unsigned *__restrict__ top) {
+__global__ void linear_ce_top_kernel(const float *grad, const int64_t *target, int64_t rows,
+                                     int64_t ignore_index, unsigned *top) {
     let_next_start();
     wait_for_previous();
     unsigned best = 0u;
@@ -1772,7 +1781,7 @@ struct ForwardSpace {
 // 64 MB 1340 / 1987 us, 128 MB 1075 / 1744, 256 MB 892 / 1557, 512 MB 866 / 1533.
 constexpr int64_t kDzBytes = 256 << 20;
 
-// What a launch costs in K blocks, and the elements of a sum that is read and written once more in the time of one.
+// What a launch costs in stages, and the elements of a sum that is read and written once more in the time of one.
 constexpr int64_t kLaunchSteps = 15, kStepElements = 200000;
 // Splits the longer tiles along K where that shortens the work of the pair with the most of it: few tiles, long K.
 Deal split_and_deal(Product &x, Product &w, int stages) {

@@ -161,7 +161,9 @@ template <typename K> inline cudaError_t allow_smem(OncePerDevice &once, K kerne
 }
 
 // Programmatic dependent launch: a kernel launched by launch_after may start when the one before it in the stream says so
-// (let_next_start) or ends; before it touches memory it waits for that one's end (wait_for_previous).
+// (let_next_start) or ends; before it touches memory it waits for that one's end (wait_for_previous).  Its pointers to what
+// earlier kernels wrote are plain ones: a load through `const __restrict__` counts as one from memory that does not change
+// while the kernel runs, and the compiler may move it above the wait or send it through a cache that has old lines.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 template <typename... Args, typename... Given>

@@ -25,9 +25,10 @@ from .norm import layer_norm
 
 
 def add_layer_norm(x, r, norm):
-    """norm(x + r) for an nn.LayerNorm over the last dimension; fused on CUDA, forward and backward (norm.py), when
-    the rules of the kernel of a warp per row hold (same dtype everywhere, last dimension a multiple of 8 up to 4096),
-    torch's operators otherwise.  `norm.layer_norm` itself takes every width up to 8192."""
+    """norm(x + r) for an nn.LayerNorm over the last dimension; on CUDA one fused call, forward and backward (norm.py),
+    where the rules of bpt_add_layer_norm hold (same dtype everywhere, last dimension a multiple of 8 up to 4096), else
+    torch's operators, whose rounding of the sum x + r callers of other widths have had so far.  `norm.layer_norm`
+    itself takes every width up to 8192."""
     dim = x.size(-1)
     if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16, torch.float16) and dim % 8 == 0 and dim <= 4096
             and norm.weight is not None and norm.bias is not None and norm.weight.dtype == x.dtype

@@ -516,8 +516,8 @@ int bpt_layer_norm_backward(const void *gy, const void *x, const void *r, const 
  * float, MEAN and SUM) are what the backward reads; either may be NULL.
  *
  * Backward: grad: gradient of the loss, n floats or one.  dx: (n, dim), dw: (vocab, dim), db: (vocab), contiguous, of
- * `dtype`; each may be NULL to skip it.  The logits are computed again, in pieces of tokens x vocabulary whose gradient
- * fits the L2.  Bitwise reproducible.
+ * `dtype`; each may be NULL to skip it.  The logits are computed again, in pieces of tokens x vocabulary with at
+ * most 256 MB of logits' gradients.  Bitwise reproducible.
  *
  * The workspace sizes depend on the operands' addresses too (operands that are not 16-byte aligned are copied).  Calls
  * that may overlap need workspaces of their own; nothing in one has to be zero.  A kernel whose bounded wait ran out
