@@ -37,7 +37,7 @@
 // accumulators out every 512 of K and add these runs up in registers; the products of the first planes have an accumulator
 // of their own, so that the small ones do not lose their low bits to it.  4099 x 8003 x 300, 12% ignored, forward +
 // backward: 290 us, 1.0e-6 from the values in 64 bits (an fp32 library product: 2.1e-6); stats 50, grad 71, products 125,
-// copies 30 us.  Runs of 1024 of K would save 10 us and nearly double the error.
+// copies 30 us.  (Runs of 1024 of K were no faster.)
 #include <algorithm>
 #include <type_traits>
 
@@ -62,12 +62,12 @@ constexpr int kPairs = 74;             // pairs of blocks at most: one block per
 constexpr int kRunTiles = 8;           // fp32: K blocks added up by the tensor core before the sum is taken out
 
 enum Kind { kStats, kGrad, kProducts };
-// Shared memory: the bias of two tiles, barriers; from the next 1024-byte boundary on operand stages, and for grad a tile
-// of 32 rows x 64 columns of dZ per finishing warp, on its way out.
+// Shared memory: the bias of two tiles, barriers; from the next 1024-byte boundary on operand stages, and 4 KB of each
+// finishing warp for results on their way out (grad: 32 rows x 64 columns of dZ).
 constexpr int kOutBytes = 32 * 128;
 constexpr int kHeadBytes = 3 << 10;
-constexpr int smem_bytes(int kind) { return kHeadBytes + kStages * kStageBytes + (kind == kProducts ? 0 : kFinishWarps * kOutBytes); }
-static_assert(smem_bytes(kGrad) <= 227 * 1024, "a block's shared memory");
+constexpr int kSmemBytes = kHeadBytes + kStages * kStageBytes + kFinishWarps * kOutBytes;
+static_assert(kSmemBytes <= 227 * 1024, "a block's shared memory");
 // stats and grad, 16-bit, rows of at most kKeepTiles K blocks: the operand that stays the same from tile to tile along a
 // pair's walk is kept, one K block in each 16 KB, and the rest of the shared memory has stages of the other operand alone:
 // half the loads.  Where a pair has at least kKeepRun tiles.  65536 x 8000 x 512 forward (109 tiles a pair) kept 392 us,
@@ -237,7 +237,8 @@ __device__ __forceinline__ uint32_t take_half_finite(float &a, float &b) {
     return word;
 }
 
-// 32 neighbouring results of one row to the output: 32-byte stores where the row's address allows, else 4 elements, else one.
+// 32 neighbouring results of one row to the output: 32-byte stores where the row's address allows, else 4 elements, else one
+// (sums of a caller's own fp32 gradient that starts anywhere).
 template <typename T> __device__ __forceinline__ void store_row(T *row, int64_t row_bytes, int col, int n, const float (&v)[32]) {
     T *p = row + col;
     const uintptr_t at = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(row_bytes);
@@ -277,6 +278,26 @@ template <typename T> __device__ __forceinline__ void store_row(T *row, int64_t 
     }
 }
 
+// The same for the warp's 32 rows where rows do not start on a multiple of 4 elements: across the lanes by way of shared
+// memory (tile, 4 KB of this warp), so that the lanes write neighbouring elements.  The products of 6 x 5194 in fp16: with
+// rows of 134 elements 26 us, by single elements of 32 rows at a time 108; with rows of 136, 8 bytes a lane, 17 us, across
+// the lanes 26.
+template <typename T> __device__ __forceinline__ void store_across(T *row, bool there, int n, const float (&v)[32], uint32_t tile, int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(tile + lane * 128 + ((i ^ lane) << 2)), "f"(v[i]) : "memory");
+    __syncwarp();
+    const unsigned rows = __ballot_sync(0xffffffffu, there);
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        float one;
+        asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(one) : "r"(tile + r * 128 + ((lane ^ r) << 2)) : "memory");
+        T *const to = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r));
+        if ((rows >> r & 1u) && lane < n) to[lane] = from_acc<T>(one);
+    }
+}
+
 // How the two products of a piece are dealt to the pairs of blocks.
 struct Deal {
     int pairs, first, busy, after_busy, after;
@@ -303,9 +324,10 @@ __host__ __device__ inline Deal deal(int pairs, int l0, int u0, int l1, int u1) 
     d.after = short_u > 0 ? room(low, each) : 0;
     return d;
 }
-// A unit's fixed cost, and that of its sums through memory where a tile has several parts, in stages (0.3 us): fitted to
-// 65536 x 256 x 512, 777 x 10001 x 512 and 28701 x 8000 x 512, where halving or doubling either cost 1 to 4%.
-constexpr int64_t kUnitSteps = 4, kPartSteps = 20;
+// A unit's fixed cost, and that of its sums through memory where a tile has several parts, in stages (0.3 us): measured.
+// 65536 x 256 x 512, forward + backward: fixed costs of 2 / 4 / 8 stages 139 / 133 / 130 us, 10 / 20 / 40 for the sums
+// 132 / 133 / 137; the larger sizes moved by less than 2%.
+constexpr int64_t kUnitSteps = 8, kPartSteps = 20;
 __host__ __device__ inline int unit_steps(int k_tiles, int parts, int stages) {
     return (k_tiles + parts - 1) / parts * stages + kUnitSteps + (parts > 1 ? kPartSteps : 0);
 }
@@ -1041,22 +1063,26 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     const Product &q = p.product[work.which];
                     const int64_t in_piece = static_cast<int64_t>(m) * kBM + trow;
                     const int col = work.n0() + c0, left = q.n_ext - col;
-                    if (work.which == 0 ? in_piece < rows_here : q.row_offset + in_piece < q.row_end) {
-                        if (q.parts > 1) {
-                            store_row(q.partial + work.part * q.partial_plane + in_piece * q.acc_ld, q.acc_ld * 4, col, left, v);
+                    const bool there = work.which == 0 ? in_piece < rows_here : q.row_offset + in_piece < q.row_end;
+                    if (q.parts > 1) {
+                        if (there) store_row(q.partial + work.part * q.partial_plane + in_piece * q.acc_ld, q.acc_ld * 4, col, left, v);
+                    } else {
+                        const int64_t at = (work.which == 0 ? a0 : q.row_offset) + in_piece, row = work.which == 0 && there && index ? index[at] : at;
+                        if (q.add && there) {
+                            const float *sums = q.acc + row * q.acc_ld + col;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] += i < left ? sums[i] : 0.f;
+                        }
+                        if (!q.last) {
+                            if (there) store_row(q.acc + row * q.acc_ld, q.acc_ld * 4, col, left, v);
                         } else {
-                            const int64_t at = (work.which == 0 ? a0 : q.row_offset) + in_piece, row = work.which == 0 && index ? index[at] : at;
-                            if (q.add) {
-                                const float *sums = q.acc + row * q.acc_ld + col;
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] += i < left ? sums[i] : 0.f;
-                            }
-                            if (q.last) {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] *= work.which == 0 ? x_scale : w_scale;
-                                store_row(static_cast<T *>(q.out) + row * q.n_ext, q.n_ext * static_cast<int64_t>(sizeof(T)), col, left, v);
+                            for (int i = 0; i < 32; ++i) v[i] *= work.which == 0 ? x_scale : w_scale;
+                            T *const out = static_cast<T *>(q.out);
+                            if ((reinterpret_cast<uintptr_t>(out) | q.n_ext * sizeof(T)) % (4 * sizeof(T)) == 0) {
+                                if (there) store_row(out + row * q.n_ext, q.n_ext * static_cast<int64_t>(sizeof(T)), col, left, v);
                             } else {
-                                store_row(q.acc + row * q.acc_ld, q.acc_ld * 4, col, left, v);
+                                store_across(out + row * q.n_ext + col, there, left, v, out_tile, lane);
                             }
                         }
                     }
@@ -1778,7 +1804,7 @@ struct ForwardSpace {
 
 // Bytes of dZ kept at a time.  More than the L2 holds: the products read it at 3 TB/s, which HBM has to spare, and larger
 // pieces leave fewer pairs of blocks idle at their ends.  28701 x 8000 x 512 / 8192 x 50000 x 512, forward + backward:
-// 64 MB 1340 / 1987 us, 128 MB 1075 / 1744, 256 MB 892 / 1557, 512 MB 866 / 1533.
+// 128 MB 905 / 1731 us, 256 MB 838 / 1568, 512 MB 833 / 1545.
 constexpr int64_t kDzBytes = 256 << 20;
 
 // What a launch costs in stages, and the elements of a sum that is read and written once more in the time of one.
@@ -1921,8 +1947,8 @@ template <typename T, int kKind> int launch_ce(const Maps &m, const Params &p, i
     auto launch = [&](auto keep) -> int {
         static OncePerDevice allowed;
         auto kernel = linear_ce_kernel<T, kKind, keep.value>;
-        BPT_CUDA(allow_smem(allowed, kernel, smem_bytes(kKind)));
-        BPT_CUDA(launch_after(kernel, 2 * pairs, kThreads, smem_bytes(kKind), stream, m.a, m.b, m.c, m.d, m.e, p));
+        BPT_CUDA(allow_smem(allowed, kernel, kSmemBytes));
+        BPT_CUDA(launch_after(kernel, 2 * pairs, kThreads, kSmemBytes, stream, m.a, m.b, m.c, m.d, m.e, p));
         return BPT_OK;
     };
     if constexpr (!kIsFloat<T> && kKind != kProducts) {

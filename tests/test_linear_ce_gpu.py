@@ -265,6 +265,33 @@ def test_strides_alignment_and_shapes(dtype):
     assert float((leaf.grad.double() - ref).abs().max()) <= 96 * torch.finfo(dtype).eps * float(got[0].abs().sum(0).max())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2100, 22000, 32), (150, 700, 134), (40, 300, 72)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_that_start_anywhere(dtype, shape):
+    """The library's own entry points: outputs off 16 bytes, in one piece and in several, with nothing written around them."""
+    from bpt_b200 import _lib
+    n, vocab, dim = shape
+    x, w, b, t = inputs(n, vocab, dim, dtype, padded=0.2, seed=5)
+    _, want = check(x, w, b, t, reduction="sum")
+    L, code, p = _lib.lib(), _lib.dtype_code(dtype), lambda v: v.data_ptr()
+    loss, lse, count, grad = (torch.empty(k, device="cuda") for k in (1, n, 1, 1))
+    grad.fill_(1.0)
+    size = L.bpt_linear_ce_forward_workspace_bytes(p(x), dim, p(w), dim, n, vocab, dim, code)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    _lib.check(L.bpt_linear_ce_forward(p(x), dim, p(w), dim, p(b), p(t), IGNORE, 0.0, 2, p(loss), p(lse), p(count), n, vocab, dim, code,
+                                       p(ws), size, _lib.stream()))
+    size = L.bpt_linear_ce_backward_workspace_bytes(p(x), dim, p(w), dim, n, vocab, dim, code, 1, 1, 1)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    for off in (1, 2, 3, 4):
+        held = [torch.full((v.numel() + 16,), 7.0, dtype=dtype, device="cuda") for v in want]
+        outs = [h[off:off + v.numel()] for h, v in zip(held, want)]
+        _lib.check(L.bpt_linear_ce_backward(p(x), dim, p(w), dim, p(b), p(t), IGNORE, 0.0, 2, p(lse), p(count), p(grad), p(outs[0]),
+                                            p(outs[1]), p(outs[2]), n, vocab, dim, code, p(ws), size, _lib.stream()))
+        for h, o, v in zip(held, outs, want):
+            assert torch.equal(o.view(v.shape), v)
+            assert bool((h[:off] == 7.0).all()) and bool((h[off + v.numel():] == 7.0).all())
+
+
 def test_only_some_gradients():
     from bpt_b200.loss import linear_cross_entropy
     x, w, b, t = inputs(500, 700, 128, torch.bfloat16, padded=0.1)
