@@ -36,7 +36,7 @@
 // device.  The tensor core rounds its running sum towards zero, a bias that grows with K, so the fp32 kernels take the
 // accumulators out every 512 of K and add these runs up in registers; the products of the first planes have an accumulator
 // of their own, so that the small ones do not lose their low bits to it.  4099 x 8003 x 300, 12% ignored, forward +
-// backward: 290 us, 1.0e-6 from the values in 64 bits (an fp32 library product: 2.1e-6); stats 50, grad 71, products 125,
+// backward: 300 us, 1.0e-6 from the values in 64 bits (an fp32 library product: 2.1e-6); stats 50, grad 71, products 125,
 // copies 30 us.  (Runs of 1024 of K were no faster.)
 #include <algorithm>
 #include <type_traits>
