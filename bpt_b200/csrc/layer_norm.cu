@@ -261,8 +261,10 @@ template <typename T, int kVec, int kVecs, int kArrays, int kBlock, int kAhead> 
 
 template <typename T, int kVec, int kVecs, bool kHasR, int kBlock, int kAhead>
 __global__ void __launch_bounds__(kBlock)
-layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma, const T *__restrict__ beta, float eps,
-                  T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int64_t n_rows, int dim, int tpr) {
+layer_norm_kernel(const T *x, const T *r, const T *gamma, const T *beta, float eps,
+                  T *y, float *mean_out, float *rstd_out, int64_t n_rows, int dim, int tpr) {
+    tc5::let_next_start();
+    tc5::wait_for_previous();
     __shared__ float slots[2][16];
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kArrays = kHasR ? 2 : 1;
@@ -342,10 +344,11 @@ layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ r, const T *__r
 
 template <typename T, int kVec, int kVecs, bool kHasR, int kBlock, int kAhead>
 __global__ void __launch_bounds__(kBlock, kBlock == 256 ? 2 : 1)
-layer_norm_backward_kernel(const T *__restrict__ gy, const T *__restrict__ x, const T *__restrict__ r, const T *__restrict__ gamma,
-                           const float *__restrict__ mean_in, const float *__restrict__ rstd_in, T *__restrict__ da,
-                           float *__restrict__ partial, int64_t n_rows, int dim, int tpr) {
-    tc5::let_next_start();  // the reduction, which waits for this kernel's end
+layer_norm_backward_kernel(const T *gy, const T *x, const T *r, const T *gamma,
+                           const float *mean_in, const float *rstd_in, T *da,
+                           float *partial, int64_t n_rows, int dim, int tpr) {
+    tc5::let_next_start();
+    tc5::wait_for_previous();
     __shared__ float slots[2][2][16];
     extern __shared__ __align__(16) unsigned char smem[];  // rows ahead; at the end the sums, [rows of the block][dim]
     const int t = threadIdx.x & (tpr - 1), rows_here = kBlock / tpr, mine = threadIdx.x / tpr, step = tpr * kVec;
@@ -535,10 +538,9 @@ int launch_layer_norm(const void *x, const void *r, const void *gamma, const voi
             static tc5::OncePerDevice allowed;
             BPT_CUDA(tc5::allow_smem(allowed, kernel, R::kSmem));
             static const int resident = ln_resident(kernel, block.value, R::kSmem);  // one wave of persistent blocks
-            kernel<<<static_cast<unsigned>(std::min<int64_t>(blocks, resident)), block.value, R::kSmem, stream>>>(
-                static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(gamma), static_cast<const T *>(beta), eps,
-                static_cast<T *>(y), mean, rstd, n_rows, dim, l.tpr);
-            BPT_LAUNCH_CHECK();
+            BPT_CUDA(tc5::launch_after(kernel, static_cast<unsigned>(std::min<int64_t>(blocks, resident)), block.value, R::kSmem, stream,
+                                       static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(gamma),
+                                       static_cast<const T *>(beta), eps, static_cast<T *>(y), mean, rstd, n_rows, dim, l.tpr));
             return BPT_OK;
         };
         auto with_block = [&](auto has_r) -> int {
@@ -565,9 +567,9 @@ int launch_layer_norm_backward(const void *gy, const void *x, const void *r, con
             const size_t smem = std::max<size_t>(kAhead * kRow * (l.block / 256), partial ? sums : 0);
             static tc5::OncePerDevice allowed[2];
             BPT_CUDA(tc5::allow_smem(allowed[l.block == 512], kernel, std::max<size_t>(kAhead * kRow * (l.block / 256), 32 << 10)));
-            kernel<<<grid, l.block, smem, stream>>>(static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const T *>(r),
-                                                    static_cast<const T *>(gamma), mean, rstd, static_cast<T *>(da), partial, n_rows, dim, l.tpr);
-            BPT_LAUNCH_CHECK();
+            BPT_CUDA(tc5::launch_after(kernel, grid, l.block, smem, stream, static_cast<const T *>(gy), static_cast<const T *>(x),
+                                       static_cast<const T *>(r), static_cast<const T *>(gamma), mean, rstd, static_cast<T *>(da), partial, n_rows,
+                                       dim, l.tpr));
             return BPT_OK;
         };
         return r ? go(std::true_type()) : go(std::false_type());

@@ -1221,16 +1221,23 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     }
 }
 
+// 16 bytes that nothing reads again.
+__device__ __forceinline__ uint4 ld_stream(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // ---- forward of a handful of tokens: there is nothing to compute, the weight has to pass by once.  A warp takes eight rows
 // of W at a time, 16 bytes a lane and piece, against all the tokens (fp32 in shared memory).  Adding up over the lanes
 // halves the rows a lane has at each of the first three steps, so a lane ends with one row's logit (four lanes with the
 // same one) and keeps its own running maximum and sum; a block leaves one piece.
 template <typename T, int kTokens>
-__global__ void __launch_bounds__(256, 2) linear_ce_few_kernel(const T *__restrict__ x, int64_t ldx, const T *__restrict__ w, int64_t ldw,
-                                                            const T *__restrict__ bias, const int64_t *__restrict__ target, int n, int vocab,
-                                                            int dim, float *__restrict__ partial, float *__restrict__ z_target,
-                                                            unsigned *ticket, int *status) {
+__global__ void __launch_bounds__(256, 2) linear_ce_few_kernel(const T *x, int64_t ldx, const T *w, int64_t ldw, const T *bias,
+                                                            const int64_t *target, int n, int vocab, int dim, float *partial,
+                                                            float *z_target, unsigned *ticket, int *status) {
     let_next_start();
+    wait_for_previous();
     constexpr int kVec = 16 / sizeof(T), kFew = 8;
     extern __shared__ float xs[];  // [kTokens][dim]
     __shared__ float s_max[8][kTokens], s_sum[8][kTokens], s_z[8][kTokens];
@@ -1262,7 +1269,7 @@ __global__ void __launch_bounds__(256, 2) linear_ce_few_kernel(const T *__restri
 #pragma unroll
             for (int r = 0; r < kFew; ++r) {  // rows past the end read the last one; they are left out below
                 const int64_t v = v0 + r < vocab ? v0 + r : vocab - 1;
-                raw[r] = __ldg(reinterpret_cast<const uint4 *>(w + v * ldw + c));
+                raw[r] = ld_stream(w + v * ldw + c);
             }
             float wf[kFew][kVec];
 #pragma unroll
@@ -2011,10 +2018,9 @@ int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x
 template <typename T> int launch_few(const Shape &s, const Call &c, ForwardSpace &f, cudaStream_t stream) {
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(kFewBlocks, ce_div(s.vocab, 64)));
     auto go = [&](auto tokens) -> int {
-        linear_ce_few_kernel<T, tokens.value><<<grid, 256, tokens.value * s.dim * sizeof(float), stream>>>(
-            static_cast<const T *>(c.x), c.ldx, static_cast<const T *>(c.w), c.ldw, static_cast<const T *>(c.bias), c.target,
-            static_cast<int>(s.n), s.vocab, s.dim, f.partial, f.z_target, f.ticket, f.status);
-        BPT_LAUNCH_CHECK();
+        BPT_CUDA(launch_after(linear_ce_few_kernel<T, tokens.value>, grid, 256, tokens.value * s.dim * sizeof(float), stream,
+                              static_cast<const T *>(c.x), c.ldx, static_cast<const T *>(c.w), c.ldw, static_cast<const T *>(c.bias), c.target,
+                              static_cast<int>(s.n), s.vocab, s.dim, f.partial, f.z_target, f.ticket, f.status));
         return BPT_OK;
     };
     if (s.n <= 1) return go(std::integral_constant<int, 1>());
