@@ -83,6 +83,14 @@ def test_values_and_gradients(dim, dtype):
         check(*inputs(rows, dim, dtype, residual, seed=dim + rows))
 
 
+# widths that are even, but no multiple of 4: pieces of 2
+@pytest.mark.parametrize("dim", [6, 62, 130, 254, 370, 474, 514, 1026, 1330, 4098, 8190])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pairs(dim, dtype):
+    for rows, residual in ((1, True), (9, False), (2500 if dim < 1000 else 300, True)):
+        check(*inputs(rows, dim, dtype, residual, seed=dim + rows))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_many_rows(dtype):
     """More rows than the grid holds at once: every block loops, and the last round is ragged."""
