@@ -30,8 +30,11 @@
 // results): a half-step error of each probability, the size of the rounding of the gradients themselves.
 // fp32 operands are split into 16-bit planes, and each product of matrices is run as the products of planes whose weight
 // is above 2^-24.  Scaled by a power of two to the top of fp16's range, an operand is two fp16 planes, the second kept
-// times 2^11: 22 significant bits by rounding, down to 2^-29 of the largest number, and good to 2^-51 of that number
-// below; three products (of second planes none is needed).  That is taken where no row's largest is below 2^-24 of the matrix's largest.  Otherwise three
+// times 2^11: 22 significant bits by rounding, down to 2^-28 of the largest number, and good to 2^-51 of that number
+// below; three products (of second planes none is needed).  That is taken where no row's and no column's largest is below
+// 2^-24 of the matrix's largest: the logits' sums run along a row, the gradients' along a column, and the logits need the
+// columns, too, where the other operand's are as much smaller.  A number is then off by at most 2^-22 of itself or 2^-27 of
+// its row's and of its column's largest.  Otherwise three
 // bf16 planes (24 bits by truncation, exact, any range), six products.  A first pass over X and W finds which, on the
 // device.  The tensor core rounds its running sum towards zero, a bias that grows with K, so the fp32 kernels take the
 // accumulators out every 512 of K and add these runs up in registers; the products of the first planes have an accumulator
@@ -151,7 +154,7 @@ __device__ __forceinline__ float top_scale(unsigned bits) {
 }
 
 // How fp32 operands are split, from what the pass over X and W found: bits of the largest finite |x|, complement of the
-// bits of the smallest of the rows' largest (rows of zeros aside), the same of w.
+// bits of the smallest of its rows' and columns' largest (see linear_ce_spread_kernel), the same of w.
 struct Split {
     bool half = false;                                 // two fp16 planes
     float x = 1.f, w = 1.f, x_back = 1.f, w_back = 1.f;  // scales before the split, and their inverses
@@ -1480,42 +1483,94 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
 
 // ---- operands that TMA cannot read where they lie (fp32, rows or bases off 16 bytes): copied into rows of a multiple
 // of 8 elements, fp32 as planes.
+
+// What decides how fp32 operands are split: the largest number of each matrix, and the smallest of the largest numbers of
+// its rows and of its columns (those of zeros aside).  Rows and columns are looked at in stretches, rows of kSpreadCols
+// columns and columns of one block's rows (kSpreadRows or more), so that a block needs nothing from another: a warp brings
+// two rows in, a lane keeps the largest of its 16 columns.  Stretches are no larger than what they are part of, so this errs
+// towards three planes.  Loads past the end take the last column or row again.  W of 50000 x 512: 29 us, by itself, from memory (3.5 TB/s),
+// with 16-byte loads.
+constexpr int kSpreadCols = 512, kSpreadRows = 32, kSpreadBlocks = 148 * 4;
+template <bool kWide>
 __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *x, int64_t ldx, int64_t x_rows, const float *w,
-                                                               int64_t ldw, int64_t w_rows, int dim, const int64_t *target,
-                                                               int64_t ignore_index, unsigned *found) {
-    __shared__ unsigned s_found[4];
-    const int lane = threadIdx.x & 31;
-    if (threadIdx.x < 4) s_found[threadIdx.x] = 0u;
+                                                               int64_t ldw, int64_t w_rows, int dim, int64_t block_rows,
+                                                               int64_t x_blocks, const int64_t *target, int64_t ignore_index,
+                                                               unsigned *found) {
+    constexpr int kRowsAtOnce = 2, kPiece = kWide ? 4 : 1, kPieces = kSpreadCols / 32 / kPiece;
+    __shared__ unsigned s_found[2], s_col[8][kSpreadCols];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x < 2) s_found[threadIdx.x] = 0u;
     let_next_start();
     wait_for_previous();
-    __syncthreads();
-    unsigned best[4] = {0u, 0u, 0u, 0u};
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * 8;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < x_rows + w_rows; i += stride) {
-        const bool of_x = i < x_rows;
-        if (of_x && target[i] == ignore_index) continue;
-        const float *row = of_x ? x + i * ldx : w + (i - x_rows) * ldw;
-        unsigned top = 0u;
-        for (int c = lane; c < dim; c += 32) {
-            const unsigned bits = __float_as_uint(row[c]) & 0x7FFFFFFFu;
-            if (bits < 0x7F800000u) top = max(top, bits);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (top == 0u) continue;
-        if (of_x) {
-            best[0] = max(best[0], top);
-            best[1] = max(best[1], ~top);
-        } else {
-            best[2] = max(best[2], top);
-            best[3] = max(best[3], ~top);
-        }
-    }
-    if (lane == 0) {
+    const bool of_x = blockIdx.x < x_blocks;
+    const int64_t first = (of_x ? blockIdx.x : blockIdx.x - x_blocks) * block_rows, end = min(first + block_rows, of_x ? x_rows : w_rows);
+    const float *const from = of_x ? x : w;
+    const int64_t ld = of_x ? ldx : ldw;
+    int at[kPieces];
+    unsigned col[kPieces][kPiece], top = 0u, low = 0u;  // low: complement of the smallest
 #pragma unroll
-        for (int k = 0; k < 4; ++k) atomicMax(&s_found[k], best[k]);
+    for (int k = 0; k < kPieces; ++k) {
+        at[k] = min(static_cast<int>(blockIdx.y) * kSpreadCols + (32 * k + lane) * kPiece, dim - kPiece);
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) col[k][i] = 0u;
+    }
+    for (int64_t row0 = first + warp * kRowsAtOnce; row0 < end; row0 += 8 * kRowsAtOnce) {
+        float v[kRowsAtOnce][kPieces][kPiece];
+        bool live[kRowsAtOnce];
+#pragma unroll
+        for (int r = 0; r < kRowsAtOnce; ++r) {
+            const int64_t row = min(row0 + r, end - 1);
+            live[r] = !of_x || target[row] != ignore_index;
+            const float *const p = from + row * ld;
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                if constexpr (kWide) {
+                    const float4 piece = *reinterpret_cast<const float4 *>(p + at[k]);
+                    v[r][k][0] = piece.x;
+                    v[r][k][1] = piece.y;
+                    v[r][k][2] = piece.z;
+                    v[r][k][3] = piece.w;
+                } else {
+                    v[r][k][0] = p[at[k]];
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kRowsAtOnce; ++r) {
+            unsigned largest = 0u;
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+#pragma unroll
+                for (int i = 0; i < kPiece; ++i) {
+                    const unsigned bits = __float_as_uint(v[r][k][i]) & 0x7FFFFFFFu, finite = live[r] && bits < 0x7F800000u ? bits : 0u;
+                    col[k][i] = max(col[k][i], finite);
+                    largest = max(largest, finite);
+                }
+            }
+            largest = __reduce_max_sync(0xffffffffu, largest);
+            top = max(top, largest);
+            if (largest) low = max(low, ~largest);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) s_col[warp][(32 * k + lane) * kPiece + i] = col[k][i];
     }
     __syncthreads();
-    if (threadIdx.x < 4) atomicMax(&found[threadIdx.x], s_found[threadIdx.x]);
+    for (int c = threadIdx.x; c < kSpreadCols; c += 256) {
+        unsigned largest = 0u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) largest = max(largest, s_col[k][c]);
+        if (largest) low = max(low, ~largest);
+    }
+    low = __reduce_max_sync(0xffffffffu, low);
+    if (lane == 0) {
+        atomicMax(&s_found[0], top);
+        atomicMax(&s_found[1], low);
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) atomicMax(&found[(of_x ? 0 : 2) + threadIdx.x], s_found[threadIdx.x]);
 }
 
 template <typename T> struct Unpacked {
@@ -2000,9 +2055,13 @@ int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x
                           c.target, c.ignore_index, t.counts, t.index, t.n_counted, t.gathered, s.packed_ld, static_cast<unsigned char *>(dx),
                           static_cast<int64_t>(s.dim) * static_cast<int64_t>(sizeof(T)), loss, found));
     if constexpr (kIsFloat<T>) {
-        const int64_t found_by = std::min<int64_t>(ce_div(s.n + s.vocab, 8), 148 * 8);
-        BPT_CUDA(launch_after(linear_ce_spread_kernel, static_cast<unsigned>(found_by), 256, 0, stream, static_cast<const float *>(c.x), c.ldx, s.n,
-                              static_cast<const float *>(c.w), c.ldw, int64_t(s.vocab), s.dim, c.target, c.ignore_index, found));
+        const int64_t block_rows = std::max<int64_t>(kSpreadRows, ce_div(s.n + s.vocab, kSpreadBlocks)), x_blocks = ce_div(s.n, block_rows);
+        const dim3 grid(static_cast<unsigned>(x_blocks + ce_div(s.vocab, block_rows)), static_cast<unsigned>(ce_div(s.dim, kSpreadCols)));
+        const bool wide = s.dim % 4 == 0 && c.ldx % 4 == 0 && c.ldw % 4 == 0 &&
+                          (reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.w)) % 16 == 0;
+        BPT_CUDA(launch_after(wide ? linear_ce_spread_kernel<true> : linear_ce_spread_kernel<false>, grid, 256, 0, stream,
+                              static_cast<const float *>(c.x), c.ldx, s.n, static_cast<const float *>(c.w), c.ldw, int64_t(s.vocab), s.dim,
+                              block_rows, x_blocks, c.target, c.ignore_index, found));
     }
     if (!s.pack_x && !s.pack_w) return BPT_OK;
     const Unpacked<T> from_x{static_cast<const T *>(c.x), c.ldx, s.n, x_to, static_cast<int64_t>(align_up(s.n * s.packed_ld, 64))};

@@ -26,8 +26,8 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, lab
 
     Rows of x and weight may have any stride; other layouts are copied.  bf16 and fp16 rows that start on 16-byte
     boundaries are read where they lie, others are copied into the workspace first; fp32 operands are split there into
-    two fp16 planes, or three bf16 planes where their rows' sizes differ by more than 2^24, which keeps fp32 accuracy on
-    the tensor cores.  Forward and backward may be captured into CUDA graphs.  Runs on the current stream of x's device;
+    two fp16 planes, or three bf16 planes where the sizes of rows or of columns differ by more than 2^24, which keeps fp32
+    accuracy on the tensor cores.  Forward and backward may be captured into CUDA graphs.  Runs on the current stream of x's device;
     bad arguments raise RuntimeError."""
     if reduction not in _REDUCTIONS:
         raise RuntimeError("bpt_b200: linear_cross_entropy: reduction must be none, mean or sum")
