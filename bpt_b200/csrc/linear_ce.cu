@@ -35,7 +35,7 @@
 // 2^-24 of the matrix's largest: the logits' sums run along a row, the gradients' along a column, and the logits need the
 // columns, too, where the other operand's are as much smaller.  A number is then off by at most 2^-22 of itself or 2^-27 of
 // its row's and of its column's largest.  Otherwise three
-// bf16 planes (24 bits by truncation, exact, any range), six products.  A first pass over X and W finds which, on the
+// bf16 planes (24 bits by truncation, exact, any range above 2^-110), six products.  A first pass over X and W finds which, on the
 // device.  The tensor core rounds its running sum towards zero, a bias that grows with K, so the fp32 kernels take the
 // accumulators out every 512 of K and add these runs up in registers; the products of the first planes have an accumulator
 // of their own, so that the small ones do not lose their low bits to it.  4099 x 8003 x 300, 12% ignored, forward +
@@ -456,14 +456,25 @@ __device__ __forceinline__ float column_sum(float (&v)[32], int lane) {
 // What the gradients are multiplied by (0: of x, 1: of w, 2: of b): the one gradient of the loss, or the power of two that
 // the tokens' own ones were divided by; and what dZ and the other operand were scaled by.
 constexpr float kHalfDz = 16384.f;  // fp32 dZ in fp16 planes, as fp16 dZ
-template <typename T> __device__ __forceinline__ float result_scale(const Params &p, int which) {
+struct Scale {  // two factors, the smaller first: their product, or a result times the larger alone, may leave fp32's range
+    float first, then;
+};
+template <typename T> __device__ __forceinline__ float scaled(float v, Scale s) {
+    v *= s.first;
+    if constexpr (kIsFloat<T>) v *= s.then;
+    return v;
+}
+template <typename T> __device__ __forceinline__ Scale result_scale(const Params &p, int which) {
     float scale = p.reduction == kReduceNone ? top_scale(*p.grad_top) : *p.grad;
     if (p.reduction == kReduceMean) scale = *p.count > 0.f ? scale / *p.count : 0.f;
     if constexpr (kIsFloat<T>) {
         const Split split = read_split(p.split);
-        return !split.half ? scale : scale * (1.f / kHalfDz) * (which == 0 ? split.w_back : which == 1 ? split.x_back : 1.f);
+        if (!split.half) return Scale{scale, 1.f};
+        scale *= 1.f / kHalfDz;
+        const float back = which == 0 ? split.w_back : which == 1 ? split.x_back : 1.f;
+        return fabsf(scale) < back ? Scale{scale, back} : Scale{back, scale};
     }
-    return scale * (1.f / kDzScale<T>);
+    return Scale{scale * (1.f / kDzScale<T>), 1.f};
 }
 
 // A piece's part of the tokens that count, evenly cut where some are ignored.
@@ -485,7 +496,7 @@ __device__ __forceinline__ PieceRows piece_rows(const Params &p) {
 // that the pairs of the grad launch (fp32: the token blocks) left, added to those of earlier rows; the last are scaled
 // and stored.
 template <typename T> __device__ __forceinline__ void finish_bias(const Params &p, int rows_here, int warp, int warps, int lane) {
-    const float scale = result_scale<T>(p, 2);
+    const Scale scale = result_scale<T>(p, 2);
     const int64_t m_tiles = (rows_here + kBM - 1) / kBM, total = m_tiles * p.grad_n_tiles;
     const int pairs = pairs_used(p.grad_pairs, total);
     for (int c0 = warp * 32; c0 < p.grad_n_ext; c0 += warps * 32) {
@@ -505,7 +516,7 @@ template <typename T> __device__ __forceinline__ void finish_bias(const Params &
         float all = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
         if (p.db_add) all += p.db_acc[c];
         if (!p.db_last) p.db_acc[c] = all;
-        else static_cast<T *>(p.db)[c] = from_acc<T>(all * scale);
+        else static_cast<T *>(p.db)[c] = from_acc<T>(scaled<T>(all, scale));
     }
 }
 
@@ -795,7 +806,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         int tgt = -1;
         float row_lse = 0.f, row_l2 = 0.f, row_g = 0.f, uniform = 0.f;
         bool row_plain = true, row_skips = false;  // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0 (none there)
-        float x_scale = 1.f, w_scale = 1.f;
+        Scale x_scale{}, w_scale{};
         if constexpr (kKind == kProducts) {
             x_scale = result_scale<T>(p, 0);
             w_scale = result_scale<T>(p, 1);
@@ -881,12 +892,14 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     const int local = tgt - (p.b0 + n * kBN + c0);  // the target's place in these 32, if it is there
                     const bool here = tgt >= 0 && local >= 0 && local < 32;
                     if constexpr (kPrecise) {  // logits; probabilities from differences of logits
-                        const float2 x_back = make_float2(split.x_back, split.x_back), w_back = make_float2(split.w_back, split.w_back);
+                        // the smaller scale first: the larger one alone may take the sum past the type's range
+                        const float low = fminf(split.x_back, split.w_back), high = fmaxf(split.x_back, split.w_back);
+                        const float2 first_back = make_float2(low, low), then_back = make_float2(high, high);
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + i);
-                            const float2 lo = fma2(mul2(make_float2(v[i], v[i + 1]), x_back), w_back, make_float2(b.x, b.y));
-                            const float2 hi = fma2(mul2(make_float2(v[i + 2], v[i + 3]), x_back), w_back, make_float2(b.z, b.w));
+                            const float2 lo = fma2(mul2(make_float2(v[i], v[i + 1]), first_back), then_back, make_float2(b.x, b.y));
+                            const float2 hi = fma2(mul2(make_float2(v[i + 2], v[i + 3]), first_back), then_back, make_float2(b.z, b.w));
                             v[i] = lo.x;
                             v[i + 1] = lo.y;
                             v[i + 2] = hi.x;
@@ -1080,7 +1093,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             if (there) store_row(q.acc + row * q.acc_ld, q.acc_ld * 4, col, left, v);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] *= work.which == 0 ? x_scale : w_scale;
+                            for (int i = 0; i < 32; ++i) v[i] = scaled<T>(v[i], work.which == 0 ? x_scale : w_scale);
                             T *const out = static_cast<T *>(q.out);
                             if ((reinterpret_cast<uintptr_t>(out) | q.n_ext * sizeof(T)) % (4 * sizeof(T)) == 0) {
                                 if (there) store_row(out + row * q.n_ext, q.n_ext * static_cast<int64_t>(sizeof(T)), col, left, v);
@@ -1756,7 +1769,8 @@ __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_const
     const Product &q = p.product[which];
     const int64_t pieces = q.acc_ld / 4, rows = which == 0 ? piece_rows(p).rows : q.row_end - q.row_offset, total = rows * pieces;
     const int32_t *const index = which == 0 && *p.n_counted < p.n_rows ? p.index : nullptr;
-    const float scale = *p.status ? __int_as_float(0x7fffffff) : result_scale<T>(p, which);
+    Scale scale = result_scale<T>(p, which);
+    if (*p.status) scale.first = __int_as_float(0x7fffffff);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t in_piece = i / pieces, at = (which == 0 ? piece_rows(p).first : q.row_offset) + in_piece, row = index ? index[at] : at;
         const int col = static_cast<int>(i % pieces) * 4, left = min(4, q.n_ext - col);
@@ -1778,7 +1792,7 @@ __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_const
             if (!q.last) {
                 sums[j] = v[j];
             } else {
-                static_cast<T *>(q.out)[row * q.n_ext + col + j] = from_acc<T>(v[j] * scale);
+                static_cast<T *>(q.out)[row * q.n_ext + col + j] = from_acc<T>(scaled<T>(v[j], scale));
             }
         }
     }

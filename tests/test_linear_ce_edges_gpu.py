@@ -26,3 +26,10 @@ def test_fp32_columns_of_very_different_size(of, down):
                 x[:, c] *= 2.0 ** down
                 w[:, c] *= 2.0 ** -down
         check(x, w, b, t, smoothing=0.1)
+
+
+@pytest.mark.parametrize("up", [100, 108, 110, -100, -108, -110])
+def test_fp32_sizes_far_from_one(up):
+    """x times 2^up and w times 2^-up: the same logits."""
+    x, w, b, t = inputs(300, 500, 72, torch.float32, padded=0.1)
+    check(x * 2.0 ** up, w * 2.0 ** -up, b, t, smoothing=0.1)
