@@ -34,7 +34,8 @@
 // below; three products (of second planes none is needed).  That is taken where no row's and no column's largest is below
 // 2^-24 of the matrix's largest: the logits' sums run along a row, the gradients' along a column, and the logits need the
 // columns, too, where the other operand's are as much smaller.  A number is then off by at most 2^-22 of itself or 2^-27 of
-// its row's and of its column's largest.  Otherwise three
+// its row's and of its column's largest.  Nor may the tokens' own gradients (reduction none) lie further apart, since the
+// rows of dZ have one scale: an entry of dZ is off by at most 2^-22 of itself or 2^-50 of the largest |g|.  Otherwise three
 // bf16 planes (24 bits by truncation, exact, any range above 2^-110), six products.  A first pass over X and W finds which, on the
 // device.  The tensor core rounds its running sum towards zero, a bias that grows with K, so the fp32 kernels take the
 // accumulators out every 512 of K and add these runs up in registers; the products of the first planes have an accumulator
@@ -159,7 +160,9 @@ struct Split {
     bool half = false;                                 // two fp16 planes
     float x = 1.f, w = 1.f, x_back = 1.f, w_back = 1.f;  // scales before the split, and their inverses
 };
-constexpr int kFound = 5;  // those four, and the bits of the largest |g|
+// those four; bits of the largest finite |g|, complement of the bits of the smallest (zeros aside), both zero where all
+// tokens have one gradient
+constexpr int kFound = 6, kFoundGrad = 4;
 constexpr unsigned kSpread = 24;
 __device__ __forceinline__ Split read_split(const unsigned *found) {
     Split s;
@@ -169,6 +172,9 @@ __device__ __forceinline__ Split read_split(const unsigned *found) {
     if (found[0] != 0u && x_top == 0u) return s;
     if (found[2] != 0u && w_top == 0u) return s;
     if (!fits(x_top, x_low) || !fits(w_top, w_low)) return s;
+    // dZ's planes have one scale, too: a token's row is good to 2^-50 of the largest |g|
+    const unsigned g_top = found[kFoundGrad] >> 23, g_low = ~found[kFoundGrad + 1] >> 23;
+    if (found[kFoundGrad] != 0u && (g_low == 0u || g_top - g_low > kSpread)) return s;
     s.half = true;
     if (x_top) {
         s.x = __uint_as_float((268u - x_top) << 23);  // the largest comes to [2^14, 2^15)
@@ -1749,16 +1755,25 @@ __global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uin
     }
 }
 
-// max |g| over the tokens that count, as bits (ordered like the numbers; a NaN is above all).
+// Over the tokens that count: max |g| as bits (ordered like the numbers; a NaN is above all), and the complement of the
+// smallest that is not zero.
 __global__ void linear_ce_top_kernel(const float *grad, const int64_t *target, int64_t rows,
-                                     int64_t ignore_index, unsigned *top) {
+                                     int64_t ignore_index, unsigned *found) {
     let_next_start();
     wait_for_previous();
-    unsigned best = 0u;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows; i += static_cast<int64_t>(gridDim.x) * blockDim.x)
-        if (target[i] != ignore_index) best = max(best, __float_as_uint(grad[i]) & 0x7FFFFFFFu);
+    unsigned best = 0u, low = 0u;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        if (target[i] == ignore_index) continue;
+        const unsigned bits = __float_as_uint(grad[i]) & 0x7FFFFFFFu;
+        best = max(best, bits);
+        if (bits) low = max(low, ~bits);
+    }
     best = __reduce_max_sync(0xffffffffu, best);
-    if ((threadIdx.x & 31) == 0) atomicMax(top, best);
+    low = __reduce_max_sync(0xffffffffu, low);
+    if ((threadIdx.x & 31) == 0) {
+        atomicMax(found, best);
+        atomicMax(found + 1, low);
+    }
 }
 
 // Sums of a product's K parts (and of earlier pieces), in their order: a thread has 4 neighbouring columns.
@@ -1929,7 +1944,7 @@ struct BackwardSpace {
         status = ws.take<int>(1);
         ticket = ws.take<unsigned>(1);
         found = ws.take<unsigned>(kFound);
-        grad_top = found + kFound - 1;
+        grad_top = found + kFoundGrad;
         dz = ws.take<uint16_t>(dz_plane * s.dz_planes);
         x = s.pack_x ? ws.take<uint16_t>(s.packed(s.n)) : nullptr;
         w = s.pack_w ? ws.take<uint16_t>(s.packed(s.vocab)) : nullptr;
@@ -2056,10 +2071,11 @@ struct Tokens {  // the index and its length, on the device
 };
 
 // The index of the tokens that count; X and W as the tiles read them: where they lie (X, where tokens are ignored: from
-// the copy), or packed.  loss: where ignored tokens' zeros go, or null; dx: the same for their rows of d x.
+// the copy), or packed.  loss: where ignored tokens' zeros go, or null; dx: the same for their rows of d x; grad: the
+// backward's gradients, or null.
 template <typename T>
 int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x_to, uint16_t *w_to, unsigned *found, float *loss, void *dx,
-                     cudaStream_t stream, Operand *x, Operand *w) {
+                     const float *grad, cudaStream_t stream, Operand *x, Operand *w) {
     *x = Operand{c.x, c.ldx, 0};
     *w = Operand{c.w, c.ldw, 0};
     const unsigned blocks = static_cast<unsigned>(ce_div(s.n, block_tokens(s.n)));
@@ -2068,6 +2084,10 @@ int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x
     BPT_CUDA(launch_after(linear_ce_gather_kernel, dim3(blocks, 4), kTokenBlock, 0, stream, static_cast<const uint16_t *>(c.x), c.ldx, s.n, s.dim,
                           c.target, c.ignore_index, t.counts, t.index, t.n_counted, t.gathered, s.packed_ld, static_cast<unsigned char *>(dx),
                           static_cast<int64_t>(s.dim) * static_cast<int64_t>(sizeof(T)), loss, found));
+    if (grad && c.reduction == kReduceNone) {
+        BPT_CUDA(launch_after(linear_ce_top_kernel, static_cast<unsigned>(std::min<int64_t>(ce_div(s.n, 256), 148)), 256, 0, stream, grad,
+                              c.target, s.n, c.ignore_index, found + kFoundGrad));
+    }
     if constexpr (kIsFloat<T>) {
         const int64_t block_rows = std::max<int64_t>(kSpreadRows, ce_div(s.n + s.vocab, kSpreadBlocks)), x_blocks = ce_div(s.n, block_rows);
         const dim3 grid(static_cast<unsigned>(x_blocks + ce_div(s.vocab, block_rows)), static_cast<unsigned>(ce_div(s.dim, kSpreadCols)));
@@ -2117,7 +2137,7 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
     } else {
         Operand x, w;
         BPT_TRY(prepare_operands<T>(s, c, Tokens{f.index, f.counts, f.n_counted, f.gathered}, f.x, f.w, f.found,
-                                    c.reduction == kReduceNone ? loss : nullptr, nullptr, stream, &x, &w));
+                                    c.reduction == kReduceNone ? loss : nullptr, nullptr, nullptr, stream, &x, &w));
         Maps maps;
         BPT_TRY(make_map(&maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
         BPT_TRY(make_map(&maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));
@@ -2179,11 +2199,7 @@ int ce_backward(const Shape &s, const Call &c, BackwardSpace &f, const float *ls
     constexpr bool kHalf = kIsHalf<T>;
     constexpr bool kFloat = std::is_same<T, float>::value;
     Operand x, w;
-    BPT_TRY(prepare_operands<T>(s, c, Tokens{f.index, f.counts, f.n_counted, f.gathered}, f.x, f.w, f.found, nullptr, dx, stream, &x, &w));
-    if (c.reduction == kReduceNone) {
-        BPT_CUDA(launch_after(linear_ce_top_kernel, static_cast<unsigned>(std::min<int64_t>(ce_div(s.n, 256), 148)), 256, 0, stream, grad,
-                              c.target, s.n, c.ignore_index, f.grad_top));
-    }
+    BPT_TRY(prepare_operands<T>(s, c, Tokens{f.index, f.counts, f.n_counted, f.gathered}, f.x, f.w, f.found, nullptr, dx, grad, stream, &x, &w));
     Maps grad_maps, maps;
     BPT_TRY(make_map(&grad_maps.a, kHalf, x.at, s.n, s.dim, x.ld, s.planes, x.plane, kRows));
     BPT_TRY(make_map(&grad_maps.b, kHalf, w.at, s.vocab, s.dim, w.ld, s.planes, w.plane, kCols));

@@ -5,7 +5,8 @@ its own row and column; what is added to them stands at each test."""
 import pytest
 import torch
 
-from test_linear_ce_gpu import DTYPES, IGNORE, U, check, inputs, near
+from bpt_b200.loss import linear_cross_entropy
+from test_linear_ce_gpu import IGNORE, check, formula, inputs, near
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +34,26 @@ def test_fp32_sizes_far_from_one(up):
     """x times 2^up and w times 2^-up: the same logits."""
     x, w, b, t = inputs(300, 500, 72, torch.float32, padded=0.1)
     check(x * 2.0 ** up, w * 2.0 ** -up, b, t, smoothing=0.1)
+
+
+def off_by(x, w, t, most):
+    """What d x, d w, d b may be off by when every entry of dZ that counts is off by `most`."""
+    counted = (t != IGNORE).double().unsqueeze(1)
+    dz = most * counted.expand(-1, w.size(0))
+    return dz @ w.double().abs(), dz.t() @ x.double().abs(), dz.sum(0)
+
+
+@pytest.mark.parametrize("spread", [12, 24, 26, 40, 60, 110])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tokens_of_very_different_weight(dtype, spread):
+    """reduction none: weights from 1 to 2^-spread.  Each token's row of d x is as good as its own weight allows.  In fp32 an
+    entry of dZ may also be off by 2^-50 of the largest weight while no weight is below 2^-24 of it."""
+    x, w, b, t = inputs(300, 500, 72, dtype, padded=0.1)
+    g = 2.0 ** -(torch.arange(300, device="cuda") % (spread + 1)).float()
+    g[7] = 0.0
+    leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+    linear_cross_entropy(*leaves[:2], t, bias=leaves[2], reduction="none").backward(g)
+    want, off = formula(x, w, b, t, 0.0, "none", g)
+    more = off_by(x, w, t, 2.0 ** -50 if dtype == torch.float32 and spread <= 24 else 0.0)
+    for name, leaf, v, e, m in zip(("dx", "dw", "db"), leaves, want[1:], off[1:], more):
+        near(leaf.grad, v, e + m, name)
