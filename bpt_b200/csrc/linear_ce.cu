@@ -127,7 +127,7 @@ struct Params {
     int db_add, db_last;
     void *db;                              // of this piece, or null
     const float *count;
-    const unsigned *grad_top;              // none: bits of max |g|
+    const unsigned *grad_top;              // none: bits of the largest finite |g|
     // products: 0 = d x, 1 = d w.  The one with the longer units goes first, dealt in turn; pairs below `busy` have one
     // more of them.  The shorter units follow in runs of `after_busy` and `after` per pair.
     Product product[2];
@@ -150,7 +150,6 @@ __device__ constexpr uint32_t ce_instr(bool fp16, int n, bool a_mn, bool b_mn) {
 // Power of two at or below the largest |g| (its bits), so that g / scale is exact and below 2.
 __device__ __forceinline__ float top_scale(unsigned bits) {
     const unsigned e = bits >> 23;
-    if (e >= 255u) return __int_as_float(0x7fffffff);  // a gradient that is not finite: everything is NaN
     return e == 0u ? (bits ? 1.17549435e-38f : 1.f) : __uint_as_float(e << 23);
 }
 
@@ -1755,8 +1754,8 @@ __global__ void __launch_bounds__(kTokenBlock) linear_ce_gather_kernel(const uin
     }
 }
 
-// Over the tokens that count: max |g| as bits (ordered like the numbers; a NaN is above all), and the complement of the
-// smallest that is not zero.
+// Over the tokens that count and whose g is finite: max |g| as bits (ordered like the numbers), and the complement of the
+// smallest that is not zero.  A g that is not finite takes no part: it spoils its own row of dZ, not the others' scale.
 __global__ void linear_ce_top_kernel(const float *grad, const int64_t *target, int64_t rows,
                                      int64_t ignore_index, unsigned *found) {
     let_next_start();
@@ -1765,8 +1764,9 @@ __global__ void linear_ce_top_kernel(const float *grad, const int64_t *target, i
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         if (target[i] == ignore_index) continue;
         const unsigned bits = __float_as_uint(grad[i]) & 0x7FFFFFFFu;
+        if (bits == 0u || bits >= 0x7F800000u) continue;
         best = max(best, bits);
-        if (bits) low = max(low, ~bits);
+        low = max(low, ~bits);
     }
     best = __reduce_max_sync(0xffffffffu, best);
     low = __reduce_max_sync(0xffffffffu, low);

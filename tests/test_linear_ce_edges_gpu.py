@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from bpt_b200.loss import linear_cross_entropy
-from test_linear_ce_gpu import IGNORE, check, formula, inputs, near
+from test_linear_ce_gpu import DTYPES, IGNORE, check, formula, inputs, near
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,26 @@ def test_tokens_of_very_different_weight(dtype, spread):
     more = off_by(x, w, t, 2.0 ** -50 if dtype == torch.float32 and spread <= 24 else 0.0)
     for name, leaf, v, e, m in zip(("dx", "dw", "db"), leaves, want[1:], off[1:], more):
         near(leaf.grad, v, e + m, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_a_gradient_that_is_not_finite_spoils_its_own_row(dtype, bad):
+    """reduction none: that token's row of d x and the sums over tokens are not finite, the other rows are as without it."""
+    for n in (300, 20):  # dZ in one plane and in two
+        x, w, b, t = inputs(n, 500, 72, dtype, padded=0.1)
+        t[17] = 3
+        g = torch.linspace(0.5, 1.5, n, device="cuda")
+
+        def grads(of_17):
+            leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+            weight = g.clone()
+            weight[17] = of_17
+            linear_cross_entropy(*leaves[:2], t, bias=leaves[2], reduction="none").backward(weight)
+            return [v.grad for v in leaves]
+
+        want, got = grads(1.0), grads(bad)
+        keep = torch.arange(n, device="cuda") != 17
+        assert torch.equal(got[0][keep], want[0][keep])
+        assert not bool(torch.isfinite(got[0][17]).any())
+        assert not bool(torch.isfinite(got[1]).any()) and not bool(torch.isfinite(got[2]).any())
