@@ -1226,15 +1226,16 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     }
     if (tid == 0) {
         if (*stop) *p.status = 1;
-        if constexpr (kKind == kProducts) {  // a wait that ran out leaves results that mean nothing: the last block says so in them
+        if constexpr (kKind == kProducts) {  // a wait that ran out leaves results that mean nothing: the last block says so in
+                                             // their first elements (in those of earlier pieces, too: status outlasts them)
             __threadfence();
             if (atomicAdd(p.ticket, 1u) == gridDim.x - 1) {
                 __threadfence();
                 if (*static_cast<volatile int *>(p.status)) {
                     const T nan = from_acc<T>(__int_as_float(0x7fffffff));
                     const Product &x = p.product[0], &w = p.product[1];
-                    if (x.tiles() && x.last) static_cast<T *>(x.out)[static_cast<int64_t>(p.a0) * x.n_ext] = nan;
-                    if (w.tiles() && w.last) static_cast<T *>(w.out)[w.row_offset * w.n_ext] = nan;
+                    if (x.tiles() && x.last) *static_cast<T *>(x.out) = nan;
+                    if (w.tiles() && w.last) *static_cast<T *>(w.out) = nan;
                     if (p.spoilt) *static_cast<T *>(p.spoilt) = nan;
                 }
             }

@@ -80,3 +80,49 @@ def test_a_gradient_that_is_not_finite_spoils_its_own_row(dtype, bad):
         assert torch.equal(got[0][keep], want[0][keep])
         assert not bool(torch.isfinite(got[0][17]).any())
         assert not bool(torch.isfinite(got[1]).any()) and not bool(torch.isfinite(got[2]).any())
+
+
+@pytest.mark.parametrize("shape", [(9000, 40000, 128, torch.bfloat16), (3000, 90000, 128, torch.float16), (60000, 3000, 256, torch.float32)],
+                         ids=lambda s: "x".join(map(str, s[:3])))
+def test_a_wait_that_ran_out_marks_every_gradient(shape):
+    """A kernel whose wait ran out sets the status word, the first of the workspace; no wait runs out here, the word is set from
+    the host while the kernels of several pieces run.  Every gradient's first element is NaN then, whichever piece it was."""
+    from bpt_b200 import _lib
+    n, vocab, dim, dtype = shape
+    x, w, b, t = inputs(n, vocab, dim, dtype, padded=0.1)
+    t[0] = IGNORE  # the first row of d x is written by no product
+    L, code, p = _lib.lib(), _lib.dtype_code(dtype), lambda v: v.data_ptr()
+    loss, lse, count = (torch.empty(k, device="cuda") for k in (1, n, 1))
+    grad = torch.ones(1, device="cuda")
+    size = L.bpt_linear_ce_forward_workspace_bytes(p(x), dim, p(w), dim, n, vocab, dim, code)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    _lib.check(L.bpt_linear_ce_forward(p(x), dim, p(w), dim, p(b), p(t), IGNORE, 0.0, 1, p(loss), p(lse), p(count), n, vocab, dim, code,
+                                       p(ws), size, _lib.stream()))
+    size = L.bpt_linear_ce_backward_workspace_bytes(p(x), dim, p(w), dim, n, vocab, dim, code, 1, 1, 1)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    assert ws.data_ptr() % 256 == 0
+    outs = [torch.empty(s, dtype=dtype, device="cuda") for s in ((n, dim), (vocab, dim), (vocab,))]
+    word, one = ws[:4].view(torch.int32), torch.ones(1, dtype=torch.int32).pin_memory()
+    side, end = torch.cuda.Stream(), torch.cuda.Event()
+
+    def backward():
+        _lib.check(L.bpt_linear_ce_backward(p(x), dim, p(w), dim, p(b), p(t), IGNORE, 0.0, 1, p(lse), p(count), p(grad), p(outs[0]),
+                                            p(outs[1]), p(outs[2]), n, vocab, dim, code, p(ws), size, _lib.stream()))
+
+    backward()  # warm
+    torch.cuda.synchronize()
+    assert all(bool(torch.isfinite(v).all()) for v in outs)
+    for _ in range(50):  # again if the host was held up while the kernels ran
+        backward()
+        end.record()
+        sent = 0
+        with torch.cuda.stream(side):  # copies need no SM, which the kernels hold
+            while not end.query():
+                word.copy_(one, non_blocking=True)
+                sent += 1
+        torch.cuda.synchronize()
+        if sent > 10:
+            break
+    assert sent > 10
+    for name, v in zip(("dx", "dw", "db"), outs):
+        assert bool(torch.isnan(v.view(-1)[0])), name
