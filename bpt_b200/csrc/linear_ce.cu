@@ -1447,7 +1447,7 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
                 const bool known = target >= 0 && target < p.vocab;
                 const float zt = known ? p.z_target[row] : __int_as_float(0x7fffffff);
                 loss = lse - zt;
-                if (p.smoothing != 0.f) loss += p.smoothing * (zt - z / static_cast<float>(p.vocab));
+                if (p.smoothing != 0.f) loss = (1.f - p.smoothing) * loss + p.smoothing * (lse - z / static_cast<float>(p.vocab));
             }
             if (*p.status) loss = __int_as_float(0x7fffffff);
             if (p.lse) p.lse[token] = lse;

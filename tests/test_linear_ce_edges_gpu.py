@@ -126,3 +126,26 @@ def test_a_wait_that_ran_out_marks_every_gradient(shape):
     assert sent > 10
     for name, v in zip(("dx", "dw", "db"), outs):
         assert bool(torch.isnan(v.view(-1)[0])), name
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 5, 300])
+def test_smoothing_over_classes_that_are_masked(n, dtype):
+    """A bias of -inf and label smoothing: the loss is infinite (not NaN), also of a token whose target is masked, and the
+    gradients, which need no logarithm, are the formula's."""
+    x, w, b, t = inputs(n, 400, 64, dtype)
+    b[3] = b[200] = -float("inf")
+    t[0] = 3
+    t[1:] = t[1:].clamp(min=4)
+    t[t == 200] = 201
+    for smoothing, row0, rows in ((0.0, float("inf"), None), (0.1, float("inf"), float("inf"))):
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+        loss = linear_cross_entropy(*leaves[:2], t, bias=leaves[2], label_smoothing=smoothing, reduction="none")
+        with torch.no_grad():
+            assert torch.equal(loss, linear_cross_entropy(x, w, t, bias=b, label_smoothing=smoothing, reduction="none"))
+        assert float(loss[0].detach()) == row0
+        assert bool(torch.isfinite(loss[1:]).all()) if rows is None else bool((loss[1:] == rows).all())
+        loss.backward(torch.ones_like(loss))
+        want, off = formula(x, w, b, t, smoothing, "none", torch.ones(n, device="cuda"))
+        for name, leaf, v, e in zip(("dx", "dw", "db"), leaves, want[1:], off[1:]):
+            near(leaf.grad, v, e, name)
