@@ -112,11 +112,11 @@ struct Params {
     int vocab;
     const void *bias;
     const int64_t *target;
-    float *partial, *z_target;             // stats: [piece][max, sum, sum of z][row], z of the target
+    float *partial, *z_target;             // stats: [piece][max, sum, part of mean z][row], z of the target
     unsigned *ticket;                      // zeroed by stats and grad for what follows them: its last block speaks for all
     int starts;                            // the call's first kernel: status is cleared
     void *spoilt;                          // db, where a wait that ran out is made known when its kernel has written it
-    int smoothed;
+    float mean_of;                         // stats: 1 / vocab where the mean of a row's logits is wanted, else 0
     const float *lse, *grad;               // grad
     float smoothing;
     int reduction;
@@ -185,6 +185,9 @@ __device__ __forceinline__ Split read_split(const unsigned *found) {
     }
     return s;
 }
+
+// What is larger than this in size is not in fp32's range when multiplied by log2(e).
+constexpr float kMostForExp = 2.3e38f;
 
 // The first tile of pair c when t tiles are dealt in order to g pairs; the pair that has tile i.
 __host__ __device__ __forceinline__ int64_t first_tile(int64_t t, int g, int c) { return t * c / g; }
@@ -810,7 +813,9 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         float run_max = -INFINITY, run_sum = 0.f, run_z = 0.f;
         int tgt = -1;
         float row_lse = 0.f, row_l2 = 0.f, row_g = 0.f, uniform = 0.f;
-        bool row_plain = true, row_skips = false;  // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0 (none there)
+        // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0 (none there); some lse times log2(e)
+        // is not in fp32's range
+        bool row_plain = true, row_skips = false, row_far = false;
         Scale x_scale{}, w_scale{};
         if constexpr (kKind == kProducts) {
             x_scale = result_scale<T>(p, 0);
@@ -850,7 +855,6 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (col < p.n_ext) {
                     const int64_t v = p.b0 + col;
                     b = p.bias ? to_acc<T>(static_cast<const T *>(p.bias)[v]) : 0.f;
-                    if constexpr (!kPrecise) b *= kLog2e;
                 }
                 s_bias[parity * kBN + tid] = b;
                 parity ^= 1;
@@ -876,6 +880,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         row_skips = __any_sync(0xffffffffu, row_g == 0.f);
                         row_plain = p.smoothing == 0.f && __all_sync(0xffffffffu, row_g == kDzScale<T> || row_g == 0.f);
                         row_l2 = row_lse * kLog2e - (row_plain && kIsHalf<T> ? 14.f : 0.f);
+                        row_far = __any_sync(0xffffffffu, fabsf(row_lse) > kMostForExp);
                     }
                 }
                 if constexpr (kKeepSums) {
@@ -896,7 +901,8 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if constexpr (kKind != kProducts) {
                     const int local = tgt - (p.b0 + n * kBN + c0);  // the target's place in these 32, if it is there
                     const bool here = tgt >= 0 && local >= 0 && local < 32;
-                    if constexpr (kPrecise) {  // logits; probabilities from differences of logits
+                    // logits.  Not times log2(e), which would take a bias near the type's lowest number to -inf.
+                    if constexpr (kPrecise) {
                         // the smaller scale first: the larger one alone may take the sum past the type's range
                         const float low = fminf(split.x_back, split.w_back), high = fmaxf(split.x_back, split.w_back);
                         const float2 first_back = make_float2(low, low), then_back = make_float2(high, high);
@@ -910,58 +916,56 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             v[i + 2] = hi.x;
                             v[i + 3] = hi.y;
                         }
-                    } else {  // logits times log2(e)
+                    } else {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + i);
-                            const float2 lo = fma2(make_float2(v[i], v[i + 1]), make_float2(kLog2e, kLog2e), make_float2(b.x, b.y));
-                            const float2 hi = fma2(make_float2(v[i + 2], v[i + 3]), make_float2(kLog2e, kLog2e), make_float2(b.z, b.w));
+                            const float2 lo = add2(make_float2(v[i], v[i + 1]), make_float2(b.x, b.y));
+                            const float2 hi = add2(make_float2(v[i + 2], v[i + 3]), make_float2(b.z, b.w));
                             v[i] = lo.x;
                             v[i + 1] = lo.y;
                             v[i + 2] = hi.x;
                             v[i + 3] = hi.y;
                         }
                     }
-                    constexpr float kUnit = kPrecise ? 1.f : kLn2;  // of v, in logits
+                    const float2 log2e = make_float2(kLog2e, kLog2e);
                     if constexpr (kKind == kStats) {
-                        if (p.smoothed) {
+                        if (p.mean_of != 0.f) {  // parts of the mean: several of the lowest numbers have no sum
                             if (cols == kBN) {
-                                float2 total = make_float2(0.f, 0.f);
+                                float2 mean = make_float2(0.f, 0.f);
 #pragma unroll
-                                for (int i = 0; i < 32; i += 2) total = add2(total, make_float2(v[i], v[i + 1]));
-                                run_z += (total.x + total.y) * kUnit;
+                                for (int i = 0; i < 32; i += 2) mean = fma2(make_float2(v[i], v[i + 1]), make_float2(p.mean_of, p.mean_of), mean);
+                                run_z += mean.x + mean.y;
                             } else {
-                                float total = 0.f;
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) total += c0 + i < cols ? v[i] : 0.f;
-                                run_z += total * kUnit;
+                                for (int i = 0; i < 32; ++i) run_z += c0 + i < cols ? v[i] * p.mean_of : 0.f;
                             }
                         }
                         if (here) {
                             float zt = 0.f;
 #pragma unroll
                             for (int i = 0; i < 32; ++i) zt = i == local ? v[i] : zt;
-                            p.z_target[a0 + static_cast<int64_t>(m) * kBM + trow] = zt * kUnit;
+                            p.z_target[a0 + static_cast<int64_t>(m) * kBM + trow] = zt;
                         }
                         // Sums of exp(v - run_max), where run_max is a number near the largest so far: it moves only when
                         // a sum gets large (or is not a number), which saves looking for the maximum of every 32.
                         float2 sum = make_float2(0.f, 0.f);
                         if constexpr (!kPrecise) {
-                            const float2 from = make_float2(-run_max, -run_max);
+                            const float2 from = make_float2(-run_max * kLog2e, -run_max * kLog2e);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                const float2 d = add2(make_float2(v[i], v[i + 1]), from);
+                                const float2 d = fma2(make_float2(v[i], v[i + 1]), log2e, from);
                                 sum = add2(sum, make_float2(ex2(d.x), ex2(d.y)));
                             }
                         }
                         float more = sum.x + sum.y;
-                        if (kPrecise || !(more < 1e18f) || run_max == -INFINITY) {
+                        if (kPrecise || !(more < 1e18f) || !(fabsf(run_max) <= kMostForExp)) {
                             float tops[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
                             for (int i = 4; i < 32; ++i) tops[i & 3] = fmaxf(tops[i & 3], v[i]);
                             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                             if (top > run_max) {
-                                run_sum *= ex2((run_max - top) * (kPrecise ? kLog2e : 1.f));
+                                run_sum *= ex2((run_max - top) * kLog2e);
                                 run_max = top;
                             }
                             const float m0 = run_max == -INFINITY ? 0.f : run_max;
@@ -969,8 +973,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             sum = make_float2(0.f, 0.f);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                float2 d = add2(make_float2(v[i], v[i + 1]), from);
-                                if constexpr (kPrecise) d = mul2(d, make_float2(kLog2e, kLog2e));
+                                const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), from), log2e);
                                 sum = add2(sum, make_float2(ex2(d.x), ex2(d.y)));
                             }
                             more = sum.x + sum.y;
@@ -983,18 +986,23 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             const float2 from = make_float2(-row_lse, -row_lse), g2 = make_float2(row_g, row_g), u2 = make_float2(-uniform, -uniform);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), from), make_float2(kLog2e, kLog2e));
+                                const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), from), log2e);
                                 const float2 dz = fma2(make_float2(ex2(d.x), ex2(d.y)), g2, u2);
                                 v[i] = dz.x;
                                 v[i + 1] = dz.y;
                             }
                         } else {
-                            const float2 from = make_float2(-row_l2, -row_l2);
+                            if (!row_far) {
+                                const float2 from = make_float2(-row_l2, -row_l2);
 #pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                const float2 d = add2(make_float2(v[i], v[i + 1]), from);
-                                v[i] = ex2(d.x);
-                                v[i + 1] = ex2(d.y);
+                                for (int i = 0; i < 32; i += 2) {
+                                    const float2 d = fma2(make_float2(v[i], v[i + 1]), log2e, from);
+                                    v[i] = ex2(d.x);
+                                    v[i + 1] = ex2(d.y);
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) v[i] = ex2((v[i] - row_lse) * kLog2e + (row_plain && kIsHalf<T> ? 14.f : 0.f));
                             }
                             if (!row_plain) {
                                 const float2 g2 = make_float2(row_g, row_g), u2 = make_float2(-uniform, -uniform);
@@ -1272,6 +1280,7 @@ __global__ void __launch_bounds__(256, 2) linear_ce_few_kernel(const T *x, int64
     for (int i = threadIdx.x; i < kTokens * dim; i += 256) xs[i] = i / dim < n ? to_acc<T>(x[i / dim * ldx + i % dim]) : 0.f;
     __syncthreads();
     float top[kTokens], sum[kTokens], total[kTokens];
+    const float mean_of = 1.f / static_cast<float>(vocab);
     int tgt[kTokens];
 #pragma unroll
     for (int k = 0; k < kTokens; ++k) {
@@ -1346,7 +1355,7 @@ __global__ void __launch_bounds__(256, 2) linear_ce_few_kernel(const T *x, int64
                 top[k] = z;
             }
             sum[k] += ex2((z - (top[k] == -INFINITY ? 0.f : top[k])) * kLog2e);
-            total[k] += z;
+            total[k] = fmaf(z, mean_of, total[k]);
             if (tgt[k] == v && (lane & 3) == 0) z_target[k] = z;
         }
     }
@@ -1403,7 +1412,7 @@ struct LossParams {
     int n_tiles, pairs, vocab, reduction;
     int pieces;            // of every row, or 0: what the tiles' dealing gives
     int64_t rows_padded;   // between a piece's numbers, or 0: whole tiles of the rows
-    float smoothing, unit;  // unit: of a piece's maximum, in logits
+    float smoothing;
     float *loss, *lse, *count;
     double *block_sums;  // [blocks][sum, count]
     unsigned *ticket;
@@ -1431,7 +1440,7 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
         for (int i = lane; i < pieces; i += kLanes) {
             const float *at = p.partial + static_cast<int64_t>(i) * 3 * rows_padded + row;
             const float s = at[rows_padded];
-            if (!(s == 0.f)) sum += s * exp2f((at[0] - top) * (p.unit * kLog2e));  // a piece without any finite logit has sum 0
+            if (!(s == 0.f)) sum += s * exp2f((at[0] - top) * kLog2e);  // a piece without any finite logit has sum 0
             z += at[2 * rows_padded];
         }
 #pragma unroll
@@ -1440,14 +1449,14 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
             z += __shfl_xor_sync(0xffffffffu, z, o);
         }
         if (lane == 0) {
-            const float lse = top * p.unit + logf(sum);
+            const float lse = top + logf(sum);
             const int64_t token = n_rows < p.n_rows ? p.index[row] : row, target = p.target[token];
             counted = target != p.ignore_index;
             if (counted) {
                 const bool known = target >= 0 && target < p.vocab;
                 const float zt = known ? p.z_target[row] : __int_as_float(0x7fffffff);
                 loss = lse - zt;
-                if (p.smoothing != 0.f) loss = (1.f - p.smoothing) * loss + p.smoothing * (lse - z / static_cast<float>(p.vocab));
+                if (p.smoothing != 0.f) loss = (1.f - p.smoothing) * loss + p.smoothing * (lse - z);
             }
             if (*p.status) loss = __int_as_float(0x7fffffff);
             if (p.lse) p.lse[token] = lse;
@@ -2134,7 +2143,6 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
         BPT_TRY(launch_few<T>(s, c, f, stream));
         l.pieces = static_cast<int>(std::min<int64_t>(kFewBlocks, ce_div(s.vocab, 64)));
         l.rows_padded = s.n;
-        l.unit = 1.f;
     } else {
         Operand x, w;
         BPT_TRY(prepare_operands<T>(s, c, Tokens{f.index, f.counts, f.n_counted, f.gathered}, f.x, f.w, f.found,
@@ -2165,11 +2173,10 @@ template <typename T> int ce_forward(const Shape &s, const Call &c, ForwardSpace
         p.z_target = f.z_target;
         p.ticket = f.ticket;
         p.starts = 1;
-        p.smoothed = c.smoothing != 0.f;
+        p.mean_of = c.smoothing != 0.f ? 1.f / static_cast<float>(s.vocab) : 0.f;
         BPT_TRY((launch_ce<T, kStats>(maps, p, pairs, stream)));
         l.n_counted = f.n_counted;
         l.index = f.index;
-        l.unit = kIsFloat<T> ? 1.f : kLn2;
     }
     l.partial = f.partial;
     l.z_target = f.z_target;

@@ -149,3 +149,35 @@ def test_smoothing_over_classes_that_are_masked(n, dtype):
         want, off = formula(x, w, b, t, smoothing, "none", torch.ones(n, device="cuda"))
         for name, leaf, v, e in zip(("dx", "dw", "db"), leaves, want[1:], off[1:]):
             near(leaf.grad, v, e, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 5, 300])
+def test_classes_masked_with_the_lowest_number(n, dtype):
+    """The bias of masked classes is the type's lowest number, whole blocks of classes among them.  Losses stay finite, and
+    gradients are those of a bias of -inf.  Losses of ordinary tokens without smoothing, too; the others are sums of at most 432 additions,
+    so off by 2^-15 of themselves."""
+    x, w, b, t = inputs(n, 400, 64, dtype)
+    masked = torch.zeros(400, dtype=torch.bool, device="cuda")
+    masked[:64] = masked[200:300] = masked[399] = True
+    t = t % 90 + 70
+    t[0] = 3
+    low, none = b.clone(), b.clone()
+    low[masked], none[masked] = torch.finfo(dtype).min, -float("inf")
+    z = x.double() @ w.double().t() + low.double()
+    for smoothing in (0.0, 0.1):
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, low)]
+        loss = linear_cross_entropy(*leaves[:2], t, bias=leaves[2], label_smoothing=smoothing, reduction="none")
+        loss.backward(torch.ones_like(loss))
+        exact = torch.nn.functional.cross_entropy(z, t, label_smoothing=smoothing, reduction="none")
+        assert bool(((loss.detach().double() - exact).abs() <= 2.0 ** -15 * exact.abs()).all())
+        want, off = formula(x, w, none, t, smoothing, "none", torch.ones(n, device="cuda"))
+        if not smoothing and n > 1:
+            near(loss.detach()[1:], want[0][1:], off[0][1:], "loss")
+        for name, leaf, v, e in zip(("dx", "dw", "db"), leaves, want[1:], off[1:]):
+            near(leaf.grad, v, e, name)
+    for smoothing in (0.0, 0.1):  # nothing is left
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, torch.full_like(b, torch.finfo(dtype).min))]
+        loss = linear_cross_entropy(*leaves[:2], t, bias=leaves[2], label_smoothing=smoothing, reduction="none")
+        loss.backward(torch.ones_like(loss))
+        assert bool(torch.isfinite(loss).all()) and all(bool(torch.isfinite(v.grad).all()) for v in leaves)
