@@ -41,6 +41,11 @@ at::Tensor or_undefined(const OptTensor &t) { return t.has_value() ? *t : at::Te
 OptTensor if_defined(const at::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 at::Tensor contiguous(const at::Tensor &t) { return t.defined() ? t.contiguous() : t; }
 bool wants_grad(const at::Tensor &t) { return t.defined() && t.requires_grad(); }
+// There are no forward-mode derivatives.  The autograd nodes would say so, but calls without a node would drop the tangent.
+void refuse_tangents(const char *name, std::initializer_list<const at::Tensor *> inputs) {
+    for (const at::Tensor *t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "bpt_b200: ", name, " has no forward-mode derivative");
+}
 
 // Results of a backward that has no derivative of its own: asking for one is an error, as with once_differentiable.
 variable_list once(variable_list grads, const char *what) {
@@ -106,6 +111,7 @@ at::Tensor layer_norm(const at::Tensor &x_, const OptTensor &weight_, const OptT
     dtype_code(x_, "layer_norm");
     TORCH_CHECK(x_.dim() >= 1 && x_.size(-1) >= 1 && x_.size(-1) <= kMaxDim, "bpt_b200: layer_norm: the last dimension must be in [1, ", kMaxDim, "]");
     const at::Tensor weight_in = or_undefined(weight_), bias_in = or_undefined(bias_), residual_in = or_undefined(residual_);
+    refuse_tangents("layer_norm", {&x_, &weight_in, &bias_in, &residual_in});
     auto check = [&](const at::Tensor &t, const char *name, at::IntArrayRef shape) {
         TORCH_CHECK(!t.defined() || (t.device() == x_.device() && t.scalar_type() == x_.scalar_type() && t.sizes() == shape),
                     "bpt_b200: layer_norm: ", name, " must be a ", x_.scalar_type(), " tensor of shape ", shape, " on ", x_.device());
@@ -206,6 +212,7 @@ at::Tensor linear_cross_entropy(const at::Tensor &x_, const at::Tensor &weight, 
                 x_.scalar_type(), " tensor on ", x_.device());
     TORCH_CHECK(weight.size(0) <= (1 << 30) && weight.size(1) <= (1 << 20), "bpt_b200: ", name, ": weight is too large");
     const at::Tensor bias_in = or_undefined(bias_);
+    refuse_tangents(name, {&x_, &weight, &bias_in});
     TORCH_CHECK(!bias_in.defined() || (bias_in.scalar_type() == x_.scalar_type() && bias_in.device() == x_.device() && bias_in.dim() == 1 &&
                                        bias_in.size(0) == weight.size(0)),
                 "bpt_b200: ", name, ": bias must be a ", x_.scalar_type(), " tensor of shape [", weight.size(0), "] on ", x_.device());

@@ -14,7 +14,8 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
-    """cross_entropy(x @ weight.T + bias, target) without the logits in memory; differentiable once in x, weight, bias.
+    """cross_entropy(x @ weight.T + bias, target) without the logits in memory; differentiable once in x, weight, bias (a
+    forward-mode tangent raises NotImplementedError).
 
     x: (..., dim) and weight: (vocab, dim), CUDA tensors of one dtype (fp32, bf16, fp16); bias: (vocab,) of that dtype
     or None; target: int64 of x's leading shape.  Returns fp32: a scalar, or target's shape for reduction="none".

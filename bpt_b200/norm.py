@@ -10,7 +10,8 @@ from . import train_extension
 
 
 def layer_norm(x, weight, bias, eps=1e-5, residual=None):
-    """LayerNorm(x + residual) over the last dimension; differentiable once in x, residual, weight and bias.
+    """LayerNorm(x + residual) over the last dimension; differentiable once in x, residual, weight and bias (a forward-mode
+    tangent raises NotImplementedError).
 
     x: (..., dim) CUDA tensor, fp32, bf16 or fp16, dim from 1 to 8192; weight, bias: (dim,) of x's dtype or None (ones,
     zeros); residual: of x's shape and dtype or None.  Any strides (non-contiguous inputs are copied).  The sum
