@@ -39,7 +39,9 @@ at::Tensor workspace(size_t bytes, const at::Tensor &like) {
 at::Tensor or_undefined(const OptTensor &t) { return t.has_value() ? *t : at::Tensor(); }
 // An autograd node takes tensors that may be missing as optionals; its edges count the ones that are there.
 OptTensor if_defined(const at::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-at::Tensor contiguous(const at::Tensor &t) { return t.defined() ? t.contiguous() : t; }
+// A view whose memory holds the negatives (the imaginary part of a conjugate) is written out: kernels read memory.
+at::Tensor as_stored(const at::Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+at::Tensor contiguous(const at::Tensor &t) { return t.defined() ? as_stored(t).contiguous() : t; }
 bool wants_grad(const at::Tensor &t) { return t.defined() && t.requires_grad(); }
 // There are no forward-mode derivatives.  The autograd nodes would say so, but calls without a node would drop the tangent.
 void refuse_tangents(const char *name, std::initializer_list<const at::Tensor *> inputs) {
@@ -87,7 +89,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const at::Tensor &x = saved[0], &residual = saved[1], &weight = saved[2], &mean_rstd = saved[3];
         const c10::cuda::CUDAGuard guard(x.device());
         const int64_t dim = x.size(-1), rows = x.numel() / dim;
-        const at::Tensor gy = grad[0].contiguous();
+        const at::Tensor gy = contiguous(grad[0]);
         size_t edge = 0;
         auto needed = [&](bool there) { return there && ctx->needs_input_grad(edge++); };
         const bool need_x = needed(true), need_r = needed(residual.defined()), need_w = needed(weight.defined());
@@ -119,7 +121,7 @@ at::Tensor layer_norm(const at::Tensor &x_, const OptTensor &weight_, const OptT
     check(weight_in, "weight", x_.sizes().slice(x_.dim() - 1));
     check(bias_in, "bias", x_.sizes().slice(x_.dim() - 1));
     check(residual_in, "residual", x_.sizes());
-    const at::Tensor x = x_.contiguous(), weight = contiguous(weight_in), bias = contiguous(bias_in), residual = contiguous(residual_in);
+    const at::Tensor x = contiguous(x_), weight = contiguous(weight_in), bias = contiguous(bias_in), residual = contiguous(residual_in);
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual) || wants_grad(weight) || wants_grad(bias)))
         return LayerNorm::apply(x, if_defined(residual), if_defined(weight), if_defined(bias), eps);
     return norm_forward(x, residual, weight, bias, eps, nullptr);
@@ -185,7 +187,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         const Rows x(saved[0]), w(saved[1]);
         const int64_t n = x.t.size(0);
         const int dim = static_cast<int>(x.t.size(1)), vocab = static_cast<int>(w.t.size(0)), dtype = dtype_code(x.t, "linear_cross_entropy");
-        const at::Tensor grad = grads[0].contiguous();
+        const at::Tensor grad = contiguous(grads[0]);
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bias.defined() && ctx->needs_input_grad(2);
         at::Tensor dx, dw, db;
         if (need_x) dx = at::empty({n, dim}, x.t.options());
@@ -201,9 +203,10 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     }
 };
 
-at::Tensor linear_cross_entropy(const at::Tensor &x_, const at::Tensor &weight, const at::Tensor &target_, const OptTensor &bias_,
+at::Tensor linear_cross_entropy(const at::Tensor &x_, const at::Tensor &weight_, const at::Tensor &target_, const OptTensor &bias_,
                                 int64_t ignore_index, double smoothing, int64_t reduction) {
     const char *const name = "linear_cross_entropy";
+    const at::Tensor weight = as_stored(weight_);
     TORCH_CHECK(x_.is_cuda(), "bpt_b200: expected a CUDA tensor (there is no CPU path)");
     dtype_code(x_, name);
     TORCH_CHECK(weight.dim() == 2 && x_.dim() >= 1 && weight.size(0) >= 1 && weight.size(1) >= 1 && x_.size(-1) == weight.size(1), "bpt_b200: ",
@@ -219,8 +222,8 @@ at::Tensor linear_cross_entropy(const at::Tensor &x_, const at::Tensor &weight, 
     TORCH_CHECK(target_.scalar_type() == at::kLong && target_.device() == x_.device() && target_.sizes() == x_.sizes().slice(0, x_.dim() - 1),
                 "bpt_b200: ", name, ": target must be an int64 tensor of shape ", x_.sizes().slice(0, x_.dim() - 1), " on ", x_.device());
     TORCH_CHECK(smoothing >= 0.0 && smoothing <= 1.0, "bpt_b200: ", name, ": label_smoothing must be in [0, 1]");
-    const at::Tensor x = x_.dim() == 2 ? x_ : x_.reshape({x_.numel() / x_.size(-1), x_.size(-1)});
-    const at::Tensor target = target_.reshape({-1}).contiguous(), bias = contiguous(bias_in);
+    const at::Tensor x = as_stored(x_.dim() == 2 ? x_ : x_.reshape({x_.numel() / x_.size(-1), x_.size(-1)}));
+    const at::Tensor target = contiguous(target_.reshape({-1})), bias = contiguous(bias_in);
     at::Tensor loss;
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(bias)))
         loss = LinearCrossEntropy::apply(x, weight, if_defined(bias), target, ignore_index, smoothing, reduction);
