@@ -14,26 +14,72 @@ BinaryPartitionTransformer.forward (modules/model.py:240-280): token embedding o
 zeros on span nodes, `n_layers` blocks over all nodes, log-softmax generator on the leaves.
 Projections, LayerNorm and the FFN are torch operators, as in the reference.
 """
+import functools
 import math
 
 import torch
 import torch.nn as nn
 
+from . import _lib, train_extension
 from .attention import bpt_attention
 from .loss import linear_cross_entropy
 from .norm import layer_norm
 
 
+@functools.lru_cache(maxsize=None)
+def _has_train_extension():
+    try:
+        train_extension()
+    except ImportError:
+        return False
+    return True
+
+
+class _AddLayerNorm(torch.autograd.Function):
+    """norm.layer_norm's library calls through ctypes, for builds without the torch extensions (build.py --no-torch-ext):
+    the same kernels and results, more host time."""
+
+    @staticmethod
+    def forward(ctx, x, r, weight, bias, eps):
+        rows, dim = x.numel() // x.size(-1), x.size(-1)
+        y, mean_rstd = torch.empty_like(x), torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        with torch.cuda.device(x.device):
+            _lib.check(_lib.lib().bpt_layer_norm_forward(
+                x.data_ptr(), r.data_ptr(), weight.data_ptr(), bias.data_ptr(), float(eps), y.data_ptr(), mean_rstd[0].data_ptr(),
+                mean_rstd[1].data_ptr(), rows, dim, _lib.dtype_code(x.dtype), _lib.stream()))
+        ctx.save_for_backward(x, r, weight, mean_rstd)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, r, weight, mean_rstd = ctx.saved_tensors
+        rows, dim = x.numel() // x.size(-1), x.size(-1)
+        gy = gy.contiguous()
+        da, dw, db = torch.empty_like(x), torch.empty_like(weight), torch.empty_like(weight)
+        with torch.cuda.device(x.device):
+            ws = _lib.workspace(_lib.lib().bpt_layer_norm_backward_workspace_bytes(rows, dim), x.device)
+            _lib.check(_lib.lib().bpt_layer_norm_backward(
+                gy.data_ptr(), x.data_ptr(), r.data_ptr(), weight.data_ptr(), mean_rstd[0].data_ptr(), mean_rstd[1].data_ptr(),
+                da.data_ptr(), dw.data_ptr(), db.data_ptr(), rows, dim, _lib.dtype_code(x.dtype), ws.data_ptr(), ws.numel(),
+                _lib.stream()))
+        if torch.is_grad_enabled():  # no second derivative: asking for one is an error
+            error = torch._C._functions.DelayedError(b"bpt_b200: layer_norm is differentiable once only", 3)
+            da, dw, db = error(*(g.detach().requires_grad_() for g in (da, dw, db)))
+        return da, da, dw, db, None
+
+
 def add_layer_norm(x, r, norm):
-    """norm(x + r) for an nn.LayerNorm over the last dimension; on CUDA one fused call, forward and backward (norm.py),
-    where the rules of bpt_add_layer_norm hold (same dtype everywhere, last dimension a multiple of 8 up to 4096), else
+    """norm(x + r) for an nn.LayerNorm over the last dimension; on CUDA one fused call, forward and backward (norm.py; without
+    the torch extensions through ctypes), where the rules of bpt_add_layer_norm hold (same dtype everywhere, last dimension a multiple of 8 up to 4096), else
     torch's operators, whose rounding of the sum x + r callers of other widths have had so far.  `norm.layer_norm`
     itself takes every width up to 8192."""
     dim = x.size(-1)
     if (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16, torch.float16) and dim % 8 == 0 and dim <= 4096
             and norm.weight is not None and norm.bias is not None and norm.weight.dtype == x.dtype
             and r.dtype == x.dtype and r.shape == x.shape and tuple(norm.normalized_shape) == (dim,)):
-        return layer_norm(x, norm.weight, norm.bias, norm.eps, residual=r)
+        if _has_train_extension():
+            return layer_norm(x, norm.weight, norm.bias, norm.eps, residual=r)
+        return _AddLayerNorm.apply(x.contiguous(), r.contiguous(), norm.weight, norm.bias, norm.eps)
     return norm(x + r)
 
 
