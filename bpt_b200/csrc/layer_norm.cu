@@ -179,6 +179,26 @@ template <int n> __device__ __forceinline__ void multiply_add(float (&c)[n], con
         }
     }
 }
+// A piece a - mean -> y, with gamma and beta from column c on (or null: ones, zeros).  v is used up.
+template <typename T, int kVec>
+__device__ __forceinline__ void finish_piece(float (&v)[kVec], float rstd, const T *gamma, const T *beta, int c, T *y) {
+    multiply(v, rstd);
+    float g[kVec], b[kVec];
+    if (gamma) {
+        widen(load_raw<T, kVec>(gamma + c), g);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) g[i] = 1.f;
+    }
+    if (beta) {
+        widen(load_raw<T, kVec>(beta + c), b);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) b[i] = 0.f;
+    }
+    multiply_add(b, v, g);
+    store_vec<T, kVec>(y, b);
+}
 // The sums of a block's rows -> one partial row: [block][d gamma, d beta][dim].
 template <int kVec, int kVecs>
 __device__ __forceinline__ void store_partial(const float (&acc_g)[kVecs][kVec], const float (&acc_b)[kVecs][kVec], float *sums, float *partial,
@@ -200,6 +220,68 @@ __device__ __forceinline__ void store_partial(const float (&acc_g)[kVecs][kVec],
             for (int k = 0; k < rows_here; ++k) s += sums[k * dim + c];
             partial[(static_cast<int64_t>(blockIdx.x) * 2 + which) * dim + c] = s;
         }
+    }
+}
+
+// The forward of rows of whole pieces of 8 that a warp holds by itself: a warp a row, a block for every few rows, nothing
+// kept from row to row.  No barrier, and the SM's other warps cover a row's loads.  Against the kernel below, whose rows to
+// come travel by cp.async and whose wider rows belong to several warps (x, r -> y, us):
+//     131064 x 8     fp16 27 / 36                         131064 x 1024  fp32 238 / 300, bf16 138 / 165
+//     131064 x 512   fp32 117 / 132, bf16 64 / 66         131064 x 1536  fp32 403 / 465, bf16 244 / 285
+//     131064 x 520   fp32 124 / 223, bf16 79 / 144        131064 x 2048  fp32 631 / 575, bf16 358 / 320
+// A few wide rows are better off with several warps each, more of them not before the memory is what bounds both:
+//     555 x 1536     fp32 7.7 / 5.2, bf16 4.6 / 4.1       4096 x 2048    fp32 20 / 23, bf16 10.4 / 11.5
+//     4096 x 1536    fp32 14 / 18, bf16 8.4 / 10.4        10000 x 2048   fp32 59 / 52, bf16 33 / 29
+bool ln_row_a_warp(int64_t n_rows, int dim) {
+    return dim <= 1024 || (n_rows > 2048 && (dim <= 1536 || (dim <= 2048 && n_rows <= 8192)));
+}
+template <typename T, int kVecs, bool kHasR, int kBlock>
+__global__ void __launch_bounds__(kBlock)
+layer_norm_row_kernel(const T *x, const T *r, const T *gamma, const T *beta, float eps, T *y, float *mean_out, float *rstd_out,
+                      int64_t n_rows, int dim) {
+    tc5::let_next_start();
+    tc5::wait_for_previous();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / 32) + (threadIdx.x >> 5), at = row * dim;
+    if (row >= n_rows) return;
+    float v[kVecs][8];
+    float sum = 0.f, sq = 0.f;  // piece by piece: chains of 8 additions and of kVecs
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        const int c = (u * 32 + lane) * 8;
+        if (c < dim) {
+            widen(load_raw<T, 8>(x + at + c), v[u]);
+            if constexpr (kHasR) {
+                float w[8];
+                widen(load_raw<T, 8>(r + at + c), w);
+                add(v[u], w);
+            }
+            float part = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part += v[u][i];
+            sum += part;
+        }
+    }
+    const float mean = warp_sum(sum) / static_cast<float>(dim);
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        if ((u * 32 + lane) * 8 < dim) {
+            add(v[u], -mean);
+            float part = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part = fmaf(v[u][i], v[u][i], part);
+            sq += part;
+        }
+    }
+    const float rstd = rsqrtf(warp_sum(sq) / static_cast<float>(dim) + eps);
+    if (mean_out && lane == 0) {
+        mean_out[row] = mean;
+        rstd_out[row] = rstd;
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        const int c = (u * 32 + lane) * 8;
+        if (c < dim) finish_piece<T, 8>(v[u], rstd, gamma, beta, c, y + at + c);
     }
 }
 
@@ -322,24 +404,7 @@ layer_norm_kernel(const T *x, const T *r, const T *gamma, const T *beta, float e
         }
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
-            if (rows.in(u)) {
-                multiply(v[u], rstd);
-                float g[kVec], c[kVec];
-                if (gamma) {
-                    widen(load_raw<T, kVec>(gamma + t * kVec + u * step), g);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) g[i] = 1.f;
-                }
-                if (beta) {
-                    widen(load_raw<T, kVec>(beta + t * kVec + u * step), c);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) c[i] = 0.f;
-                }
-                multiply_add(c, v[u], g);
-                store_vec<T, kVec>(y + row * dim + t * kVec + u * step, c);
-            }
+            if (rows.in(u)) finish_piece<T, kVec>(v[u], rstd, gamma, beta, t * kVec + u * step, y + row * dim + t * kVec + u * step);
         }
     }
     if constexpr (kAhead > 0) tc5::cp_async_wait_all();
@@ -503,11 +568,16 @@ int ln_vec(int dim, size_t elem, std::initializer_list<const void *> ptrs) {
     if (dim % 2 == 0 && all % (2 * elem) == 0) return 2;
     return 1;
 }
-// Calls f(kVec, kVecs) as compile-time constants for the pieces a thread of this layout has.
-template <typename F> int ln_dispatch(const LnLayout &l, int dim, F f) {
+// Calls f(kVec, kVecs) as compile-time constants for the pieces a thread of this layout has.  kLeast8: the fewest pieces of 8
+// that there are calls for: 2, where one would be a row that a warp holds by itself, or 3, where 4 is the widest piece.
+template <int kLeast8, typename F> int ln_dispatch(const LnLayout &l, int dim, F f) {
     const int n = (dim + l.tpr * l.vec - 1) / (l.tpr * l.vec);
-    if (l.vec == 8) return n <= 1 ? f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>())
-                                  : f(std::integral_constant<int, 8>(), std::integral_constant<int, 2>());
+    if constexpr (kLeast8 <= 1) {
+        if (l.vec == 8 && n <= 1) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
+    }
+    if constexpr (kLeast8 <= 2) {
+        if (l.vec == 8) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 2>());
+    }
     if (l.vec == 4) return n <= 2 ? f(std::integral_constant<int, 4>(), std::integral_constant<int, 2>())
                          : n <= 3 ? f(std::integral_constant<int, 4>(), std::integral_constant<int, 3>())
                                   : f(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
@@ -535,8 +605,30 @@ template <typename T>
 int launch_layer_norm(const void *x, const void *r, const void *gamma, const void *beta, float eps, void *y, float *mean, float *rstd,
                       int64_t n_rows, int dim, cudaStream_t stream) {
     const LnLayout l = ln_layout(dim, ln_vec(dim, sizeof(T), {x, r, gamma, beta, y}));
+    if (l.vec == 8 && ln_row_a_warp(n_rows, dim)) {
+        auto go = [&](auto vecs, auto has_r) -> int {
+            constexpr int kBlock = vecs.value == 1 ? 256 : 128;  // 131064 x 512 bf16 63 against 65, x 8 35 against 27
+            const auto blocks = static_cast<unsigned>((n_rows + kBlock / 32 - 1) / (kBlock / 32));
+            BPT_CUDA(tc5::launch_after(layer_norm_row_kernel<T, vecs.value, has_r.value, kBlock>, blocks, kBlock, 0, stream,
+                                       static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(gamma),
+                                       static_cast<const T *>(beta), eps, static_cast<T *>(y), mean, rstd, n_rows, dim));
+            return BPT_OK;
+        };
+        auto with_vecs = [&](auto has_r) -> int {
+            switch ((dim + 255) / 256) {
+                case 1: return go(std::integral_constant<int, 1>(), has_r);
+                case 2: return go(std::integral_constant<int, 2>(), has_r);
+                case 3: return go(std::integral_constant<int, 3>(), has_r);
+                case 4: return go(std::integral_constant<int, 4>(), has_r);
+                case 5: return go(std::integral_constant<int, 5>(), has_r);
+                case 6: return go(std::integral_constant<int, 6>(), has_r);
+                default: return go(std::integral_constant<int, 8>(), has_r);
+            }
+        };
+        return r ? with_vecs(std::true_type()) : with_vecs(std::false_type());
+    }
     const int64_t rows_here = l.block / l.tpr, blocks = (n_rows + rows_here - 1) / rows_here;
-    return ln_dispatch(l, dim, [&](auto vec, auto vecs) -> int {
+    return ln_dispatch<2>(l, dim, [&](auto vec, auto vecs) -> int {
         auto go = [&](auto has_r, auto block) -> int {
             constexpr int kPiece = vec.value * sizeof(T), kAhead = kPiece >= 16 ? 2 : 0;
             using R = Rows<T, vec.value, vecs.value, has_r.value ? 2 : 1, block.value, kAhead>;
@@ -562,7 +654,7 @@ int launch_layer_norm_backward(const void *gy, const void *x, const void *r, con
                                int64_t n_rows, int dim, cudaStream_t stream) {
     const LnLayout l = ln_layout(dim, std::min<int>(ln_vec(dim, sizeof(T), {gy, x, r, gamma, da}), 16 / sizeof(T)));
     const unsigned grid = static_cast<unsigned>(ln_backward_grid(n_rows, dim));
-    const int rc = ln_dispatch(l, dim, [&](auto vec, auto vecs) -> int {
+    const int rc = ln_dispatch<sizeof(T) == 4 ? 3 : 1>(l, dim, [&](auto vec, auto vecs) -> int {
         auto go = [&](auto has_r) -> int {
             // three rows ahead where two blocks a SM have the room, else two; pieces that are not 16 bytes come directly
             constexpr int kRow = 256 * 16 * vecs.value * (has_r.value ? 3 : 2);
