@@ -27,8 +27,12 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, lab
 
     Rows of x and weight may have any stride; other layouts are copied.  bf16 and fp16 rows that start on 16-byte
     boundaries are read where they lie, others are copied into the workspace first; fp32 operands are split there into
-    two fp16 planes, or three bf16 planes where the sizes of rows or of columns differ by more than 2^24, which keeps fp32
-    accuracy on the tensor cores.  Forward and backward may be captured into CUDA graphs.  Runs on the current stream of x's device;
+    two fp16 planes, or three bf16 planes where the sizes of rows, of columns or (reduction "none") of the tokens' gradients
+    differ by more than 2^24, which keeps fp32 accuracy on the tensor cores, with two limits: numbers of an operand below
+    2^-110 keep fewer bits, and with two planes a logit's gradient is held to 2^-22 of itself or 2^-50 of the largest token's
+    gradient, so a row of d weight whose class has a probability far below 2^-28 for every token has few bits, or is zero.
+    fp16: the latter bound is 2^-39.  For more than 256 tokens of bf16 or fp16 a logit's gradient is rounded to that type before the
+    products.  Forward and backward may be captured into CUDA graphs.  Runs on the current stream of x's device;
     bad arguments raise RuntimeError."""
     if reduction not in _REDUCTIONS:
         raise RuntimeError("bpt_b200: linear_cross_entropy: reduction must be none, mean or sum")

@@ -181,3 +181,22 @@ def test_classes_masked_with_the_lowest_number(n, dtype):
         loss = linear_cross_entropy(*leaves[:2], t, bias=leaves[2], label_smoothing=smoothing, reduction="none")
         loss.backward(torch.ones_like(loss))
         assert bool(torch.isfinite(loss).all()) and all(bool(torch.isfinite(v.grad).all()) for v in leaves)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_probabilities_of_very_different_size(dtype):
+    """Classes whose probability is from 2^-4 down to 2^-60 for every token: rows of d w that are as small.  An entry of dZ is off by
+    the note's bound and, in fp32, by no more than 2^-50 beside it (in fp16 by 2^-39, which the formula has)."""
+    for n in (300, 90):
+        x, w, b, t = inputs(n, 600, 72, dtype, spread=0.3)
+        b = (b.float() - 0.6931 * (torch.arange(600, device="cuda") % 60)).to(dtype)
+        t = t // 60 * 60  # classes that are probable
+        t[::7] = IGNORE
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+        linear_cross_entropy(*leaves[:2], t, bias=leaves[2], reduction="sum").backward()
+        want, off = formula(x, w, b, t, 0.0, "sum", torch.ones((), device="cuda"))
+        p = torch.softmax(x.double() @ w.double().t() + b.double(), 1)
+        assert float(p.max()) > 2.0 ** -5 and float(p.min()) < 2.0 ** -60
+        more = off_by(x, w, t, 2.0 ** -50 if dtype == torch.float32 else 0.0)
+        for name, leaf, v, e, m in zip(("dx", "dw", "db"), leaves, want[1:], off[1:], more):
+            near(leaf.grad, v, e + m, name)
