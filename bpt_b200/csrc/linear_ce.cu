@@ -58,7 +58,7 @@ constexpr int kRows = kBM / 2, kCols = kBN / 2;               // what a block lo
 constexpr int kABytes = kRows * kBK * 2, kBBytes = kCols * kBK * 2, kStageBytes = kABytes + kBBytes;
 constexpr int kChunkBytes = 64 * 128;  // an MN-major tile: 64 rows along K of 64 elements
 // Eight warps finish tiles, one loads, one issues products (two more make its warpgroup whole).  The finishing warps take
-// registers that the others leave: 256 * 216 + 128 * 72 = 384 * 168, what the block is launched with.
+// registers that the others leave: 256 * 208 + 128 * 88 = 384 * 168, what the block is launched with.
 constexpr int kFinishWarps = 8, kThreads = (kFinishWarps + 4) * 32;
 constexpr int kFinishRegs = 208, kOtherRegs = 88;
 static_assert(kFinishWarps * 32 * kFinishRegs + 128 * kOtherRegs <= kThreads * 168, "the block's registers");

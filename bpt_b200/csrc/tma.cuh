@@ -101,14 +101,8 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t slot_smem_addr, uint32_
 __device__ __forceinline__ void tmem_free_pair(uint32_t taddr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(cols) : "memory");
 }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
-    asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
-}
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t done;
