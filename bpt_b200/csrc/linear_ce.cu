@@ -812,10 +812,8 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         uint32_t ready_phase = 0;
         float run_max = -INFINITY, run_sum = 0.f, run_z = 0.f;
         int tgt = -1;
-        float row_lse = 0.f, row_l2 = 0.f, row_g = 0.f, uniform = 0.f;
-        // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0 (none there); some lse times log2(e)
-        // is not in fp32's range
-        bool row_plain = true, row_skips = false, row_far = false;
+        float row_lse = 0.f, row_l2 = 0.f, row_unit = 0.f, row_g = 0.f, uniform = 0.f;
+        bool row_plain = true, row_skips = false;  // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0 (none there)
         Scale x_scale{}, w_scale{};
         if constexpr (kKind == kProducts) {
             x_scale = result_scale<T>(p, 0);
@@ -879,8 +877,9 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         uniform = p.smoothing / static_cast<float>(p.vocab) * row_g;
                         row_skips = __any_sync(0xffffffffu, row_g == 0.f);
                         row_plain = p.smoothing == 0.f && __all_sync(0xffffffffu, row_g == kDzScale<T> || row_g == 0.f);
-                        row_l2 = row_lse * kLog2e - (row_plain && kIsHalf<T> ? 14.f : 0.f);
-                        row_far = __any_sync(0xffffffffu, fabsf(row_lse) > kMostForExp);
+                        // beyond kMostForExp two numbers are equal or 2^104 apart: the factor changes no exponential
+                        row_unit = fabsf(row_lse) > kMostForExp ? 1.f : kLog2e;
+                        row_l2 = row_lse * row_unit - (row_plain && kIsHalf<T> ? 14.f : 0.f);
                     }
                 }
                 if constexpr (kKeepSums) {
@@ -992,17 +991,12 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                 v[i + 1] = dz.y;
                             }
                         } else {
-                            if (!row_far) {
-                                const float2 from = make_float2(-row_l2, -row_l2);
+                            const float2 from = make_float2(-row_l2, -row_l2), unit = make_float2(row_unit, row_unit);
 #pragma unroll
-                                for (int i = 0; i < 32; i += 2) {
-                                    const float2 d = fma2(make_float2(v[i], v[i + 1]), log2e, from);
-                                    v[i] = ex2(d.x);
-                                    v[i + 1] = ex2(d.y);
-                                }
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] = ex2((v[i] - row_lse) * kLog2e + (row_plain && kIsHalf<T> ? 14.f : 0.f));
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 d = fma2(make_float2(v[i], v[i + 1]), unit, from);
+                                v[i] = ex2(d.x);
+                                v[i + 1] = ex2(d.y);
                             }
                             if (!row_plain) {
                                 const float2 g2 = make_float2(row_g, row_g), u2 = make_float2(-uniform, -uniform);
