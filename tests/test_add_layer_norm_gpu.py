@@ -52,3 +52,26 @@ def test_rows_that_are_not_finite_stay_to_themselves(dtype):
         keep[7] = keep[20] = False
         assert torch.equal(got[keep], want[keep]) and not bool(torch.isfinite(got[7]).any())
         assert bool(torch.isnan(got[20]).all())
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows are as in a call of their own, forward and backward."""
+    from bpt_b200.norm import layer_norm
+    rows, dim = (1 << 31) // 512 + 5000, 512
+    x = torch.empty(rows, dim, dtype=torch.bfloat16, device="cuda")
+    last = slice(rows - 6000, rows)
+    part, r, w, b, gy = inputs(6000, dim, torch.bfloat16, True)
+    x.zero_()
+    x[last] = part
+    grad = torch.zeros_like(x)
+    grad[last] = gy
+    leaf, weight = x.requires_grad_(True), w.clone().requires_grad_(True)
+    y = layer_norm(leaf, weight, b)
+    few, weight_of_few = part.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    want = layer_norm(few, weight_of_few, b)
+    assert torch.equal(y.detach()[last], want.detach())
+    y.backward(grad)
+    want.backward(gy)
+    assert torch.equal(leaf.grad[last], few.grad)
+    full = formula(part, None, w, b, gy, 1e-5)  # the other rows add nothing
+    near(weight.grad, full[0][2], full[1][2])

@@ -200,3 +200,74 @@ def test_probabilities_of_very_different_size(dtype):
         more = off_by(x, w, t, 2.0 ** -50 if dtype == torch.float32 else 0.0)
         for name, leaf, v, e, m in zip(("dx", "dw", "db"), leaves, want[1:], off[1:], more):
             near(leaf.grad, v, e + m, name)
+
+
+def test_label_smoothing_and_a_summed_divergence():
+    """KLDivLoss(reduction="sum") of the log-probabilities against targets with smoothing / vocab on every class is the summed
+    loss minus the targets' entropy, a constant for each token that counts: the same gradients.  Tolerances: the module's note."""
+    x, w, b, t = inputs(200, 300, 64, torch.float32, padded=0.2)
+    leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+    loss = linear_cross_entropy(*leaves[:2], t, bias=leaves[2], label_smoothing=0.1, reduction="sum")
+    loss.backward()
+    exact = [v.double().requires_grad_(True) for v in (x, w, b)]
+    counted = t != IGNORE
+    logp = torch.log_softmax(exact[0] @ exact[1].t() + exact[2], 1)[counted]
+    q = torch.full_like(logp, 0.1 / 300).scatter_(1, t[counted].unsqueeze(1), 0.9 + 0.1 / 300)
+    divergence = torch.nn.functional.kl_div(logp, q, reduction="sum")
+    divergence.backward()
+    entropy = -(q * q.log()).sum()
+    want, off = formula(x, w, b, t, 0.1, "sum", torch.ones((), device="cuda"))
+    near(loss.detach(), (divergence + entropy).detach(), off[0], "loss")
+    for name, leaf, e, slack in zip(("dx", "dw", "db"), leaves, exact, off[1:]):
+        near(leaf.grad, e.grad, slack, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_far_apart_in_memory(dtype):
+    """Rows whose offsets pass 2^31 elements, read in place and copied: the same as close together."""
+    n, step, dim = 140000, 16384, 64
+    big = torch.empty(n * step, dtype=dtype, device="cuda").view(n, step)
+    x, w, b, t = inputs(n, 100, dim, dtype, padded=0.1)
+    want = linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    for at in (8, 3):
+        far = big[:, at:at + dim]
+        far.copy_(x)
+        assert torch.equal(linear_cross_entropy(far, w, t, bias=b, reduction="none"), want)
+    leaves = [v.clone().requires_grad_(True) for v in (x, w)]
+    linear_cross_entropy(*leaves, t, bias=b).backward()
+    held = far.detach().requires_grad_(True)
+    again = w.clone().requires_grad_(True)
+    linear_cross_entropy(held, again, t, bias=b).backward()
+    assert torch.equal(held.grad, leaves[0].grad) and torch.equal(again.grad, leaves[1].grad)
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_replayed_graphs_choose_the_planes_again(reduction):
+    """fp32: which planes the operands take is found on the device.  A step captured with ordinary numbers is replayed with a
+    column far below the others and tokens of far smaller weight, then with ordinary ones again."""
+    x, w, b, t = inputs(300, 500, 72, torch.float32, padded=0.1)
+    leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+    weight = torch.ones(300, device="cuda") if reduction == "none" else torch.ones((), device="cuda")
+
+    def step():
+        loss = linear_cross_entropy(*leaves[:2], t, bias=leaves[2], reduction=reduction)
+        return (loss.detach(),) + torch.autograd.grad(loss, leaves, weight)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for column, small in ((1.0, 0), (2.0 ** -40, 0), (1.0, 50), (2.0 ** -40, 50), (1.0, 0)):
+        with torch.no_grad():
+            leaves[0].copy_(x)
+            leaves[0][:, 5] *= column
+            if reduction == "none":
+                weight.copy_(2.0 ** -(torch.arange(300, device="cuda") % (small + 1)).float())
+        graph.replay()
+        got = [v.clone() for v in out]
+        assert all(torch.equal(a, e) for a, e in zip(got, step()))
