@@ -2,8 +2,8 @@
 //
 // The block of modules/attention.py ends each of its two halves with `norm(h + sublayer(h))`
 // (attention.py:79-81, 141, 168-171).  As two torch operators that is a read of two tensors and a
-// write for the sum, then a read and a write for the normalisation; here a row belongs to one warp (up to
-// 512 elements; to more warps beyond), which keeps the sum in registers (fp32), reduces mean and variance with
+// write for the sum, then a read and a write for the normalisation; here a row belongs to one warp (wide ones to
+// several), which keeps the sum in registers (fp32), reduces mean and variance with
 // shuffles and writes the result once: 3 passes of N x dim instead of 5.
 //
 // With a = x + r, mean and rstd of a row of a, n = (a - mean) rstd and q = gy gamma the derivative is
@@ -13,9 +13,10 @@
 // the threads that own a column, then go through one partial row per block (no atomics: the order is fixed).
 //
 // HBM-bound: (2 reads + 1 write) x N x dim x bytes forward, (3 reads + 1 write) backward.  131064 x 512 in bf16:
-// forward 68 us, backward 92 us, 5.9 and 5.8 TB/s or 90 and 89% of what a copy reaches; the sums of the partial rows
+// forward 64 to 66 us, backward 91 us, 6.2 and 5.9 TB/s or 95 and 90% of what a copy reaches; the sums of the partial rows
 // 8 us by themselves, half of it behind the backward's end.  What is left: the reads and writes of a memory that turns
-// round between them, and 23% (backward) and 41% (forward) of the warps an SM could hold, which the rows ahead make up for.
+// round between them, and of the warps an SM could hold 65% (forward) and 24% (backward, whose column sums take the
+// registers; the rows ahead make up for that).
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>

@@ -2,8 +2,9 @@
 bpt_linear_ce_backward.
 
 The reference's models end in a generator (modules/model.py:8-17: projection, log-softmax) whose log-probabilities the
-task scripts hand to a loss: nll_loss (lm.py:120-140) or label smoothing (loss/__init__.py:4-28).
-`linear_cross_entropy(x, weight, target, bias)` is both as one differentiable call.  The (tokens, vocabulary) logits
+task scripts hand to a loss: nll_loss (lm.py:120-140), or a summed KL divergence from smoothed targets
+(loss/__init__.py:4-28), which is the summed cross entropy with label smoothing minus the targets' entropy.
+`linear_cross_entropy(x, weight, target, bias)` is projection and cross entropy as one differentiable call.  The (tokens, vocabulary) logits
 are made tile by tile and never kept: the forward keeps one number per token, the backward makes them again, a piece
 of tokens x vocabulary at a time.  Results do not vary from run to run.  The autograd node is compiled
 (csrc_torch/train_ext.cpp).

@@ -342,7 +342,8 @@ class BPTEncoderDecoder(nn.Module):
 
     def loss(self, enc_tokens, enc_leaf_ids, enc_plan, dec_tokens, dec_leaf_ids, dec_plan, inter_plan, readout_ids,
              target, **options):
-        """Cross entropy of forward(...) against target (len(readout_ids),), without the log-probabilities in memory
-        (mt.py trains with label smoothing, loss/__init__.py:4-28).  options: ignore_index, label_smoothing, reduction."""
+        """Cross entropy of forward(...) against target (len(readout_ids),), without the log-probabilities in memory.
+        options: ignore_index, label_smoothing, reduction.  (mt.py trains with a summed KL divergence from smoothed targets,
+        loss/__init__.py:4-28: the summed loss minus the targets' entropy where every class is smoothed alike.)"""
         return self.generator.loss(self.features(enc_tokens, enc_leaf_ids, enc_plan, dec_tokens, dec_leaf_ids, dec_plan,
                                                  inter_plan, readout_ids), target, **options)

@@ -504,8 +504,8 @@ int bpt_layer_norm_backward(const void *gy, const void *x, const void *r, const 
 
 /* ------------------------------------------------------------------------------------
  * Softmax cross entropy of the logits z = x W^T + bias, without the logits: the generator of modules/model.py:8-17
- * (projection + log-softmax) and the loss the task scripts put on it (nll_loss, lm.py:120-140; label smoothing,
- * loss/__init__.py:4-28) as one call, and its gradients.
+ * (projection + log-softmax) and the loss the task scripts put on it (nll_loss, lm.py:120-140) as one call, and its
+ * gradients.  With smoothing: the summed KL divergence of loss/__init__.py:4-28 plus the entropy of targets smoothed as here.
  *
  * x: (n, dim), w: (vocab, dim), row strides ldx, ldw in elements; bias (vocab) or NULL; all of `dtype` (BPT_F32,
  * BPT_BF16, BPT_F16).  target: (n) int64.  A token whose target is ignore_index has loss 0 and no gradient, whatever
