@@ -1507,19 +1507,20 @@ template <int kLanes> __global__ void __launch_bounds__(kLossThreads) linear_ce_
 // of 8 elements, fp32 as planes.
 
 // What decides how fp32 operands are split: the largest number of each matrix, and the smallest of the largest numbers of
-// its rows and of its columns (those of zeros aside).  Rows and columns are looked at in stretches, rows of kSpreadCols
+// its rows and of its columns (those of zeros aside).  Rows and columns are looked at in stretches, rows of 128 kUnits
 // columns and columns of one block's rows (kSpreadRows or more), so that a block needs nothing from another: a warp brings
-// two rows in, a lane keeps the largest of its 16 columns.  Stretches are no larger than what they are part of, so this errs
-// towards three planes.  Loads past the end take the last column or row again.  W of 50000 x 512: 29 us, by itself, from memory (3.5 TB/s),
-// with 16-byte loads.
-constexpr int kSpreadCols = 512, kSpreadRows = 32, kSpreadBlocks = 148 * 4;
-template <bool kWide>
+// four rows in, a lane keeps the largest of its 4 kUnits columns.  Stretches are no larger than what they are part of, so this
+// errs towards three planes.  Loads past the end take the last columns or row again.  kPiece: elements of a load, as many as
+// dim and the rows' places allow.  By itself, without the columns' part and with it: 50000 x 512 16 and 19 us, 34558 x 626
+// 14 and 19, 12102 x 300 7.3 and 7.3; with stretches of 512 columns for every width 20300 x 101 took 15 us, now 7.
+constexpr int kSpreadRows = 32, kSpreadBlocks = 148 * 8;
+template <int kPiece, int kUnits>
 __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *x, int64_t ldx, int64_t x_rows, const float *w,
                                                                int64_t ldw, int64_t w_rows, int dim, int64_t block_rows,
                                                                int64_t x_blocks, const int64_t *target, int64_t ignore_index,
                                                                unsigned *found) {
-    constexpr int kRowsAtOnce = 2, kPiece = kWide ? 4 : 1, kPieces = kSpreadCols / 32 / kPiece;
-    __shared__ unsigned s_found[2], s_col[8][kSpreadCols];
+    constexpr int kCols = 128 * kUnits, kRowsAtOnce = 4, kPieces = kCols / 32 / kPiece;
+    __shared__ unsigned s_found[2], s_col[8][kCols];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x < 2) s_found[threadIdx.x] = 0u;
     let_next_start();
@@ -1532,7 +1533,7 @@ __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *x, i
     unsigned col[kPieces][kPiece], top = 0u, low = 0u;  // low: complement of the smallest
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
-        at[k] = min(static_cast<int>(blockIdx.y) * kSpreadCols + (32 * k + lane) * kPiece, dim - kPiece);
+        at[k] = min(static_cast<int>(blockIdx.y) * kCols + (32 * k + lane) * kPiece, dim - kPiece);
 #pragma unroll
         for (int i = 0; i < kPiece; ++i) col[k][i] = 0u;
     }
@@ -1546,12 +1547,16 @@ __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *x, i
             const float *const p = from + row * ld;
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) {
-                if constexpr (kWide) {
+                if constexpr (kPiece == 4) {
                     const float4 piece = *reinterpret_cast<const float4 *>(p + at[k]);
                     v[r][k][0] = piece.x;
                     v[r][k][1] = piece.y;
                     v[r][k][2] = piece.z;
                     v[r][k][3] = piece.w;
+                } else if constexpr (kPiece == 2) {
+                    const float2 piece = *reinterpret_cast<const float2 *>(p + at[k]);
+                    v[r][k][0] = piece.x;
+                    v[r][k][1] = piece.y;
                 } else {
                     v[r][k][0] = p[at[k]];
                 }
@@ -1580,7 +1585,7 @@ __global__ void __launch_bounds__(256) linear_ce_spread_kernel(const float *x, i
         for (int i = 0; i < kPiece; ++i) s_col[warp][(32 * k + lane) * kPiece + i] = col[k][i];
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < kSpreadCols; c += 256) {
+    for (int c = threadIdx.x; c < kCols; c += 256) {
         unsigned largest = 0u;
 #pragma unroll
         for (int k = 0; k < 8; ++k) largest = max(largest, s_col[k][c]);
@@ -2074,6 +2079,30 @@ struct Tokens {  // the index and its length, on the device
     uint16_t *gathered;
 };
 
+int launch_spread(const Shape &s, const Call &c, unsigned *found, cudaStream_t stream) {
+    const int64_t units = ce_div(s.dim, 128), stretches = ce_div(units, 4);
+    const int64_t block_rows = std::max<int64_t>(kSpreadRows, ce_div((s.n + s.vocab) * stretches, kSpreadBlocks)), x_blocks = ce_div(s.n, block_rows);
+    const dim3 grid(static_cast<unsigned>(x_blocks + ce_div(s.vocab, block_rows)), static_cast<unsigned>(stretches));
+    auto launch = [&](auto piece, auto units_each) -> int {
+        BPT_CUDA(launch_after(linear_ce_spread_kernel<piece.value, units_each.value>, grid, 256, 0, stream, static_cast<const float *>(c.x), c.ldx,
+                              s.n, static_cast<const float *>(c.w), c.ldw, int64_t(s.vocab), s.dim, block_rows, x_blocks, c.target,
+                              c.ignore_index, found));
+        return BPT_OK;
+    };
+    auto with_piece = [&](auto piece) -> int {
+        switch (ce_div(units, stretches)) {
+            case 1: return launch(piece, std::integral_constant<int, 1>());
+            case 2: return launch(piece, std::integral_constant<int, 2>());
+            case 3: return launch(piece, std::integral_constant<int, 3>());
+            default: return launch(piece, std::integral_constant<int, 4>());
+        }
+    };
+    const uint64_t places = static_cast<uint64_t>(s.dim | c.ldx | c.ldw) * sizeof(float) | reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.w);
+    return places % 16 == 0  ? with_piece(std::integral_constant<int, 4>())
+           : places % 8 == 0 ? with_piece(std::integral_constant<int, 2>())
+                             : with_piece(std::integral_constant<int, 1>());
+}
+
 // The index of the tokens that count; X and W as the tiles read them: where they lie (X, where tokens are ignored: from
 // the copy), or packed.  loss: where ignored tokens' zeros go, or null; dx: the same for their rows of d x; grad: the
 // backward's gradients, or null.
@@ -2093,13 +2122,7 @@ int prepare_operands(const Shape &s, const Call &c, const Tokens &t, uint16_t *x
                               c.target, s.n, c.ignore_index, found + kFoundGrad));
     }
     if constexpr (kIsFloat<T>) {
-        const int64_t block_rows = std::max<int64_t>(kSpreadRows, ce_div(s.n + s.vocab, kSpreadBlocks)), x_blocks = ce_div(s.n, block_rows);
-        const dim3 grid(static_cast<unsigned>(x_blocks + ce_div(s.vocab, block_rows)), static_cast<unsigned>(ce_div(s.dim, kSpreadCols)));
-        const bool wide = s.dim % 4 == 0 && c.ldx % 4 == 0 && c.ldw % 4 == 0 &&
-                          (reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.w)) % 16 == 0;
-        BPT_CUDA(launch_after(wide ? linear_ce_spread_kernel<true> : linear_ce_spread_kernel<false>, grid, 256, 0, stream,
-                              static_cast<const float *>(c.x), c.ldx, s.n, static_cast<const float *>(c.w), c.ldw, int64_t(s.vocab), s.dim,
-                              block_rows, x_blocks, c.target, c.ignore_index, found));
+        BPT_TRY(launch_spread(s, c, found, stream));
     }
     if (!s.pack_x && !s.pack_w) return BPT_OK;
     const Unpacked<T> from_x{static_cast<const T *>(c.x), c.ldx, s.n, x_to, static_cast<int64_t>(align_up(s.n * s.packed_ld, 64))};

@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 def test_fp32_columns_of_very_different_size(of, down):
     """One feature far below the others: its column of d w has what that column of x keeps, its column of d x what that of w
     does.  One far above the others in x and as far below in w: the logits have what the other columns of x keep."""
-    for n, dim in ((300, 72), (70, 73), (90, 1100)):
+    for n, dim in ((300, 72), (70, 73), (90, 1100), (65, 150), (40, 270), (33, 642), (50, 401)):
         x, w, b, t = inputs(n, 500, dim, torch.float32, padded=0.1)
         for c in (5, dim - 100) if dim > 512 else (5,):
             if of == "x":
