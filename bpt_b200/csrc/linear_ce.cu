@@ -165,15 +165,18 @@ constexpr int kFound = 6, kFoundGrad = 4;
 constexpr unsigned kSpread = 24;
 __device__ __forceinline__ Split read_split(const unsigned *found) {
     Split s;
-    const unsigned x_top = found[0] >> 23, x_low = ~found[1] >> 23, w_top = found[2] >> 23, w_low = ~found[3] >> 23;
+    unsigned f[kFound];  // all under way at once: kernels start with this
+#pragma unroll
+    for (int k = 0; k < kFound; ++k) f[k] = found[k];
+    const unsigned x_top = f[0] >> 23, x_low = ~f[1] >> 23, w_top = f[2] >> 23, w_low = ~f[3] >> 23;
     auto fits = [](unsigned top, unsigned low) { return top == 0u || (top >= 15u && top <= 254u && top - low <= kSpread); };
     // a matrix of zeros (or of nothing but denormal numbers, which the planes do not hold) has top 0
-    if (found[0] != 0u && x_top == 0u) return s;
-    if (found[2] != 0u && w_top == 0u) return s;
+    if (f[0] != 0u && x_top == 0u) return s;
+    if (f[2] != 0u && w_top == 0u) return s;
     if (!fits(x_top, x_low) || !fits(w_top, w_low)) return s;
     // dZ's planes have one scale, too: a token's row is good to 2^-50 of the largest |g|
-    const unsigned g_top = found[kFoundGrad] >> 23, g_low = ~found[kFoundGrad + 1] >> 23;
-    if (found[kFoundGrad] != 0u && (g_low == 0u || g_top - g_low > kSpread)) return s;
+    const unsigned g_top = f[kFoundGrad] >> 23, g_low = ~f[kFoundGrad + 1] >> 23;
+    if (f[kFoundGrad] != 0u && (g_low == 0u || g_top - g_low > kSpread)) return s;
     s.half = true;
     if (x_top) {
         s.x = __uint_as_float((268u - x_top) << 23);  // the largest comes to [2^14, 2^15)
@@ -472,11 +475,10 @@ template <typename T> __device__ __forceinline__ float scaled(float v, Scale s) 
     if constexpr (kIsFloat<T>) v *= s.then;
     return v;
 }
-template <typename T> __device__ __forceinline__ Scale result_scale(const Params &p, int which) {
+template <typename T> __device__ __forceinline__ Scale result_scale(const Params &p, const Split &split, int which) {
     float scale = p.reduction == kReduceNone ? top_scale(*p.grad_top) : *p.grad;
     if (p.reduction == kReduceMean) scale = *p.count > 0.f ? scale / *p.count : 0.f;
     if constexpr (kIsFloat<T>) {
-        const Split split = read_split(p.split);
         if (!split.half) return Scale{scale, 1.f};
         scale *= 1.f / kHalfDz;
         const float back = which == 0 ? split.w_back : which == 1 ? split.x_back : 1.f;
@@ -503,8 +505,8 @@ __device__ __forceinline__ PieceRows piece_rows(const Params &p) {
 // d b of a piece, by two warps of each products block that have nothing else to do, 32 columns at a time: the column sums
 // that the pairs of the grad launch (fp32: the token blocks) left, added to those of earlier rows; the last are scaled
 // and stored.
-template <typename T> __device__ __forceinline__ void finish_bias(const Params &p, int rows_here, int warp, int warps, int lane) {
-    const Scale scale = result_scale<T>(p, 2);
+template <typename T> __device__ __forceinline__ void finish_bias(const Params &p, const Split &split, int rows_here, int warp, int warps, int lane) {
+    const Scale scale = result_scale<T>(p, split, 2);
     const int64_t m_tiles = (rows_here + kBM - 1) / kBM, total = m_tiles * p.grad_n_tiles;
     const int pairs = pairs_used(p.grad_pairs, total);
     for (int c0 = warp * 32; c0 < p.grad_n_ext; c0 += warps * 32) {
@@ -801,7 +803,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 }
             }
         } else if (kKind == kProducts && p.db) {
-            finish_bias<T>(p, rows_here, static_cast<int>(blockIdx.x) * 2 + warp - (kFinishWarps + 2), static_cast<int>(gridDim.x) * 2, lane);
+            finish_bias<T>(p, split, rows_here, static_cast<int>(blockIdx.x) * 2 + warp - (kFinishWarps + 2), static_cast<int>(gridDim.x) * 2, lane);
         }
     } else {  // ---- finishing: warp % 4 names the 32 of this block's rows, warp / 4 the half of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kFinishRegs));
@@ -816,8 +818,8 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         bool row_plain = true, row_skips = false;  // of the warp's rows: every g is 1 (or 0) and nothing smoothed; some g is 0 (none there)
         Scale x_scale{}, w_scale{};
         if constexpr (kKind == kProducts) {
-            x_scale = result_scale<T>(p, 0);
-            w_scale = result_scale<T>(p, 1);
+            x_scale = result_scale<T>(p, split, 0);
+            w_scale = result_scale<T>(p, split, 1);
         }
         // grad, 16-bit: column sums over the pair's token blocks of one vocabulary block
         constexpr bool kKeepSums = kKind == kGrad && !kPrecise;
@@ -1793,7 +1795,7 @@ __global__ void __launch_bounds__(256) linear_ce_parts_kernel(const __grid_const
     const Product &q = p.product[which];
     const int64_t pieces = q.acc_ld / 4, rows = which == 0 ? piece_rows(p).rows : q.row_end - q.row_offset, total = rows * pieces;
     const int32_t *const index = which == 0 && *p.n_counted < p.n_rows ? p.index : nullptr;
-    Scale scale = result_scale<T>(p, which);
+    Scale scale = result_scale<T>(p, kIsFloat<T> ? read_split(p.split) : Split(), which);
     if (*p.status) scale.first = __int_as_float(0x7fffffff);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t in_piece = i / pieces, at = (which == 0 ? piece_rows(p).first : q.row_offset) + in_piece, row = index ? index[at] : at;
