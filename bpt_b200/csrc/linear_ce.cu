@@ -30,13 +30,15 @@
 // results): a half-step error of each probability, the size of the rounding of the gradients themselves.
 // fp32 operands are split into 16-bit planes, and each product of matrices is run as the products of planes whose weight
 // is above 2^-24.  Scaled by a power of two to the top of fp16's range, an operand is two fp16 planes, the second kept
-// times 2^11: 22 significant bits by rounding, down to 2^-28 of the largest number, and good to 2^-51 of that number
-// below; three products (of second planes none is needed).  That is taken where no row's and no column's largest is below
-// 2^-24 of the matrix's largest: the logits' sums run along a row, the gradients' along a column, and the logits need the
-// columns, too, where the other operand's are as much smaller.  A number is then off by at most 2^-22 of itself or 2^-27 of
-// its row's and of its column's largest.  Nor may the tokens' own gradients (reduction none) lie further apart, since the
-// rows of dZ have one scale: an entry of dZ is off by at most 2^-22 of itself or 2^-50 of the largest |g|.  Otherwise three
-// bf16 planes (24 bits by truncation, exact, any range above 2^-110), six products.  A first pass over X and W finds which, on the
+// times 2^11: 22 significant bits by rounding, down to 2^-28 of the largest number, and good to 2^-50 of that number
+// below; three products (that of second planes adds 2^-22 of a term at most, or 2^-50 as below).  That is taken where no
+// row's and no column's largest is below 2^-24 of the matrix's largest: the logits' sums run along a row, the gradients'
+// along a column, and the logits need the columns, too, where the other operand's are as much smaller.  With the product
+// that is left out a number counts as off by at most 2^-21 of itself or 2^-25 of its row's and of its column's largest.  Nor
+// may the tokens' own gradients (reduction none) lie further apart, since the rows of dZ have one scale: an entry of dZ
+// counts as off by at most 2^-21 of itself or 2^-49 of the largest |g| (half a step of a second plane, 2^-25 / 2^11 / 2^14,
+// and a second plane of up to 2^-25 / 2^14 times the other operand's of up to 2^-11).  Otherwise three bf16 planes (24
+// bits by truncation, exact, any range above 2^-110), six products.  A first pass over X and W finds which, on the
 // device.  The tensor core rounds its running sum towards zero, a bias that grows with K, so the fp32 kernels take the
 // accumulators out every 512 of K and add these runs up in registers; the products of the first planes have an accumulator
 // of their own, so that the small ones do not lose their low bits to it.  4099 x 8003 x 300, 12% ignored, forward +
@@ -174,7 +176,7 @@ __device__ __forceinline__ Split read_split(const unsigned *found) {
     if (f[0] != 0u && x_top == 0u) return s;
     if (f[2] != 0u && w_top == 0u) return s;
     if (!fits(x_top, x_low) || !fits(w_top, w_low)) return s;
-    // dZ's planes have one scale, too: a token's row is good to 2^-50 of the largest |g|
+    // dZ's planes have one scale, too: a token's row is good to 2^-49 of the largest |g|
     const unsigned g_top = f[kFoundGrad] >> 23, g_low = ~f[kFoundGrad + 1] >> 23;
     if (f[kFoundGrad] != 0u && (g_low == 0u || g_top - g_low > kSpread)) return s;
     s.half = true;

@@ -30,7 +30,7 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, lab
     boundaries are read where they lie, others are copied into the workspace first; fp32 operands are split there into
     two fp16 planes, or three bf16 planes where the sizes of rows, of columns or (reduction "none") of the tokens' gradients
     differ by more than 2^24, which keeps fp32 accuracy on the tensor cores, with two limits: numbers of an operand below
-    2^-110 keep fewer bits, and with two planes a logit's gradient is held to 2^-22 of itself or 2^-50 of the largest token's
+    2^-110 keep fewer bits, and with two planes a logit's gradient is held to 2^-21 of itself or 2^-49 of the largest token's
     gradient, so a row of d weight whose class has a probability far below 2^-28 for every token has few bits, or is zero.
     fp16: the latter bound is 2^-39.  For more than 256 tokens of bf16 or fp16 a logit's gradient is rounded to that type before the
     products.  Forward and backward may be captured into CUDA graphs.  Runs on the current stream of x's device;

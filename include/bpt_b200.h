@@ -520,8 +520,8 @@ int bpt_layer_norm_backward(const void *gy, const void *x, const void *r, const 
  * most 256 MB of logits' gradients.  Bitwise reproducible.
  *
  * fp32 operands run on the tensor cores as two fp16 planes, or as three bf16 planes where rows, columns or (NONE) the
- * tokens' gradients differ by more than 2^24 in size.  With two, an entry of the logits' gradient is held to 2^-22 of itself or
- * 2^-50 of the largest token's gradient (fp16 operands: half a step, or 2^-39).  NONE: a token's gradient that is not
+ * tokens' gradients differ by more than 2^24 in size.  With two, an entry of the logits' gradient is held to 2^-21 of itself or
+ * 2^-49 of the largest token's gradient (fp16 operands: half a step, or 2^-39).  NONE: a token's gradient that is not
  * finite spoils its row of dx and the sums over tokens, not the other rows.
  *
  * The workspace sizes depend on the operands' addresses too (operands that are not 16-byte aligned are copied).  Calls

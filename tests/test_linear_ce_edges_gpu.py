@@ -10,6 +10,11 @@ from test_linear_ce_gpu import DTYPES, IGNORE, check, formula, inputs, near
 
 pytestmark = pytest.mark.gpu
 
+# fp32 in two fp16 planes: an entry of dZ times 2^14 has a second plane times 2^11, whose smallest half step is 2^-25: 2^-50 of
+# dZ.  The product of second planes is left out: that of dZ is up to 2^-25 (where the first is at its smallest step), 2^-39
+# of dZ, and the other operand's up to 2^-11 of its numbers: 2^-50 again.
+FLOOR = 2.0 ** -49
+
 
 @pytest.mark.parametrize("down", [12, 40, 52, 90])
 @pytest.mark.parametrize("of", ["x", "w", "x up, w down"])
@@ -47,14 +52,14 @@ def off_by(x, w, t, most):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_tokens_of_very_different_weight(dtype, spread):
     """reduction none: weights from 1 to 2^-spread.  Each token's row of d x is as good as its own weight allows.  In fp32 an
-    entry of dZ may also be off by 2^-50 of the largest weight while no weight is below 2^-24 of it."""
+    entry of dZ may also be off by FLOOR of the largest weight while no weight is below 2^-24 of it."""
     x, w, b, t = inputs(300, 500, 72, dtype, padded=0.1)
     g = 2.0 ** -(torch.arange(300, device="cuda") % (spread + 1)).float()
     g[7] = 0.0
     leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
     linear_cross_entropy(*leaves[:2], t, bias=leaves[2], reduction="none").backward(g)
     want, off = formula(x, w, b, t, 0.0, "none", g)
-    more = off_by(x, w, t, 2.0 ** -50 if dtype == torch.float32 and spread <= 24 else 0.0)
+    more = off_by(x, w, t, FLOOR if dtype == torch.float32 and spread <= 24 else 0.0)
     for name, leaf, v, e, m in zip(("dx", "dw", "db"), leaves, want[1:], off[1:], more):
         near(leaf.grad, v, e + m, name)
 
@@ -186,7 +191,7 @@ def test_classes_masked_with_the_lowest_number(n, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_probabilities_of_very_different_size(dtype):
     """Classes whose probability is from 2^-4 down to 2^-60 for every token: rows of d w that are as small.  An entry of dZ is off by
-    the note's bound and, in fp32, by no more than 2^-50 beside it (in fp16 by 2^-39, which the formula has)."""
+    the note's bound and, in fp32, by no more than FLOOR beside it (in fp16 by 2^-39, which the formula has)."""
     for n in (300, 90):
         x, w, b, t = inputs(n, 600, 72, dtype, spread=0.3)
         b = (b.float() - 0.6931 * (torch.arange(600, device="cuda") % 60)).to(dtype)
@@ -197,7 +202,7 @@ def test_probabilities_of_very_different_size(dtype):
         want, off = formula(x, w, b, t, 0.0, "sum", torch.ones((), device="cuda"))
         p = torch.softmax(x.double() @ w.double().t() + b.double(), 1)
         assert float(p.max()) > 2.0 ** -5 and float(p.min()) < 2.0 ** -60
-        more = off_by(x, w, t, 2.0 ** -50 if dtype == torch.float32 else 0.0)
+        more = off_by(x, w, t, FLOOR if dtype == torch.float32 else 0.0)
         for name, leaf, v, e, m in zip(("dx", "dw", "db"), leaves, want[1:], off[1:], more):
             near(leaf.grad, v, e + m, name)
 
